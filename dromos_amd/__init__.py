@@ -14,12 +14,16 @@ from .abi import (  # noqa: F401
     MATH_FP4,
     MATH_FP8,
     MATH_INT8,
+    NORM_LAYER,
+    NORM_RMS,
     NOT_SUPPORTED,
     W_BF16,
     W_FP8,
     W_INT8,
     W_NVFP4,
     Kernels,
+    LxKv8,
+    LxKv8Batch,
     LxWeight,
     hip_library_path,
     load_hip,

@@ -21,6 +21,7 @@ F32, BF16 = 0, 1
 DTYPE = {torch.float32: F32, torch.bfloat16: BF16}
 W_BF16, W_INT8, W_FP8, W_NVFP4, W_BF16X = 0, 1, 2, 3, 4
 MATH_BF16, MATH_INT8, MATH_FP8, MATH_FP4 = 0, 1, 2, 3
+NORM_RMS, NORM_LAYER = 0, 1
 NOT_SUPPORTED = 801
 FORMATS = {"bf16": W_BF16, "int8": W_INT8, "fp8": W_FP8, "nvfp4": W_NVFP4}
 
@@ -37,6 +38,37 @@ class LxWeight(ctypes.Structure):
         ("scale", ctypes.c_void_p),
         ("global_", ctypes.c_float),
         ("expert_global", ctypes.c_void_p),
+    ]
+
+
+class LxKv8(ctypes.Structure):
+    """lx_kv8 (include/dromos_hip.h): a paged cache of 8-bit keys and values."""
+
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("pages", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("page", ctypes.c_int),
+        ("block", ctypes.c_int),
+        ("dim", ctypes.c_int),
+    ]
+
+
+class LxKv8Batch(ctypes.Structure):
+    """lx_kv8_batch (include/dromos_hip.h): the rows of one call and where their sequences' tokens lie."""
+
+    _fields_ = [
+        ("seqs", ctypes.c_int),
+        ("rows", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("ld_table", ctypes.c_int),
+        ("max_rows", ctypes.c_int),
+        ("max_length", ctypes.c_int),
     ]
 
 

@@ -296,6 +296,33 @@ __device__ __forceinline__ float weight_element(int type, const void* data, cons
   }
 }
 
+// f32 -> e4m3fn, nearest even, saturating at 448, NaN -> 0x7f with the sign (engine/cpu/quant.cpp:20-39).
+__device__ __forceinline__ uint32_t e4m3_encode(float f) {
+  uint32_t u = __float_as_uint(f);
+  const uint32_t sign = (u >> 24) & 0x80u;
+  u &= 0x7fffffffu;
+  if (u > 0x7f800000u) return sign | 0x7fu;
+  const float a = __uint_as_float(u);
+  if (a >= 448.0f) return sign | 0x7eu;
+  if (a < 0x1p-6f) return sign | static_cast<uint32_t>(static_cast<int>(rintf(a * 512.0f)));
+  u += 0x7ffffu + ((u >> 20) & 1u);
+  const int e = static_cast<int>(u >> 23) - 127 + 7;
+  const uint32_t m = (u >> 20) & 7u;
+  if (e > 15 || (e == 15 && m == 7u)) return sign | 0x7eu;
+  return sign | (static_cast<uint32_t>(e) << 3) | m;
+}
+
+// Four e4m3_encode()s as a dword by the conversion instruction, which does not saturate by itself and gives every NaN one sign.
+// Equal to e4m3_encode() on all 2^32 arguments.
+__device__ __forceinline__ uint32_t e4m3_encode_four(const float* v) {
+  const float sum = (v[0] + v[1]) + (v[2] + v[3]);
+  if (__builtin_expect(sum != sum, 0)) return e4m3_encode(v[0]) | e4m3_encode(v[1]) << 8 | e4m3_encode(v[2]) << 16 | e4m3_encode(v[3]) << 24;
+  float c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c[j] = fminf(fmaxf(v[j], -448.0f), 448.0f);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false), true);
+}
+
 // silu as the reference's CPU computes it (engine/cpu/cpu.h:68), with the device's exp.
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 

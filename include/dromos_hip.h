@@ -226,6 +226,83 @@ LX_API int lx_gemm_bf16(const void* x, int ld_x, const void* w, const void* bias
 LX_API int lx_moe_experts_noalloc(const void* latent, const int32_t* ids, const float* weights, const void* gate_up,
                                   const void* down, float* out, int T, int L, int I, int top_k, void* stream);
 
+/* ---- an attention layer's step between its products (no counterpart in the reference's headers: these are this library's own) ------
+ * x = lx_block_norm(...); qkv = lx_gemm_w(x); lx_kv8_append(qkv); lx_kv8_attention(q); lx_gemm_w(o); lx_block_norm(...)
+ *
+ * A cache of keys and values in pages, eight bits a value, one scale per block of `block` tokens and head (host structs, device
+ * pointers; the caller owns all of it):
+ *   k, v              codes [pages, heads, page, dim], 16-byte aligned: int8 (LX_W_INT8) or e4m3fn (LX_W_FP8)
+ *   k_scale, v_scale  f32 [pages, heads, page / block]                           value = code * scale
+ *   dim 64, 128, 192 or 256; block 16, 32, 64 or 128; page a multiple of block, at most 4096; pages * heads * page < 2^34
+ * The rows of one call:
+ *   rows     [seqs + 1] sequence s has the rows rows[s] .. rows[s + 1] - 1 of the call (ascending, from 0 on, to T at most: rows behind
+ *            the last sequence belong to nobody and stay as they were); null: one row a sequence, row s
+ *   lengths  [seqs] tokens of each sequence in the cache, this call's rows (its last ones) among them; 0 is fine
+ *   table    [seqs, ld_table] page number of the tokens [i * page, (i + 1) * page) of a sequence
+ *   max_rows, max_length   at least the most rows and the greatest length of any sequence (rows and tokens beyond them are not attended
+ *            to). They and T size the launch: a captured call replays with whatever rows, lengths and table hold then, within them.
+ * The numbers in device memory are not refused but bounded: a page number outside [0, pages) is a page without tokens (nothing is
+ * stored, nothing attended), rows end at T, lengths at max_length and at the table's end; a row in front of position 0 is not
+ * stored and attends to nothing.
+ *
+ * lx_kv8_append: row i of a sequence of n rows and length L is its token p = L - n + i. k and v [T, heads * dim] and q [T, q_heads * dim]
+ * (q may be null, then q_out is too), all f32 or all bf16, row strides in elements; q_out f32 or bf16, q itself allowed where type
+ * and stride agree.
+ *   rotation   the first `rot` values of a head (a multiple of 8, 0 for none) of q and k, by the angles p * freq[i], i < rot / 2 (freq
+ *              f32 on the device; the angles are formed and reduced in 64 bits, so far positions lose nothing): pairs (i, i + rot / 2),
+ *              or (2 i, 2 i + 1) where `interleaved`; (a, b) -> (a cos - b sin, b cos + a sin). v is stored unrotated.
+ *   codes      per block and head, keys and values apart, qmax 127 or 448: s = max(|finite values of this call in the block|) / qmax, and at
+ *              least the scale the block has while tokens of it in front of this call's stay; code = rne(x * (1 / s)), clamped to +-qmax
+ *              (infinities too; a NaN is e4m3's NaN, and 0 in int8). Where s grew, the codes that stay become rne(code * (s_old / s)).
+ *              A block of zeros has scale 0. Codes of places behind the sequence's last token stay as they were.
+ * A block may be written by one sequence of a call only; pages that sequences share are read by all of them.
+ *
+ * lx_kv8_dequantize: the whole cache back as bf16 [pages, heads, page, dim] (either output may be null).
+ *
+ * lx_kv8_attention: out[row, h] = sum_t softmax_t(scale * q[row, h] . k[t]) v[t] over the tokens p - window < t <= p of the row's own
+ * sequence (window 0: all up to p), p as above; query head h reads the cache's head h / (q_heads / heads). Rows without a token are 0.
+ * q f32 (rounded to bf16, as lx_gemm_w's BF16 math does) or bf16, out f32 or bf16, row strides in elements; products on the matrix
+ * cores, sums and softmax in f32, one pass over the keys. Contents of the cache where no token lies (NaNs too) have no
+ * part in it. The workspace (lx_kv8_attention_workspace_bytes for the same cache, batch, T and q_heads; 0: none, may be null) holds
+ * partial sums of long sequences, may hold garbage, and belongs to one call at a time. */
+typedef struct {
+  lx_wtype type;
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int pages, heads, page, block, dim;
+} lx_kv8;
+typedef struct {
+  int seqs;
+  const int32_t* rows;
+  const int32_t* lengths;
+  const int32_t* table;
+  int ld_table;
+  int max_rows, max_length;
+} lx_kv8_batch;
+LX_API int lx_kv8_append(const lx_kv8* cache, const lx_kv8_batch* batch, const void* q, const void* k, const void* v, lx_dtype dtype,
+                         int ld_q, int ld_k, int ld_v, void* q_out, lx_dtype q_out_dtype, int ld_q_out, const float* freq, int rot,
+                         int interleaved, int T, int q_heads, void* stream);
+LX_API int lx_kv8_dequantize(const lx_kv8* cache, void* k, void* v, void* stream);
+LX_API int lx_kv8_attention(const void* q, lx_dtype q_dtype, int ld_q, const lx_kv8* cache, const lx_kv8_batch* batch, void* out,
+                            lx_dtype out_dtype, int ld_out, int T, int q_heads, float scale, int window, void* workspace, void* stream);
+LX_API int64_t lx_kv8_attention_workspace_bytes(const lx_kv8* cache, const lx_kv8_batch* batch, int T, int q_heads);
+/* lx_block_norm: from a block's output to the next block's input, one row [H] at a time, H <= 32768:
+ *   r = norm(y) * post_weight (+ post_bias)      or y itself where post_weight is null
+ *   h_out = beta * h + alpha * gate * r          gate [T, H] in y's type, ld_gate 0: one row for all; null: 1
+ *   x = norm(h_out) * weight (+ bias)            of the sum before it is rounded to h's type; null weight: no norm and no x
+ * With y null there is no block yet: x = norm(h), and post_weight, gate and h_out are not used (h_out may be null).
+ * norm: LX_NORM_RMS v / sqrt(mean(v^2) + eps), LX_NORM_LAYER (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps), sums in f32 and in a
+ * fixed order. y, h (and h_out, which may be h) and x f32 or bf16 each; weights and biases in w_dtype, biases may be null. x may be y where
+ * type and stride agree; nothing else may overlap.
+ * beta 0: h is not read and may be null. */
+typedef enum { LX_NORM_RMS = 0, LX_NORM_LAYER = 1 } lx_norm;
+LX_API int lx_block_norm(lx_norm norm, const void* y, lx_dtype y_dtype, int ld_y, const void* post_weight, const void* post_bias,
+                         const void* gate, int ld_gate, float alpha, float beta, const void* h, void* h_out, lx_dtype h_dtype, int ld_h,
+                         const void* weight, const void* bias, lx_dtype w_dtype, void* x, lx_dtype x_dtype, int ld_x, float eps, int T,
+                         int H, void* stream);
+
 /* ---- runtime (replaces engine/cuda/kernels.h:308-381 on the HIP runtime) --------------------------- */
 typedef struct {
   char name[256];

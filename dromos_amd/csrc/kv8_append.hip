@@ -124,21 +124,22 @@ __device__ __forceinline__ float top_of(const float* v, float top) {
   return top;
 }
 
-// Four codes as a dword.
+// Four codes as a dword. A NaN becomes 0: a code that is no number would reach rows that do not see its token, as nothing
+// times a NaN on the matrix cores.
 template <int F>
 __device__ __forceinline__ uint32_t encode_four(const float* v, float inverse) {
   float c[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) c[j] = v[j] * inverse;
+  for (int j = 0; j < 4; ++j) {
+    c[j] = v[j] * inverse;
+    c[j] = c[j] == c[j] ? c[j] : 0.0f;
+  }
   if constexpr (F == LX_W_FP8) {
     return e4m3_encode_four(c);
   } else {
     uint32_t d = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int code = c[j] == c[j] ? static_cast<int>(fminf(fmaxf(rintf(c[j]), -127.0f), 127.0f)) : 0;
-      d |= (static_cast<uint32_t>(code) & 0xffu) << (8 * j);
-    }
+    for (int j = 0; j < 4; ++j) d |= (static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(c[j]), -127.0f), 127.0f))) & 0xffu) << (8 * j);
     return d;
   }
 }

@@ -1,0 +1,459 @@
+// lx_kv8_attention for few rows a sequence: the cache is streamed once, so its bytes decide.
+//
+// Mathematics. o = sum_t w_t v_t / sum_t w_t with w_t = 2^(c_t - m), c_t = (q . k_t) * scale * log2 e, m the largest c so far:
+// one pass over the keys, sums and values rescaled by 2^(m_old - m_new) where a larger score comes. Scores are taken the other
+// way round, S^T = K Q^T, sixteen keys (A) by sixteen rows (B): a lane then holds the scores of one row (lane % 16) and four
+// keys, which is the layout in which O^T = V^T P^T wants its B operand, so weights never change lanes, and a row's
+// rescaling is its lanes' own. The matrix instruction sums over k in any order that both operands agree on: keys are read 16
+// bytes a lane as they lie, and a lane's slots of a sum over tokens are the four of one run of 16 and the four of the next
+// that it holds weights of. Values are read DIM / 16 bytes a lane and token (16 lanes a row) and transposed by bytes in
+// registers, two permutations for four tokens' pairs. Key codes become bf16 exactly, as the queries are; value codes become
+// f16 exactly. A key block's scale multiplies its scores, a value block's its weights, both f32, and the product is rounded to
+// f16 for the matrix cores: three more bits than bf16, so the roundings of the weights (2^-11 of each term) stay well below
+// the result's own. f16's range is made enough: scales are taken relative to the part's largest one, and weights times 2^15,
+// so that the largest is 2^15 and one 2^-29 of it is still a normal number. The sum of weights is f32.
+//
+// Split. A workgroup takes one sequence, 16 RT rows of one of the cache's heads (rows of a head: its tokens' query heads,
+// token after token) and up to kMaxRuns runs of 16 tokens of it. Its four wavefronts take 64 tokens at a time in turn (32 of heads wider than 128) and keep
+// sums of their own; the workgroup adds them up at its end, in order. Where a sequence has several such parts they leave
+// their sums in the workspace, and a second kernel adds those, in order.
+#pragma once
+
+#include "kv8.h"
+#include "tile_mfma.h"
+
+namespace dro {
+
+constexpr int kStreamWaves = 4;
+constexpr int kMaxRuns = 256;  // runs of 16 tokens a workgroup takes at most
+
+// Runs a wavefront takes at a time: four, or two where four runs' codes and the sums (DIM * RT / 4 registers) would not fit
+// the 256 registers that two wavefronts a SIMD leave each.
+template <int DIM>
+constexpr int step_runs() {
+  return DIM <= 128 ? 4 : 2;
+}
+
+struct AttentionArgs {
+  Kv8Cache c;
+  Kv8Batch b;
+  const void* q;
+  void* out;
+  float* partial;
+  int64_t ld_q, ld_out;
+  int q_dtype, out_dtype, group, window;
+  float scale;
+  int wide_q;                    // q is bf16 and can be read 16 bytes at a time
+  int row_tiles, splits, chunk;  // chunk: tokens of a part, a multiple of 256, 16 * kMaxRuns at most
+};
+
+// What one tile of rows of a sequence attends to.
+struct RowTile {
+  Kv8Span span;
+  int first, count;      // flat rows (token * group + query head) of the tile
+  int low_pos, high_pos; // positions of its first and last row
+  int begin, end;        // tokens that any of its rows sees: begin is a multiple of 16; begin >= end: none
+};
+
+__device__ __forceinline__ RowTile row_tile(const AttentionArgs& p, int seq, int tile, int per_tile) {
+  RowTile t;
+  t.span = kv8_span(p.b, p.c.page, seq);
+  const int rows = min(t.span.rows, p.b.max_rows) * p.group;
+  t.first = tile * per_tile;
+  t.count = min(rows - t.first, per_tile);
+  const int lead = t.span.length - t.span.rows;
+  t.low_pos = lead + t.first / p.group;
+  t.high_pos = lead + (t.first + max(t.count, 1) - 1) / p.group;
+  t.end = t.count > 0 ? t.high_pos + 1 : 0;
+  const int64_t first_seen = p.window > 0 ? static_cast<int64_t>(t.low_pos) - p.window + 1 : 0;
+  t.begin = first_seen > 0 ? static_cast<int>(first_seen) & ~(kRun - 1) : 0;
+  return t;
+}
+
+// Where a partial sum lies: 16 RT rows of DIM sums, then a row's largest score and sum of weights.
+template <int DIM>
+__device__ __forceinline__ float* partial_at(const AttentionArgs& p, int64_t item, int split, int per_tile) {
+  return p.partial + (item * p.splits + split) * per_tile * (DIM + 2);
+}
+
+// The bytes of a run's key rows that a lane holds: 16 at 16 g of every 64, and its values': DIM / 16 of four tokens.
+template <int DIM>
+struct KeyRegs {
+  u32x4 w[DIM / 64];
+};
+template <int DIM>
+struct ValueRegs {
+  uint32_t w[4][DIM / 64];
+};
+
+template <int DIM>
+__device__ __forceinline__ void load_keys(KeyRegs<DIM>& r, const uint8_t* run, int lane_off) {
+#pragma unroll
+  for (int c = 0; c < DIM / 64; ++c) r.w[c] = *reinterpret_cast<const u32x4*>(run + lane_off + 64 * c);
+}
+
+template <int DIM>
+__device__ __forceinline__ void load_values(ValueRegs<DIM>& r, const uint8_t* run, int lane_off) {
+  typedef uint32_t vec __attribute__((ext_vector_type(DIM / 64 == 3 ? 3 : DIM / 64), aligned(4)));
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if constexpr (DIM == 64) {
+      r.w[t][0] = *reinterpret_cast<const uint32_t*>(run + lane_off + t * DIM);
+    } else {
+      const vec v = *reinterpret_cast<const vec*>(run + lane_off + t * DIM);
+#pragma unroll
+      for (int j = 0; j < DIM / 64; ++j) r.w[t][j] = v[j];
+    }
+  }
+}
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// Two neighbouring codes of a dword (the low or the high pair) as f16. An int8 code with its top bit flipped is code + 128; as
+// the low byte under 0x64 it is the half 1024 + 128 + code.
+template <int F, bool HIGH>
+__device__ __forceinline__ f16x2 pair_of(uint32_t d) {
+  if constexpr (F == LX_W_FP8) {
+    return __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d, 1.0f, HIGH));
+  } else {
+    const uint32_t h = __builtin_amdgcn_perm(0x64646464u, d, HIGH ? 0x04030402u : 0x04010400u);
+    return __builtin_bit_cast(f16x2, h) - f16x2{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+  }
+}
+
+// The bytes of value codes as pair_of takes them.
+template <int F>
+__device__ __forceinline__ uint32_t flipped(uint32_t d) {
+  return F == LX_W_INT8 ? d ^ 0x80808080u : d;
+}
+
+__device__ __forceinline__ f16x2 pack_f16(float a, float b) { return f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)}; }
+
+constexpr float kWeightBits = 15.0f;  // weights are held times 2^15
+
+// Eight consecutive values of a query as the matrix instruction's operand; f32 ones are rounded to bf16 here.
+__device__ __forceinline__ bf16x8 query_fragment(const AttentionArgs& p, bool have, int64_t at) {
+  if (!have) return __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+  if (p.wide_q) return *reinterpret_cast<const bf16x8*>(static_cast<const uint16_t*>(p.q) + at);
+  bf16x2 v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = pack_bf16(load_as_f32(p.q, p.q_dtype, at + 2 * j), load_as_f32(p.q, p.q_dtype, at + 2 * j + 1));
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+template <int F, int DIM, int RT>
+__global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
+  constexpr int kC = DIM / 64, kTiles = DIM / 16, kPerTile = 16 * RT, kRuns = step_runs<DIM>(), kStep = kRuns * kRun;
+  __shared__ int run_of[kMaxRuns];
+  __shared__ float key_scale[kMaxRuns], value_scale[kMaxRuns];
+  __shared__ float wave_top[kStreamWaves][kPerTile], wave_sum_of[kStreamWaves][kPerTile];
+  __shared__ float sums[kStreamWaves][16][DIM + 4];
+  __shared__ float scale_top[kStreamWaves];
+  __shared__ int holes;
+  const Kv8Cache& c = p.c;
+  const int head = blockIdx.x % c.heads;
+  int64_t rest = blockIdx.x / c.heads;
+  const int split = static_cast<int>(rest % p.splits);
+  rest /= p.splits;
+  const int tile = static_cast<int>(rest % p.row_tiles), seq = static_cast<int>(rest / p.row_tiles);
+  const RowTile t = row_tile(p, seq, tile, kPerTile);
+  if (t.count <= 0) return;
+  const int64_t start = t.begin + static_cast<int64_t>(split) * p.chunk;
+  if (start >= t.end && split > 0) return;
+  const bool alone = static_cast<int64_t>(t.begin) + p.chunk >= t.end;  // the only part: the rows are written at once
+  const int token0 = static_cast<int>(start), stop = static_cast<int>(min(start + p.chunk, static_cast<int64_t>(t.end)));
+  const int runs = (stop - token0 + kRun - 1) / kRun;  // none where the rows see nothing
+
+  // Where the part's runs lie (-1: no page, no tokens), and their scales.
+  const int lane = threadIdx.x % kWave, g = lane / 16, i = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (threadIdx.x == 0) holes = 0;
+  __syncthreads();
+  float largest = 0.0f;
+  for (int e = threadIdx.x; e < runs; e += 256) {
+    const int token = token0 + kRun * e, page = kv8_page(c, p.b, seq, token);
+    float ks = 0.0f, vs = 0.0f;
+    int run = -1;
+    if (page >= 0) {
+      const int64_t at = kv8_row(c, page, head) + token % c.page;
+      run = static_cast<int>(at / kRun);
+      ks = c.k_scale[at >> c.block_shift] * p.scale * 1.4426950408889634f;
+      vs = c.v_scale[at >> c.block_shift];
+    } else {
+      holes = 1;
+    }
+    run_of[e] = run;
+    key_scale[e] = ks;
+    value_scale[e] = vs;
+    largest = fmaxf(largest, fabsf(vs));
+  }
+  largest = wave_max(largest);
+  if (lane == 0) scale_top[wave] = largest;
+  __syncthreads();
+  const bool whole = !holes;
+  largest = fmaxf(fmaxf(scale_top[0], scale_top[1]), fmaxf(scale_top[2], scale_top[3]));
+  const float per_largest = largest > 0.0f ? 1.0f / largest : 0.0f;
+
+  // The rows' queries: row 16 r + i, dims 64 c + 16 g + 8 h .. + 8 (the key's bytes of the same lane group).
+  bf16x8 q[RT][kC][2];
+  int pos[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int flat = t.first + 16 * r + i, token = flat / p.group;
+    const bool have = 16 * r + i < t.count;
+    pos[r] = t.span.length - t.span.rows + token;
+    const int64_t at = have ? (t.span.row0 + token) * p.ld_q + static_cast<int64_t>(head * p.group + flat % p.group) * DIM : 0;
+#pragma unroll
+    for (int cc = 0; cc < kC; ++cc)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        q[r][cc][h] = query_fragment(p, have, at + 64 * cc + 16 * g + 8 * h);
+      }
+  }
+
+  f32x4 acc[RT][kTiles] = {};
+  float top[RT], total[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    top[r] = -__builtin_inff();
+    total[r] = 0.0f;
+  }
+  const int steps = (runs + kRuns - 1) / kRuns;
+  const int key_off = i * DIM + 16 * g, value_off = 4 * g * DIM + i * (DIM / 16);
+  KeyRegs<DIM> keys[kRuns];
+  ValueRegs<DIM> values[kRuns];
+  auto run_base = [&](int step, int j) {
+    const int at = min(step * kRuns + j, runs - 1);
+    return static_cast<int64_t>(max(__builtin_amdgcn_readfirstlane(run_of[at]), 0)) * (kRun * DIM);
+  };
+  auto ask_keys = [&](int step) {
+#pragma unroll
+    for (int j = 0; j < kRuns; ++j) load_keys<DIM>(keys[j], c.k + run_base(step, j), key_off);
+  };
+  auto ask_values = [&](int step) {
+#pragma unroll
+    for (int j = 0; j < kRuns; ++j) load_values<DIM>(values[j], c.v + run_base(step, j), value_off);
+  };
+  if (wave < steps) {
+    ask_keys(wave);
+    ask_values(wave);
+  }
+  for (int step = wave; step < steps; step += kStreamWaves) {
+    const int at = token0 + step * kStep;
+    f32x4 s[RT][kRuns];
+#pragma unroll
+    for (int j = 0; j < kRuns; ++j) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int cc = 0; cc < kC; ++cc)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bf16x8 a = weight_fragment<F>(keys[j].w[cc], 0, h);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) s[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[r][cc][h], s[r][j], 0, 0, 0);
+        }
+    }
+    const bool more = step + kStreamWaves < steps;
+    if (more) ask_keys(step + kStreamWaves);
+    // Every token of the step is seen by every row?
+    const bool plain = whole && at + kStep - 1 <= t.low_pos && (p.window == 0 || at > t.high_pos - p.window);
+    float vs[kRuns];
+#pragma unroll
+    for (int j = 0; j < kRuns; ++j) {
+      const int run = min(step * kRuns + j, runs - 1);
+      const float ks = key_scale[run];
+      vs[j] = value_scale[run] * per_largest;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s[r][j] *= ks;
+    }
+    if (!plain) {
+#pragma unroll
+      for (int j = 0; j < kRuns; ++j) {
+        const bool there = step * kRuns + j < runs && run_of[min(step * kRuns + j, runs - 1)] >= 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int token = at + kRun * j + 4 * g + e;
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            if (!there || token > pos[r] || (p.window > 0 && token <= pos[r] - p.window)) s[r][j][e] = -__builtin_inff();
+          // Codes of places without a token (NaNs perhaps) times a weight of nothing have to be nothing.
+          if (!there || token >= t.span.length)
+#pragma unroll
+            for (int d = 0; d < kC; ++d) values[j].w[e][d] = 0;
+        }
+      }
+    }
+    f16x8 weights[RT][kRuns / 2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float m = s[r][0][0];
+#pragma unroll
+      for (int j = 0; j < kRuns; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, s[r][j][e]);
+      float a, b;
+      swap_halves<true>(m, a, b);
+      m = fmaxf(a, b);
+      swap_halves<false>(m, a, b);
+      m = fmaxf(top[r], fmaxf(a, b));
+      const float base = m == -__builtin_inff() ? 0.0f : m;
+      const float keep = __builtin_amdgcn_exp2f(top[r] - base);
+      if (__any(m != top[r])) {
+#pragma unroll
+        for (int f = 0; f < kTiles; ++f) acc[r][f] *= keep;
+        total[r] *= keep;
+      }
+      top[r] = m;
+      const float lifted = base - kWeightBits;
+#pragma unroll
+      for (int j = 0; j < kRuns; j += 2) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_amdgcn_exp2f(s[r][j + e / 4][e % 4] - lifted);
+          total[r] += x;
+          w[e] = x * vs[j + e / 4];
+        }
+        const f16x2 v[4] = {pack_f16(w[0], w[1]), pack_f16(w[2], w[3]), pack_f16(w[4], w[5]), pack_f16(w[6], w[7])};
+        weights[r][j / 2] = __builtin_bit_cast(f16x8, v);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kRuns; j += 2)
+#pragma unroll
+      for (int d = 0; d < kC; ++d) {
+        // Dword d of the eight tokens' bytes: [pair of tokens][low, high two dims]
+        uint32_t two[4][2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t x = flipped<F>(values[j + e / 2].w[2 * (e % 2)][d]), y = flipped<F>(values[j + e / 2].w[2 * (e % 2) + 1][d]);
+          two[e][0] = __builtin_amdgcn_perm(y, x, 0x05010400u);
+          two[e][1] = __builtin_amdgcn_perm(y, x, 0x07030602u);
+        }
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          f16x2 v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = f % 2 ? pair_of<F, true>(two[e][f / 2]) : pair_of<F, false>(two[e][f / 2]);
+          const f16x8 a = __builtin_bit_cast(f16x8, v);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) acc[r][4 * d + f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, weights[r][j / 2], acc[r][4 * d + f], 0, 0, 0);
+        }
+      }
+    if (more) ask_values(step + kStreamWaves);
+  }
+
+  // The wavefronts' sums together.
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    float a, b;
+    swap_halves<true>(total[r], a, b);
+    const float w = a + b;
+    swap_halves<false>(w, a, b);
+    if (g == 0) {
+      wave_top[wave][16 * r + i] = top[r];
+      wave_sum_of[wave][16 * r + i] = a + b;
+    }
+  }
+  __syncthreads();
+  float* const part = alone ? nullptr : partial_at<DIM>(p, (static_cast<int64_t>(seq) * p.row_tiles + tile) * c.heads + head, split, kPerTile);
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    if (16 * r >= t.count) break;
+    const int row = 16 * r + i;
+    const float m = fmaxf(fmaxf(wave_top[0][row], wave_top[1][row]), fmaxf(wave_top[2][row], wave_top[3][row]));
+    const float keep = top[r] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top[r] - m) * largest;
+    if (r > 0) __syncthreads();
+    // Tile f of a lane: dims kTiles * (4 g + e) + f.
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int f = 0; f < kTiles; f += 4) {
+        f32x4 v = {acc[r][f][e], acc[r][f + 1][e], acc[r][f + 2][e], acc[r][f + 3][e]};
+        *reinterpret_cast<f32x4*>(&sums[wave][i][kTiles * (4 * g + e) + f]) = v * keep;
+      }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * (DIM / 4); e += 256) {
+      const int local = e / (DIM / 4), d = 4 * (e % (DIM / 4)), row = 16 * r + local;
+      if (row >= t.count) continue;
+      const float m = fmaxf(fmaxf(wave_top[0][row], wave_top[1][row]), fmaxf(wave_top[2][row], wave_top[3][row]));
+      float sum = 0.0f;
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kStreamWaves; ++w) {
+        const float keep = wave_top[w][row] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(wave_top[w][row] - m);
+        sum += wave_sum_of[w][row] * keep;
+        v += *reinterpret_cast<const f32x4*>(&sums[w][local][d]);
+      }
+      if (alone) {
+        const int flat = t.first + row;
+        const int64_t at = (t.span.row0 + flat / p.group) * p.ld_out + static_cast<int64_t>(head * p.group + flat % p.group) * DIM + d;
+        const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) store_from_f32(p.out, p.out_dtype, at + k, v[k] * inverse);
+      } else {
+        *reinterpret_cast<f32x4*>(part + row * DIM + d) = v;
+        if (d == 0) {
+          part[kPerTile * DIM + 2 * row] = m;
+          part[kPerTile * DIM + 2 * row + 1] = sum;
+        }
+      }
+    }
+  }
+}
+
+// The parts of one row added up. A workgroup takes a row of one of the cache's heads: every thread looks at some parts' largest
+// scores, then 1024 / DIM groups of DIM / 4 threads add up every so-manieth part each, and the groups' sums are added, all in a
+// fixed order. (One thread after another over all parts took 35 us of 57 for 64 of them.)
+template <int DIM>
+__global__ void __launch_bounds__(256) combine_kernel(const AttentionArgs p, int per_tile, int rows) {
+  constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
+  __shared__ float tops[4], sums_of[4];
+  __shared__ f32x4 sums[kGroups][kLanes];
+  const Kv8Cache& c = p.c;
+  const int row = blockIdx.x % rows;
+  const int64_t item = blockIdx.x / rows;
+  const int head = static_cast<int>(item % c.heads), tile = static_cast<int>(item / c.heads % p.row_tiles),
+            seq = static_cast<int>(item / c.heads / p.row_tiles);
+  const RowTile t = row_tile(p, seq, tile, per_tile);
+  if (row >= t.count || static_cast<int64_t>(t.begin) + p.chunk >= t.end) return;
+  const int parts = (t.end - t.begin + p.chunk - 1) / p.chunk;
+  const float* const first = partial_at<DIM>(p, item, 0, per_tile);
+  const int64_t pitch = static_cast<int64_t>(per_tile) * (DIM + 2);
+  const float* const marks = first + per_tile * DIM + 2 * row;  // largest score, sum of weights
+  const int wave = threadIdx.x / kWave;
+  float m = -__builtin_inff();
+  for (int s = threadIdx.x; s < parts; s += 256) m = fmaxf(m, marks[s * pitch]);
+  m = wave_max(m);
+  if (threadIdx.x % kWave == 0) tops[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const float base = m == -__builtin_inff() ? 0.0f : m;
+  float sum = 0.0f;
+  for (int s = threadIdx.x; s < parts; s += 256) sum += marks[s * pitch + 1] * __builtin_amdgcn_exp2f(marks[s * pitch] - base);
+  sum = wave_sum(sum);
+  if (threadIdx.x % kWave == 0) sums_of[wave] = sum;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (group < kGroups) {
+#pragma unroll 4
+    for (int s = group; s < parts; s += kGroups)
+      v += *reinterpret_cast<const f32x4*>(first + s * pitch + row * DIM + 4 * lane) * __builtin_amdgcn_exp2f(marks[s * pitch] - base);
+    sums[group][lane] = v;
+  }
+  __syncthreads();
+  if (group > 0) return;
+  v = sums[0][lane];
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g) v += sums[g][lane];
+  sum = sums_of[0] + sums_of[1] + sums_of[2] + sums_of[3];
+  const int flat = t.first + row;
+  const int64_t at = (t.span.row0 + flat / p.group) * p.ld_out + static_cast<int64_t>(head * p.group + flat % p.group) * DIM + 4 * lane;
+  const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) store_from_f32(p.out, p.out_dtype, at + k, v[k] * inverse);
+}
+
+}  // namespace dro

@@ -253,7 +253,7 @@ LX_API int lx_moe_experts_noalloc(const void* latent, const int32_t* ids, const 
  *              or (2 i, 2 i + 1) where `interleaved`; (a, b) -> (a cos - b sin, b cos + a sin). v is stored unrotated.
  *   codes      per block and head, keys and values apart, qmax 127 or 448: s = max(|finite values of this call in the block|) / qmax, and at
  *              least the scale the block has while tokens of it in front of this call's stay; code = rne(x * (1 / s)), clamped to +-qmax
- *              (infinities too; a NaN is e4m3's NaN, and 0 in int8). Where s grew, the codes that stay become rne(code * (s_old / s)).
+ *              (infinities too; a NaN is 0). Where s grew, the codes that stay become rne(code * (s_old / s)).
  *              A block of zeros has scale 0. Codes of places behind the sequence's last token stay as they were.
  * A block may be written by one sequence of a call only; pages that sequences share are read by all of them.
  *
@@ -262,8 +262,8 @@ LX_API int lx_moe_experts_noalloc(const void* latent, const int32_t* ids, const 
  * lx_kv8_attention: out[row, h] = sum_t softmax_t(scale * q[row, h] . k[t]) v[t] over the tokens p - window < t <= p of the row's own
  * sequence (window 0: all up to p), p as above; query head h reads the cache's head h / (q_heads / heads). Rows without a token are 0.
  * q f32 (rounded to bf16, as lx_gemm_w's BF16 math does) or bf16, out f32 or bf16, row strides in elements; products on the matrix
- * cores, sums and softmax in f32, one pass over the keys. Contents of the cache where no token lies (NaNs too) have no
- * part in it. The workspace (lx_kv8_attention_workspace_bytes for the same cache, batch, T and q_heads; 0: none, may be null) holds
+ * cores (weights rounded to f16), sums and softmax in f32, one pass over the keys. Contents of the cache where no token lies (NaNs too) have no
+ * part in it; where one lies its codes and scales are numbers, as lx_kv8_append writes them. The workspace (lx_kv8_attention_workspace_bytes for the same cache, batch, T and q_heads; 0: none, may be null) holds
  * partial sums of long sequences, may hold garbage, and belongs to one call at a time. */
 typedef struct {
   lx_wtype type;

@@ -170,7 +170,7 @@ def attended(q, cache, batch, q_heads, scale, window=0):
 
 
 def check_attention(got, q, cache, batch, q_heads, scale, window=0, rows=None):
-    """The weights are rounded to bf16 (half a step, 2^-8 of each); a score is an f32 sum of dim products, off by dim 2^-24
+    """The weights are rounded to f16 (half a step, 2^-11 of each, and one under 2^-29 of the row's largest perhaps to nothing); a score is an f32 sum of dim products, off by dim 2^-24
     of the sum of their magnitudes, and its exponential by as much relatively, in the weight and in the sum it is divided by;
     2^-20 covers the exponentials, the scales and the division; the result is rounded once to its type. A weight under 2^-126
     of the row's largest is no f32 number any more (a value of 1.5e-58 cannot come back): 2^17 tokens of such weights and
@@ -178,7 +178,8 @@ def check_attention(got, q, cache, batch, q_heads, scale, window=0, rows=None):
     out, spread, size = attended(q, cache, batch, q_heads, scale, window)
     half = torch.finfo(got.dtype).eps / 2
     off = 2 * abs(scale) * size * cache.dim * 2.0**-24
-    bound = spread * (2.0**-8 + off[..., None] + 2.0**-20) * (1 + half) + half * out.abs() + 2.0**-101
+    lost = max(batch.lengths_of, default=0) * 2.0**-29 * cache.values().abs().max()
+    bound = (spread * (2.0**-11 + off[..., None] + 2.0**-20) + lost) * (1 + half) + half * out.abs() + 2.0**-101
     err = (got.double().cpu().view_as(out) - out).abs()
     assert not torch.isnan(err).any(), f"NaN in rows {torch.isnan(err).any(-1).any(-1).nonzero().flatten().tolist()[:8]}"
     worst = (err - bound).flatten().argmax()
@@ -245,7 +246,7 @@ def check_appended(before, after, batch, k, v, freq, rot, interleaved):
             live = (got > 0)[None, :, None].expand_as(infinite)
             assert bool((codes[infinite & live] == qmax * value.sign()[infinite & live]).all())
             nans = value.isnan()
-            assert bool(codes[nans].isnan().all()) if after.fmt == "fp8" else bool((codes[nans] == 0).all())
+            assert bool((codes[nans] == 0).all())
             touched[page, :, in_page] = True
             scale_touched[page, :, at] = True
             if first:

@@ -1,12 +1,14 @@
-// lx_kv8_attention: softmax attention of a call's rows over the 8-bit paged cache. The kernels are in kv8_stream.h.
-#include "kv8_stream.h"
+// lx_kv8_attention: softmax attention of a call's rows over the 8-bit paged cache. The kernels are in kv8_stream.h (few rows a sequence)
+// and kv8_tile.h (many).
+#include "kv8_tile.h"
 
 namespace dro {
 namespace {
 
 // How a call is cut up: from the host's numbers alone, so that a captured call does not depend on what the device holds.
 struct Plan {
-  int row_tile_units;  // rows of a tile, in sixteens
+  bool tiles;          // kv8_tile.h's kernel
+  int per_tile;        // rows of a tile
   int row_tiles;       // tiles a sequence
   int tile_rows;       // rows of its fullest tile
   int splits, chunk;
@@ -22,18 +24,24 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads) {
   const int64_t most = b.max_rows < T ? b.max_rows : T;
   const int64_t rows = most * group;
   // Heads of 256 leave no registers for the sums of 32 rows.
-  p.row_tile_units = rows <= 16 || c.dim == 256 ? 1 : 2;
-  const int per = 16 * p.row_tile_units;
+  // Below 97 rows a sequence tiles of 32 rows that stream the cache (again from L2 for each) are ahead: 8 streams of up to 8191
+  // tokens at 40 / 64 / 96 / 128 rows 41.3 / 42.1 / 50.3 / 62.8 us, in tiles of 128 rows 47.6 / 48.9 / 52.1 / 54.3. Sums of 32 rows of
+  // heads wider than 128 leave the tile kernel's wavefronts too few registers (2048 rows of 256: 246 us against 352).
+  p.tiles = rows > 96 && c.dim <= 128;
+  p.per_tile = p.tiles ? kTileRowsOfGroup : rows <= 16 || c.dim == 256 ? 16 : 32;
+  const int per = p.per_tile;
   p.row_tiles = static_cast<int>((rows + per - 1) / per);
   p.tile_rows = static_cast<int>(rows < per ? rows : per);
   const int64_t held = static_cast<int64_t>(b.ld_table) * c.page;
   const int64_t length = held < b.max_length ? held : b.max_length;
   const int64_t items = static_cast<int64_t>(b.seqs) * p.row_tiles * c.heads;
-  const int64_t want = items > 0 ? (2 * compute_units() + items - 1) / items : 1;
+  int64_t want = items > 0 ? (2 * compute_units() + items - 1) / items : 1;
+  if (p.tiles && items >= compute_units()) want = 1;
   int64_t chunk = (length + want - 1) / (want > 0 ? want : 1);
   chunk = (chunk + 255) / 256 * 256;
   if (chunk < 256) chunk = 256;
-  if (chunk > kMaxRuns * kRun) chunk = kMaxRuns * kRun;
+  if (chunk > kMaxRuns * kRun && !p.tiles) chunk = kMaxRuns * kRun;
+  if (p.tiles && want <= 1) chunk = 0x7fffff00;
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((length + chunk - 1) / chunk);
   if (p.splits < 1) p.splits = 1;
@@ -45,14 +53,20 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads) {
 template <int F, int DIM>
 int stream(const AttentionArgs& a, const Plan& p, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(p.workgroups));
-  if (p.row_tile_units == 1) {
+  if (p.tiles) {
+    if constexpr (DIM <= 128) {
+      allow_lds(reinterpret_cast<const void*>(&tile_kernel<F, DIM>), tile_lds_bytes<DIM>());
+      hipLaunchKernelGGL((tile_kernel<F, DIM>), grid, dim3(256), tile_lds_bytes<DIM>(), s, a);
+    }
+  } else if (p.per_tile == 16) {
     hipLaunchKernelGGL((stream_kernel<F, DIM, 1>), grid, dim3(256), 0, s, a);
   } else {
     if constexpr (DIM < 256) hipLaunchKernelGGL((stream_kernel<F, DIM, 2>), grid, dim3(256), 0, s, a);
   }
   if (int st = status_of(hipGetLastError())) return st;
   if (p.splits == 1) return kOk;
-  hipLaunchKernelGGL((combine_kernel<DIM>), dim3(static_cast<unsigned>(p.workgroups / p.splits * p.tile_rows)), dim3(256), 0, s, a, 16 * p.row_tile_units, p.tile_rows);
+  const int64_t rows = p.workgroups / p.splits * p.tile_rows, per = p.splits <= kFewParts ? 1024 / DIM : 1;
+  hipLaunchKernelGGL((combine_kernel<DIM>), dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, s, a, p.per_tile, p.tile_rows);
   return status_of(hipGetLastError());
 }
 
@@ -83,13 +97,14 @@ int lx_kv8_attention(const void* q, lx_dtype q_dtype, int ld_q, const lx_kv8* ca
   const int64_t width = static_cast<int64_t>(q_heads) * cache->dim;
   if (!q || !out || (T > 1 && (ld_q < width || ld_out < width))) return fail(kInvalid);
   const Plan plan = plan_for(*cache, *batch, T, q_heads);
-  if (plan.workgroups > 0x7fffffff / 32 || (plan.bytes > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))) return fail(kInvalid);
+  if (plan.workgroups > 0x7fffffff / kTileRowsOfGroup || (plan.bytes > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))) return fail(kInvalid);
   AttentionArgs a{};
   a.c = kv8_cache(*cache);
   a.b = kv8_batch(*batch, T);
   a.q = q, a.out = out, a.partial = static_cast<float*>(workspace), a.ld_q = ld_q, a.ld_out = ld_out;
   a.q_dtype = q_dtype, a.out_dtype = out_dtype, a.group = q_heads / cache->heads, a.window = window, a.scale = scale;
   a.wide_q = q_dtype == LX_BF16 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld_q % 8 == 0;
+  a.wide_out = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld_out % 4 == 0;
   a.row_tiles = plan.row_tiles, a.splits = plan.splits, a.chunk = plan.chunk;
   return cache->type == LX_W_INT8 ? attention<LX_W_INT8>(a, plan, as_stream(stream)) : attention<LX_W_FP8>(a, plan, as_stream(stream));
 }

@@ -44,6 +44,7 @@ struct AttentionArgs {
   int q_dtype, out_dtype, group, window;
   float scale;
   int wide_q;                    // q is bf16 and can be read 16 bytes at a time
+  int wide_out;                  // out can be written 8 (bf16) or 16 (f32) bytes at a time
   int row_tiles, splits, chunk;  // chunk: tokens of a part, a multiple of 256, 16 * kMaxRuns at most
 };
 
@@ -140,6 +141,19 @@ __device__ __forceinline__ bf16x8 query_fragment(const AttentionArgs& p, bool ha
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = pack_bf16(load_as_f32(p.q, p.q_dtype, at + 2 * j), load_as_f32(p.q, p.q_dtype, at + 2 * j + 1));
   return __builtin_bit_cast(bf16x8, v);
+}
+
+// Four consecutive values of a result.
+__device__ __forceinline__ void store_four(const AttentionArgs& p, int64_t at, f32x4 v) {
+  if (!p.wide_out) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) store_from_f32(p.out, p.out_dtype, at + k, v[k]);
+  } else if (p.out_dtype == LX_BF16) {
+    const bf16x2 two[2] = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + at) = __builtin_bit_cast(u32x2, two);
+  } else {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + at) = v;
+  }
 }
 
 template <int F, int DIM, int RT>
@@ -391,8 +405,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
         const int flat = t.first + row;
         const int64_t at = (t.span.row0 + flat / p.group) * p.ld_out + static_cast<int64_t>(head * p.group + flat % p.group) * DIM + d;
         const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) store_from_f32(p.out, p.out_dtype, at + k, v[k] * inverse);
+        store_four(p, at, v * inverse);
       } else {
         *reinterpret_cast<f32x4*>(part + row * DIM + d) = v;
         if (d == 0) {
@@ -404,56 +417,68 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
   }
 }
 
-// The parts of one row added up. A workgroup takes a row of one of the cache's heads: every thread looks at some parts' largest
-// scores, then 1024 / DIM groups of DIM / 4 threads add up every so-manieth part each, and the groups' sums are added, all in a
-// fixed order. (One thread after another over all parts took 35 us of 57 for 64 of them.)
+// The parts of one row added up, in a fixed order. A row of one of the cache's heads is DIM / 4 threads; with up to kFewParts
+// parts they read them one after another. More parts are dealt out to the 1024 / DIM such groups of a whole workgroup, whose
+// sums are then added. (One group over 64 parts took 35 us of a call's 57; a workgroup for each of 48880 rows of two parts 110 of 243.)
+constexpr int kFewParts = 8;
+
 template <int DIM>
 __global__ void __launch_bounds__(256) combine_kernel(const AttentionArgs p, int per_tile, int rows) {
   constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
-  __shared__ float tops[4], sums_of[4];
+  __shared__ float sums_of[kGroups], tops[4];
   __shared__ f32x4 sums[kGroups][kLanes];
   const Kv8Cache& c = p.c;
-  const int row = blockIdx.x % rows;
-  const int64_t item = blockIdx.x / rows;
-  const int head = static_cast<int>(item % c.heads), tile = static_cast<int>(item / c.heads % p.row_tiles),
-            seq = static_cast<int>(item / c.heads / p.row_tiles);
-  const RowTile t = row_tile(p, seq, tile, per_tile);
+  const bool few = p.splits <= kFewParts;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int64_t which = few ? static_cast<int64_t>(blockIdx.x) * kGroups + group : blockIdx.x;
+  const int row = static_cast<int>(which % rows);
+  const int64_t item = which / rows;
+  const int head = static_cast<int>(item % c.heads), tile = static_cast<int>(item / c.heads % p.row_tiles);
+  const int64_t seq = item / c.heads / p.row_tiles;
+  if (few && group >= kGroups) return;  // heads of 192: 16 threads too many
+  if (seq >= p.b.seqs) return;
+  const RowTile t = row_tile(p, static_cast<int>(seq), tile, per_tile);
   if (row >= t.count || static_cast<int64_t>(t.begin) + p.chunk >= t.end) return;
   const int parts = (t.end - t.begin + p.chunk - 1) / p.chunk;
   const float* const first = partial_at<DIM>(p, item, 0, per_tile);
   const int64_t pitch = static_cast<int64_t>(per_tile) * (DIM + 2);
   const float* const marks = first + per_tile * DIM + 2 * row;  // largest score, sum of weights
-  const int wave = threadIdx.x / kWave;
   float m = -__builtin_inff();
-  for (int s = threadIdx.x; s < parts; s += 256) m = fmaxf(m, marks[s * pitch]);
-  m = wave_max(m);
-  if (threadIdx.x % kWave == 0) tops[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  if (few) {
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) m = fmaxf(m, marks[s * pitch]);
+  } else {
+    for (int s = threadIdx.x; s < parts; s += 256) m = fmaxf(m, marks[s * pitch]);
+    m = wave_max(m);
+    if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  }
   const float base = m == -__builtin_inff() ? 0.0f : m;
   float sum = 0.0f;
-  for (int s = threadIdx.x; s < parts; s += 256) sum += marks[s * pitch + 1] * __builtin_amdgcn_exp2f(marks[s * pitch] - base);
-  sum = wave_sum(sum);
-  if (threadIdx.x % kWave == 0) sums_of[wave] = sum;
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (group < kGroups) {
+  const int step = few ? 1 : kGroups;
 #pragma unroll 4
-    for (int s = group; s < parts; s += kGroups)
-      v += *reinterpret_cast<const f32x4*>(first + s * pitch + row * DIM + 4 * lane) * __builtin_amdgcn_exp2f(marks[s * pitch] - base);
-    sums[group][lane] = v;
+  for (int s = few ? 0 : group < kGroups ? group : parts; s < parts; s += step) {
+    const float keep = __builtin_amdgcn_exp2f(marks[s * pitch] - base);
+    sum += marks[s * pitch + 1] * keep;
+    v += *reinterpret_cast<const f32x4*>(first + s * pitch + row * DIM + 4 * lane) * keep;
   }
-  __syncthreads();
-  if (group > 0) return;
-  v = sums[0][lane];
+  if (!few) {
+    if (group < kGroups) sums[group][lane] = v;
+    if (group < kGroups && lane == 0) sums_of[group] = sum;
+    __syncthreads();
+    if (group > 0) return;
 #pragma unroll
-  for (int g = 1; g < kGroups; ++g) v += sums[g][lane];
-  sum = sums_of[0] + sums_of[1] + sums_of[2] + sums_of[3];
+    for (int g = 1; g < kGroups; ++g) {
+      v += sums[g][lane];
+      sum += sums_of[g];
+    }
+  }
   const int flat = t.first + row;
   const int64_t at = (t.span.row0 + flat / p.group) * p.ld_out + static_cast<int64_t>(head * p.group + flat % p.group) * DIM + 4 * lane;
   const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) store_from_f32(p.out, p.out_dtype, at + k, v[k] * inverse);
+  store_four(p, at, v * inverse);
 }
 
 }  // namespace dro

@@ -38,12 +38,15 @@ __host__ __device__ __forceinline__ int kv8_capacity(const Kv8Batch& b, int page
   return held < b.max_length ? static_cast<int>(held) : b.max_length;
 }
 
+// Its three numbers are asked for at once: no address depends on a branch.
 __host__ __device__ __forceinline__ Kv8Span kv8_span(const Kv8Batch& b, int page, int s) {
+  const int32_t* const rows = b.rows ? b.rows : b.lengths;
+  const int from = rows[s], to = rows[b.rows ? s + 1 : s], length = b.lengths[s];
   Kv8Span p;
-  p.row0 = b.rows ? clamp_int(b.rows[s], 0, b.T) : (s < b.T ? s : b.T);
-  const int end = b.rows ? clamp_int(b.rows[s + 1], 0, b.T) : (s + 1 < b.T ? s + 1 : b.T);
+  p.row0 = clamp_int(b.rows ? from : s, 0, b.T);
+  const int end = clamp_int(b.rows ? to : s + 1, 0, b.T);
   p.rows = end > p.row0 ? end - p.row0 : 0;
-  p.length = clamp_int(b.lengths[s], 0, kv8_capacity(b, page));
+  p.length = clamp_int(length, 0, kv8_capacity(b, page));
   return p;
 }
 

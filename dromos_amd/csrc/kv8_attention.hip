@@ -16,8 +16,8 @@ struct Plan {
   int64_t bytes;       // workspace
 };
 
-// Enough parts that the device has about two workgroups a compute unit, none shorter than 256 tokens (a step or two of each
-// wavefront). Four a unit: 131072 tokens of one stream 58.6 -> 61.6 us, 64 streams of 1024 tokens 29.3 -> 36.7.
+// Enough parts that the device has about two workgroups a compute unit, none shorter than 256 tokens (a step of each
+// wavefront); one part where sequences and heads alone make a workgroup a unit.
 Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads) {
   Plan p{};
   const int group = q_heads / c.heads;
@@ -36,9 +36,11 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads) {
   const int64_t length = held < b.max_length ? held : b.max_length;
   const int64_t items = static_cast<int64_t>(b.seqs) * p.row_tiles * c.heads;
   int64_t want = items > 0 ? (2 * compute_units() + items - 1) / items : 1;
-  if (p.tiles && items >= compute_units()) want = 1;
+  if (items >= compute_units()) want = 1;
   int64_t chunk = (length + want - 1) / (want > 0 ? want : 1);
   chunk = (chunk + 255) / 256 * 256;
+  // Parts cost a second kernel (about 4 us); one part costs a step of each wavefront more for every 256 tokens (1.6 us).
+  if (length <= 768) chunk = 768;
   if (chunk < 256) chunk = 256;
   if (chunk > kMaxRuns * kRun && !p.tiles) chunk = kMaxRuns * kRun;
   if (p.tiles && want <= 1) chunk = 0x7fffff00;
@@ -59,9 +61,9 @@ int stream(const AttentionArgs& a, const Plan& p, hipStream_t s) {
       hipLaunchKernelGGL((tile_kernel<F, DIM>), grid, dim3(256), tile_lds_bytes<DIM>(), s, a);
     }
   } else if (p.per_tile == 16) {
-    hipLaunchKernelGGL((stream_kernel<F, DIM, 1>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((stream_kernel<F, DIM, 1>), grid, dim3(kStreamThreads), 0, s, a);
   } else {
-    if constexpr (DIM < 256) hipLaunchKernelGGL((stream_kernel<F, DIM, 2>), grid, dim3(256), 0, s, a);
+    if constexpr (DIM < 256) hipLaunchKernelGGL((stream_kernel<F, DIM, 2>), grid, dim3(kStreamThreads), 0, s, a);
   }
   if (int st = status_of(hipGetLastError())) return st;
   if (p.splits == 1) return kOk;

@@ -8,10 +8,13 @@
 // bytes a lane as they lie, and a lane's slots of a sum over tokens are the four of one run of 16 and the four of the next
 // that it holds weights of. Values are read DIM / 16 bytes a lane and token (16 lanes a row) and transposed by bytes in
 // registers, two permutations for four tokens' pairs. Key codes become bf16 exactly, as the queries are; value codes become
-// f16 exactly. A key block's scale multiplies its scores, a value block's its weights, both f32, and the product is rounded to
-// f16 for the matrix cores: three more bits than bf16, so the roundings of the weights (2^-11 of each term) stay well below
-// the result's own. f16's range is made enough: scales are taken relative to the part's largest one, and weights times 2^15,
-// so that the largest is 2^15 and one 2^-29 of it is still a normal number. The sum of weights is f32.
+// f16 exactly. A key block's scale multiplies its scores; a value block's goes into its weights as an exponent: a weight is
+// 2^(score * key scale + (log2 of the value scale - m)), one multiply-add and one exponential, rounded to f16 for the matrix
+// cores: three more bits than bf16, so the roundings of the weights (2^-11 of each term) stay well below the result's own.
+// The sum of weights adds up the rounded ones, by twos, in f32, and takes the value scale off again once per run. f16's range is
+// made enough: value scales are taken relative to the part's largest one (under 2^-60 of it they count as that), weights are
+// held times 2^7, and the reference m follows a row's largest score only where that is 2^8 ahead: the largest weight is 2^15
+// at most, one 2^-21 of the reference's still a normal number, and most steps leave the sums as they are.
 //
 // Split. A workgroup takes one sequence, 16 RT rows of one of the cache's heads (rows of a head: its tokens' query heads,
 // token after token) and up to kMaxRuns runs of 16 tokens of it. Its four wavefronts take 64 tokens at a time in turn (32 of heads wider than 128) and keep
@@ -24,7 +27,7 @@
 
 namespace dro {
 
-constexpr int kStreamWaves = 4;
+constexpr int kStreamWaves = 4, kStreamThreads = kStreamWaves * kWave;
 constexpr int kMaxRuns = 256;  // runs of 16 tokens a workgroup takes at most
 
 // Runs a wavefront takes at a time: four, or two where four runs' codes and the sums (DIM * RT / 4 registers) would not fit
@@ -45,7 +48,7 @@ struct AttentionArgs {
   float scale;
   int wide_q;                    // q is bf16 and can be read 16 bytes at a time
   int wide_out;                  // out can be written 8 (bf16) or 16 (f32) bytes at a time
-  int row_tiles, splits, chunk;  // chunk: tokens of a part, a multiple of 256, 16 * kMaxRuns at most
+  int row_tiles, splits, chunk;  // chunk: tokens of a part, a multiple of 256, 16 * kMaxRuns at most (tiles of 128 rows: any number)
 };
 
 // What one tile of rows of a sequence attends to.
@@ -131,16 +134,31 @@ __device__ __forceinline__ uint32_t flipped(uint32_t d) {
 
 __device__ __forceinline__ f16x2 pack_f16(float a, float b) { return f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)}; }
 
-constexpr float kWeightBits = 15.0f;  // weights are held times 2^15
+constexpr float kWeightBits = 7.0f;   // weights are held times 2^7
+constexpr float kSlack = 8.0f;        // how far a score may be ahead of its row's reference (log2)
+constexpr float kLeastScale = -60.0f; // of a value block, relative to the largest (log2)
 
-// Eight consecutive values of a query as the matrix instruction's operand; f32 ones are rounded to bf16 here.
-__device__ __forceinline__ bf16x8 query_fragment(const AttentionArgs& p, bool have, int64_t at) {
-  if (!have) return __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
-  if (p.wide_q) return *reinterpret_cast<const bf16x8*>(static_cast<const uint16_t*>(p.q) + at);
-  bf16x2 v[4];
+// N eights of a query's values, `stride` values apart from `at` on, as the matrix instruction's operands; f32 ones are rounded to
+// bf16 here. A negative scale's sign goes to them, so that the scales of the scores never turn a largest one into a smallest.
+// A row that is none is read as row 0's and becomes zeros.
+template <int N, typename Offset>
+__device__ __forceinline__ void load_query(const AttentionArgs& p, bool have, int64_t at, Offset offset, bf16x8 (&q)[N]) {
+  u32x4 w[N];
+  if (p.wide_q) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = pack_bf16(load_as_f32(p.q, p.q_dtype, at + 2 * j), load_as_f32(p.q, p.q_dtype, at + 2 * j + 1));
-  return __builtin_bit_cast(bf16x8, v);
+    for (int k = 0; k < N; ++k) w[k] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.q) + at + offset(k));
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      bf16x2 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = pack_bf16(load_as_f32(p.q, p.q_dtype, at + offset(k) + 2 * j), load_as_f32(p.q, p.q_dtype, at + offset(k) + 2 * j + 1));
+      w[k] = __builtin_bit_cast(u32x4, v);
+    }
+  }
+  const uint32_t sign = p.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+  for (int k = 0; k < N; ++k) q[k] = __builtin_bit_cast(bf16x8, have ? w[k] ^ sign : u32x4{0u, 0u, 0u, 0u});
 }
 
 // Four consecutive values of a result.
@@ -157,20 +175,35 @@ __device__ __forceinline__ void store_four(const AttentionArgs& p, int64_t at, f
 }
 
 template <int F, int DIM, int RT>
-__global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
+__global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const AttentionArgs p) {
   constexpr int kC = DIM / 64, kTiles = DIM / 16, kPerTile = 16 * RT, kRuns = step_runs<DIM>(), kStep = kRuns * kRun;
   __shared__ int run_of[kMaxRuns];
-  __shared__ float key_scale[kMaxRuns], value_scale[kMaxRuns];
+  __shared__ float key_scale[kMaxRuns], value_log[kMaxRuns];
   __shared__ float wave_top[kStreamWaves][kPerTile], wave_sum_of[kStreamWaves][kPerTile];
-  __shared__ float sums[kStreamWaves][16][DIM + 4];
   __shared__ float scale_top[kStreamWaves];
-  __shared__ int holes;
+  __shared__ int hole_in[kStreamWaves];
+  __shared__ float sums[kStreamWaves][16][DIM + 4];
   const Kv8Cache& c = p.c;
   const int head = blockIdx.x % c.heads;
   int64_t rest = blockIdx.x / c.heads;
   const int split = static_cast<int>(rest % p.splits);
   rest /= p.splits;
   const int tile = static_cast<int>(rest % p.row_tiles), seq = static_cast<int>(rest / p.row_tiles);
+  const int lane = threadIdx.x % kWave, g = lane / 16, i = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+
+  // A part begins at a multiple of its length unless a window moves it, so its line of the page table is asked for together with
+  // the sequence's bounds: a thread's run of the part, and (lanes 0 .. 3) those that its wavefront begins with.
+  const int32_t* const line = p.b.table + static_cast<int64_t>(seq) * p.b.ld_table;
+  const int most = p.b.ld_table - 1;
+  auto page_of = [&](int64_t token) { return line[min(static_cast<int>(token / c.page), most)]; };
+  const int64_t guess = static_cast<int64_t>(split) * p.chunk;
+  const int mine = threadIdx.x, first_mine = wave * kRuns + lane % kRuns;
+  int page = -1, first_page = -1;
+  if (most >= 0 && p.window == 0) {
+    if (mine < kMaxRuns) page = page_of(guess + kRun * mine);
+    first_page = page_of(guess + kRun * first_mine);
+  }
   const RowTile t = row_tile(p, seq, tile, kPerTile);
   if (t.count <= 0) return;
   const int64_t start = t.begin + static_cast<int64_t>(split) * p.chunk;
@@ -178,39 +211,37 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
   const bool alone = static_cast<int64_t>(t.begin) + p.chunk >= t.end;  // the only part: the rows are written at once
   const int token0 = static_cast<int>(start), stop = static_cast<int>(min(start + p.chunk, static_cast<int64_t>(t.end)));
   const int runs = (stop - token0 + kRun - 1) / kRun;  // none where the rows see nothing
-
-  // Where the part's runs lie (-1: no page, no tokens), and their scales.
-  const int lane = threadIdx.x % kWave, g = lane / 16, i = lane % 16;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (threadIdx.x == 0) holes = 0;
-  __syncthreads();
-  float largest = 0.0f;
-  for (int e = threadIdx.x; e < runs; e += 256) {
-    const int token = token0 + kRun * e, page = kv8_page(c, p.b, seq, token);
-    float ks = 0.0f, vs = 0.0f;
-    int run = -1;
-    if (page >= 0) {
-      const int64_t at = kv8_row(c, page, head) + token % c.page;
-      run = static_cast<int>(at / kRun);
-      ks = c.k_scale[at >> c.block_shift] * p.scale * 1.4426950408889634f;
-      vs = c.v_scale[at >> c.block_shift];
-    } else {
-      holes = 1;
-    }
-    run_of[e] = run;
-    key_scale[e] = ks;
-    value_scale[e] = vs;
-    largest = fmaxf(largest, fabsf(vs));
+  const int steps = (runs + kRuns - 1) / kRuns;
+  if (p.window > 0) {
+    if (mine < runs) page = page_of(token0 + kRun * mine);
+    if (first_mine < runs) first_page = page_of(token0 + kRun * first_mine);
   }
-  largest = wave_max(largest);
-  if (lane == 0) scale_top[wave] = largest;
-  __syncthreads();
-  const bool whole = !holes;
-  largest = fmaxf(fmaxf(scale_top[0], scale_top[1]), fmaxf(scale_top[2], scale_top[3]));
-  const float per_largest = largest > 0.0f ? 1.0f / largest : 0.0f;
+  // The run of 16 tokens number e of the part, -1 where there is none or no page.
+  auto run_at = [&](int e, int page) {
+    if (e >= runs || page < 0 || page >= c.pages) return -1;
+    return static_cast<int>((kv8_row(c, page, head) + (token0 + kRun * e) % c.page) / kRun);
+  };
 
+  const int run = run_at(mine, page);
+  const int64_t scale_at = static_cast<int64_t>(max(run, 0)) * kRun >> c.block_shift;
+  const float ks = c.k_scale[scale_at], vs = c.v_scale[scale_at];
+  const int key_off = i * DIM + 16 * g, value_off = 4 * g * DIM + i * (DIM / 16);
+  KeyRegs<DIM> keys[kRuns];
+  ValueRegs<DIM> values[kRuns];
+  auto ask_keys = [&](auto where) {
+#pragma unroll
+    for (int j = 0; j < kRuns; ++j) load_keys<DIM>(keys[j], c.k + static_cast<int64_t>(max(where(j), 0)) * (kRun * DIM), key_off);
+  };
+  auto ask_values = [&](auto where) {
+#pragma unroll
+    for (int j = 0; j < kRuns; ++j) load_values<DIM>(values[j], c.v + static_cast<int64_t>(max(where(j), 0)) * (kRun * DIM), value_off);
+  };
+  // Everything the first step needs is on its way before anything is waited for; a wavefront without a step reads run 0.
+  const int first_run = run_at(first_mine, first_page);
+  auto first_where = [&](int j) { return __builtin_amdgcn_readlane(first_run, j); };
+  ask_keys(first_where);
   // The rows' queries: row 16 r + i, dims 64 c + 16 g + 8 h .. + 8 (the key's bytes of the same lane group).
-  bf16x8 q[RT][kC][2];
+  bf16x8 q[RT][2 * kC];
   int pos[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
@@ -218,13 +249,34 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
     const bool have = 16 * r + i < t.count;
     pos[r] = t.span.length - t.span.rows + token;
     const int64_t at = have ? (t.span.row0 + token) * p.ld_q + static_cast<int64_t>(head * p.group + flat % p.group) * DIM : 0;
-#pragma unroll
-    for (int cc = 0; cc < kC; ++cc)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        q[r][cc][h] = query_fragment(p, have, at + 64 * cc + 16 * g + 8 * h);
-      }
+    load_query(p, have, at, [&](int k) { return 64 * (k / 2) + 16 * g + 8 * (k % 2); }, q[r]);
   }
+  ask_values(first_where);
+  // Where the part's runs lie, and their scales.
+  const float log_here = run >= 0 ? __builtin_amdgcn_logf(fabsf(vs)) : -__builtin_inff();
+  if (mine < runs) {
+    run_of[mine] = run;
+    key_scale[mine] = run >= 0 ? ks * fabsf(p.scale) * 1.4426950408889634f : 0.0f;
+    value_log[mine] = log_here;
+  }
+  const float largest_here = wave_max(log_here);
+  const bool hole = __any(mine < runs && run < 0);
+  if (lane == 0) {
+    scale_top[wave] = largest_here;
+    hole_in[wave] = hole;
+  }
+  __syncthreads();
+  float largest = scale_top[0];  // log2 of the part's largest value scale
+  bool whole = !hole_in[0];
+#pragma unroll
+  for (int w = 1; w < kMaxRuns / kWave; ++w) {
+    largest = fmaxf(largest, scale_top[w]);
+    whole = whole && !hole_in[w];
+  }
+  if (largest == -__builtin_inff()) largest = 0.0f;  // every scale 0
+  auto run_in = [&](int step) {
+    return [&, step](int j) { return __builtin_amdgcn_readfirstlane(run_of[min(step * kRuns + j, runs - 1)]); };
+  };
 
   f32x4 acc[RT][kTiles] = {};
   float top[RT], total[RT];
@@ -232,26 +284,6 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
   for (int r = 0; r < RT; ++r) {
     top[r] = -__builtin_inff();
     total[r] = 0.0f;
-  }
-  const int steps = (runs + kRuns - 1) / kRuns;
-  const int key_off = i * DIM + 16 * g, value_off = 4 * g * DIM + i * (DIM / 16);
-  KeyRegs<DIM> keys[kRuns];
-  ValueRegs<DIM> values[kRuns];
-  auto run_base = [&](int step, int j) {
-    const int at = min(step * kRuns + j, runs - 1);
-    return static_cast<int64_t>(max(__builtin_amdgcn_readfirstlane(run_of[at]), 0)) * (kRun * DIM);
-  };
-  auto ask_keys = [&](int step) {
-#pragma unroll
-    for (int j = 0; j < kRuns; ++j) load_keys<DIM>(keys[j], c.k + run_base(step, j), key_off);
-  };
-  auto ask_values = [&](int step) {
-#pragma unroll
-    for (int j = 0; j < kRuns; ++j) load_values<DIM>(values[j], c.v + run_base(step, j), value_off);
-  };
-  if (wave < steps) {
-    ask_keys(wave);
-    ask_values(wave);
   }
   for (int step = wave; step < steps; step += kStreamWaves) {
     const int at = token0 + step * kStep;
@@ -266,21 +298,20 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
         for (int h = 0; h < 2; ++h) {
           const bf16x8 a = weight_fragment<F>(keys[j].w[cc], 0, h);
 #pragma unroll
-          for (int r = 0; r < RT; ++r) s[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[r][cc][h], s[r][j], 0, 0, 0);
+          for (int r = 0; r < RT; ++r) s[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[r][2 * cc + h], s[r][j], 0, 0, 0);
         }
     }
     const bool more = step + kStreamWaves < steps;
-    if (more) ask_keys(step + kStreamWaves);
+    if (more) ask_keys(run_in(step + kStreamWaves));
     // Every token of the step is seen by every row?
     const bool plain = whole && at + kStep - 1 <= t.low_pos && (p.window == 0 || at > t.high_pos - p.window);
-    float vs[kRuns];
+    float ks[kRuns], ve[kRuns], per[kRuns];
 #pragma unroll
     for (int j = 0; j < kRuns; ++j) {
       const int run = min(step * kRuns + j, runs - 1);
-      const float ks = key_scale[run];
-      vs[j] = value_scale[run] * per_largest;
-#pragma unroll
-      for (int r = 0; r < RT; ++r) s[r][j] *= ks;
+      ks[j] = key_scale[run];
+      ve[j] = fmaxf(value_log[run] - largest, kLeastScale) + kWeightBits;
+      per[j] = __builtin_amdgcn_exp2f(-ve[j]);
     }
     if (!plain) {
 #pragma unroll
@@ -290,47 +321,54 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
         for (int e = 0; e < 4; ++e) {
           const int token = at + kRun * j + 4 * g + e;
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
-            if (!there || token > pos[r] || (p.window > 0 && token <= pos[r] - p.window)) s[r][j][e] = -__builtin_inff();
+          for (int r = 0; r < RT; ++r) {
+            const bool hidden = !there || token > pos[r] || (p.window > 0 && token <= pos[r] - p.window);
+            s[r][j][e] = hidden ? -__builtin_inff() : s[r][j][e] * ks[j];
+          }
           // Codes of places without a token (NaNs perhaps) times a weight of nothing have to be nothing.
           if (!there || token >= t.span.length)
 #pragma unroll
             for (int d = 0; d < kC; ++d) values[j].w[e][d] = 0;
         }
+        ks[j] = 1.0f;
       }
     }
     f16x8 weights[RT][kRuns / 2];
+    const f16x2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      float m = s[r][0][0];
+      float m = -__builtin_inff();
 #pragma unroll
       for (int j = 0; j < kRuns; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, s[r][j][e]);
+        m = fmaxf(m, fmaxf(fmaxf(s[r][j][0], s[r][j][1]), fmaxf(s[r][j][2], s[r][j][3])) * ks[j]);
       float a, b;
       swap_halves<true>(m, a, b);
       m = fmaxf(a, b);
       swap_halves<false>(m, a, b);
-      m = fmaxf(top[r], fmaxf(a, b));
-      const float base = m == -__builtin_inff() ? 0.0f : m;
-      const float keep = __builtin_amdgcn_exp2f(top[r] - base);
-      if (__any(m != top[r])) {
+      m = fmaxf(a, b);
+      if (__any(m > top[r] + kSlack)) {
+        m = fmaxf(m, top[r]);
+        const float keep = __builtin_amdgcn_exp2f(top[r] - (m == -__builtin_inff() ? 0.0f : m));
 #pragma unroll
         for (int f = 0; f < kTiles; ++f) acc[r][f] *= keep;
         total[r] *= keep;
+        top[r] = m;
       }
-      top[r] = m;
-      const float lifted = base - kWeightBits;
+      const float base = top[r] == -__builtin_inff() ? 0.0f : top[r];
 #pragma unroll
       for (int j = 0; j < kRuns; j += 2) {
-        float w[8];
+        f16x2 v[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = __builtin_amdgcn_exp2f(s[r][j + e / 4][e % 4] - lifted);
-          total[r] += x;
-          w[e] = x * vs[j + e / 4];
+        for (int e = 0; e < 2; ++e) {
+          const float lift = ve[j + e] - base;
+          float w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][j + e][k], ks[j + e], lift));
+          v[2 * e] = pack_f16(w[0], w[1]);
+          v[2 * e + 1] = pack_f16(w[2], w[3]);
+          const float sum = __builtin_amdgcn_fdot2(v[2 * e + 1], ones, __builtin_amdgcn_fdot2(v[2 * e], ones, 0.0f, false), false);
+          total[r] = __builtin_fmaf(sum, per[j + e], total[r]);
         }
-        const f16x2 v[4] = {pack_f16(w[0], w[1]), pack_f16(w[2], w[3]), pack_f16(w[4], w[5]), pack_f16(w[6], w[7])};
         weights[r][j / 2] = __builtin_bit_cast(f16x8, v);
       }
     }
@@ -356,7 +394,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
           for (int r = 0; r < RT; ++r) acc[r][4 * d + f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, weights[r][j / 2], acc[r][4 * d + f], 0, 0, 0);
         }
       }
-    if (more) ask_values(step + kStreamWaves);
+    if (more) ask_values(run_in(step + kStreamWaves));
   }
 
   // The wavefronts' sums together.
@@ -372,13 +410,20 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
     }
   }
   __syncthreads();
+  const float to_value = __builtin_amdgcn_exp2f(largest - kWeightBits);  // the sums are of weights times 2^7 and scales over the largest
+  auto row_top = [&](int row) {
+    float m = wave_top[0][row];
+#pragma unroll
+    for (int w = 1; w < kStreamWaves; ++w) m = fmaxf(m, wave_top[w][row]);
+    return m;
+  };
   float* const part = alone ? nullptr : partial_at<DIM>(p, (static_cast<int64_t>(seq) * p.row_tiles + tile) * c.heads + head, split, kPerTile);
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     if (16 * r >= t.count) break;
     const int row = 16 * r + i;
-    const float m = fmaxf(fmaxf(wave_top[0][row], wave_top[1][row]), fmaxf(wave_top[2][row], wave_top[3][row]));
-    const float keep = top[r] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top[r] - m) * largest;
+    const float m = row_top(row);
+    const float keep = top[r] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top[r] - m) * to_value;
     if (r > 0) __syncthreads();
     // Tile f of a lane: dims kTiles * (4 g + e) + f.
 #pragma unroll
@@ -389,10 +434,10 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const AttentionArgs p) {
         *reinterpret_cast<f32x4*>(&sums[wave][i][kTiles * (4 * g + e) + f]) = v * keep;
       }
     __syncthreads();
-    for (int e = threadIdx.x; e < 16 * (DIM / 4); e += 256) {
+    for (int e = threadIdx.x; e < 16 * (DIM / 4); e += kStreamThreads) {
       const int local = e / (DIM / 4), d = 4 * (e % (DIM / 4)), row = 16 * r + local;
       if (row >= t.count) continue;
-      const float m = fmaxf(fmaxf(wave_top[0][row], wave_top[1][row]), fmaxf(wave_top[2][row], wave_top[3][row]));
+      const float m = row_top(row);
       float sum = 0.0f;
       f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll

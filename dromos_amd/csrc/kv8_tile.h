@@ -7,9 +7,7 @@
 // scores of one row, tokens 8 a + 4 h + b (h = lane / 32), and a sum over 16 tokens takes its eight of them as they
 // lie, so the value columns are stored in that order and weights never change lanes.
 //
-// A score costs half a maximum, one multiply-add, one exponential, half a conversion and half a sum: the key block's scale and
-// the value block's (as an exponent) go into the multiply-add, and the sum of weights (the rounded ones, by twos, in f32)
-// takes the latter off again once per run.
+// A score costs half a maximum, one multiply-add, one exponential, half a conversion and half a sum.
 // LDS rows are swizzled by 16-byte pieces so that the 32 rows of a read fall on all banks.
 #pragma once
 
@@ -28,10 +26,6 @@ template <int DIM>
 constexpr int tile_tokens() {
   return 8192 / DIM;
 }
-
-// Weights are held times 2^7, and the row's reference follows its largest score only where that is 2^8 ahead: most tiles leave
-// the sums as they are, and the largest weight is 2^15 at most.
-constexpr float kTileWeightBits = 7.0f, kTileSlack = 8.0f;
 
 // Where 16-byte piece `piece` of a row lies in its row. Sixteen rows that a read takes a piece of each fall on sixteen places of
 // the 256 bytes that the banks are wide, and eight neighbouring lanes that write (neighbouring rows, or of the keys' image every
@@ -92,13 +86,8 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
   bf16x8 q[DIM / 16];
   {
     const int flat = my_first + n, token = flat / p.group;
-    const int64_t at = (t.span.row0 + token) * p.ld_q + static_cast<int64_t>(head * p.group + flat % p.group) * DIM;
-#pragma unroll
-    for (int k = 0; k < DIM / 16; ++k) q[k] = query_fragment(p, n < my_count, at + 16 * k + 8 * h);
-    if (p.scale < 0.0f) {  // the sign goes to the queries: the scales below are none that turn a maximum into a minimum
-#pragma unroll
-      for (int k = 0; k < DIM / 16; ++k) q[k] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, q[k]) ^ 0x80008000u);
-    }
+    const int64_t at = n < my_count ? (t.span.row0 + token) * p.ld_q + static_cast<int64_t>(head * p.group + flat % p.group) * DIM : 0;
+    load_query(p, n < my_count, at, [&](int k) { return 16 * k + 8 * h; }, q);
   }
   f32x16 acc[DIM / 32] = {};
   float top = -__builtin_inff(), total = 0.0f, largest = 0.0f;
@@ -189,7 +178,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
     most = fmaxf(fmaxf(fmaxf(scale_top[0], scale_top[1]), fmaxf(scale_top[2], scale_top[3])), largest);
     // Scales as exponents relative to the largest so far; one under 2^-60 of it counts as that.
     if (static_cast<int>(threadIdx.x) < runs) {
-      const float e = most > 0.0f ? fmaxf(__builtin_amdgcn_logf(vs / most), -60.0f) + kTileWeightBits : 0.0f;
+      const float e = most > 0.0f ? fmaxf(__builtin_amdgcn_logf(vs / most), kLeastScale) + kWeightBits : 0.0f;
       value_exp[threadIdx.x] = e;
       value_per[threadIdx.x] = __builtin_amdgcn_exp2f(-e);
     }
@@ -261,7 +250,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
         float x0, x1;
         swap_halves<false>(m, x0, x1);
         m = fmaxf(x0, x1);
-        if (__any(m > top + kTileSlack)) {
+        if (__any(m > top + kSlack)) {
           m = fmaxf(m, top);
           const float base = m == -__builtin_inff() ? 0.0f : m;
           const float keep = __builtin_amdgcn_exp2f(top - base);
@@ -305,7 +294,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
   swap_halves<false>(total, x0, x1);
   const float sum = x0 + x1;
   if (n >= my_count) return;
-  const float to_value = largest * 0x1p-7f;  // kTileWeightBits
+  const float to_value = largest * 0x1p-7f;  // kWeightBits
   if (alone) {
     const int flat = my_first + n;
     const int64_t at = (t.span.row0 + flat / p.group) * p.ld_out + static_cast<int64_t>(head * p.group + flat % p.group) * DIM;

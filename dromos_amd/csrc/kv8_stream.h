@@ -469,8 +469,8 @@ constexpr int kFewParts = 8;
 
 template <int DIM>
 __global__ void __launch_bounds__(256) combine_kernel(const AttentionArgs p, int per_tile, int rows) {
-  constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
-  __shared__ float sums_of[kGroups], tops[4];
+  constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes, kAtOnce = 4;
+  __shared__ float tops[kGroups], sums_of[kGroups];
   __shared__ f32x4 sums[kGroups][kLanes];
   const Kv8Cache& c = p.c;
   const bool few = p.splits <= kFewParts;
@@ -487,37 +487,53 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttentionArgs p, int
   const int parts = (t.end - t.begin + p.chunk - 1) / p.chunk;
   const float* const first = partial_at<DIM>(p, item, 0, per_tile);
   const int64_t pitch = static_cast<int64_t>(per_tile) * (DIM + 2);
-  const float* const marks = first + per_tile * DIM + 2 * row;  // largest score, sum of weights
-  float m = -__builtin_inff();
-  if (few) {
-#pragma unroll 4
-    for (int s = 0; s < parts; ++s) m = fmaxf(m, marks[s * pitch]);
-  } else {
-    for (int s = threadIdx.x; s < parts; s += 256) m = fmaxf(m, marks[s * pitch]);
-    m = wave_max(m);
-    if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  }
-  const float base = m == -__builtin_inff() ? 0.0f : m;
-  float sum = 0.0f;
+  const int begin = few ? 0 : group < kGroups ? group : parts, step = few ? 1 : kGroups;
+  float m = -__builtin_inff(), sum = 0.0f;
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int step = few ? 1 : kGroups;
-#pragma unroll 4
-  for (int s = few ? 0 : group < kGroups ? group : parts; s < parts; s += step) {
-    const float keep = __builtin_amdgcn_exp2f(marks[s * pitch] - base);
-    sum += marks[s * pitch + 1] * keep;
-    v += *reinterpret_cast<const f32x4*>(first + s * pitch + row * DIM + 4 * lane) * keep;
+  // Sums and marks (largest score, sum of weights) of kAtOnce parts are asked for together; the last part again for those behind it.
+  for (int s = begin; s < parts; s += kAtOnce * step) {
+    f32x2 marks[kAtOnce];
+    f32x4 data[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const float* const part = first + min(s + k * step, parts - 1) * pitch;
+      marks[k] = *reinterpret_cast<const f32x2*>(part + per_tile * DIM + 2 * row);
+      data[k] = *reinterpret_cast<const f32x4*>(part + row * DIM + 4 * lane);
+    }
+    float now = m;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) now = fmaxf(now, marks[k].x);
+    const float base = now == -__builtin_inff() ? 0.0f : now, keep = __builtin_amdgcn_exp2f(m - base);
+    sum *= keep;
+    v *= keep;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const float w = s + k * step < parts ? __builtin_amdgcn_exp2f(marks[k].x - base) : 0.0f;
+      sum += marks[k].y * w;
+      v += data[k] * w;
+    }
+    m = now;
   }
   if (!few) {
-    if (group < kGroups) sums[group][lane] = v;
-    if (group < kGroups && lane == 0) sums_of[group] = sum;
+    if (group < kGroups) {
+      sums[group][lane] = v;
+      if (lane == 0) {
+        tops[group] = m;
+        sums_of[group] = sum;
+      }
+    }
     __syncthreads();
     if (group > 0) return;
 #pragma unroll
-    for (int g = 1; g < kGroups; ++g) {
-      v += sums[g][lane];
-      sum += sums_of[g];
+    for (int g = 1; g < kGroups; ++g) m = fmaxf(m, tops[g]);
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+    sum = 0.0f;
+    v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const float w = __builtin_amdgcn_exp2f(tops[g] - base);
+      sum += sums_of[g] * w;
+      v += sums[g][lane] * w;
     }
   }
   const int flat = t.first + row;

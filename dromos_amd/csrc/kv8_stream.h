@@ -185,10 +185,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
   __shared__ float sums[kStreamWaves][16][DIM + 4];
   const Kv8Cache& c = p.c;
   const int head = blockIdx.x % c.heads;
-  int64_t rest = blockIdx.x / c.heads;
-  const int split = static_cast<int>(rest % p.splits);
-  rest /= p.splits;
-  const int tile = static_cast<int>(rest % p.row_tiles), seq = static_cast<int>(rest / p.row_tiles);
+  // The first parts of all sequences go first: later ones may have nothing to do, and workgroups that do lie side by side evenly
+  // (16 streams of up to 8192 tokens: with a sequence's parts side by side 160 compute units had all the work).
+  const int rest = blockIdx.x / c.heads, items = p.b.seqs * p.row_tiles;
+  const int split = rest / items, tile = rest % items % p.row_tiles, seq = rest % items / p.row_tiles;
   const int lane = threadIdx.x % kWave, g = lane / 16, i = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 

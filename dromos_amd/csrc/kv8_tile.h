@@ -27,6 +27,9 @@ constexpr int tile_tokens() {
   return 8192 / DIM;
 }
 
+// What the scheduler is told to group: matrix instructions, reads of LDS, vector arithmetic.
+constexpr int kMatrix = 0x8, kReads = 0x100, kVector = 0x2;
+
 // Where 16-byte piece `piece` of a row lies in its row. Sixteen rows that a read takes a piece of each fall on sixteen places of
 // the 256 bytes that the banks are wide, and eight neighbouring lanes that write (neighbouring rows, or of the keys' image every
 // other piece of a row, which is why its even pieces come first) on eight places of 128.
@@ -204,17 +207,23 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
       if (some) {
         // The wavefronts of a SIMD take turns: the one that feeds the matrix cores goes first (176 -> 169 us on a 4096-row prompt).
         __builtin_amdgcn_s_setprio(1);
-        f32x16 s[kTok / 32];
+        f32x16 s[kTok / 32] = {};
 #pragma unroll
-        for (int b = 0; b < kTok / 32; ++b) {
-          s[b] = f32x16{};
+        for (int k = 0; k < DIM / 16; ++k)
 #pragma unroll
-          for (int k = 0; k < DIM / 16; ++k) {
+          for (int b = 0; b < kTok / 32; ++b) {
             const int row = 32 * b + n;
             const bf16x8 a = *reinterpret_cast<const bf16x8*>(keys + row * kKeyPitch + key_place<DIM>(row, 2 * k + h));
             s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[k], s[b], 0, 0, 0);
           }
+        // Six reads ahead of the matrix instructions, not one or two (162 -> 150 us).
+        __builtin_amdgcn_sched_group_barrier(kReads, 6, 0);
+#pragma unroll
+        for (int e = 0; e < 10; ++e) {
+          __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kReads, 1, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(kMatrix, 6, 0);
         __builtin_amdgcn_s_setprio(0);
         const bool plain = clean(i) && at + kTok - 1 <= low_pos && (p.window == 0 || at > high_pos - p.window);
         float ks[kTok / kRun], ve[kTok / kRun], per[kTok / kRun];
@@ -261,9 +270,20 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
         }
         const float base = top == -__builtin_inff() ? 0.0f : top;
         const f16x2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-        f16x8 weights[kTok / kRun];
+        // A run's weights are made while the matrix cores work on the one before it, from values that were read before that.
+        f16x8 a[2][DIM / 32];
+        auto read_values = [&](int j, f16x8 (&to)[DIM / 32]) {
+#pragma unroll
+          for (int f = 0; f < DIM / 32; ++f) {
+            const int row = 32 * f + n;
+            to[f] = *reinterpret_cast<const f16x8*>(values + row * kValuePitch + 16 * swizzled<kValuePitch>(row, 2 * j + h));
+          }
+        };
+        if (DIM == 128) __builtin_amdgcn_s_setprio(1);
+        read_values(0, a[0]);
 #pragma unroll
         for (int j = 0; j < kTok / kRun; ++j) {
+          if (j + 1 < kTok / kRun) read_values(j + 1, a[(j + 1) % 2]);
           const float lift = ve[j] - base;
           float w[8], sum = 0.0f;
 #pragma unroll
@@ -272,19 +292,12 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_fdot2(v[e], ones, sum, false);
           total = __builtin_fmaf(sum, per[j], total);
-          weights[j] = __builtin_bit_cast(f16x8, v);
+          const f16x8 weights = __builtin_bit_cast(f16x8, v);
+#pragma unroll
+          for (int f = 0; f < DIM / 32; ++f) acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[j % 2][f], weights, acc[f], 0, 0, 0);
         }
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int f = 0; f < DIM / 32; ++f)
-#pragma unroll
-          for (int j = 0; j < kTok / kRun; ++j) {
-            const int row = 32 * f + n;
-            const f16x8 a = *reinterpret_cast<const f16x8*>(values + row * kValuePitch + 16 * swizzled<kValuePitch>(row, 2 * j + h));
-            acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, weights[j], acc[f], 0, 0, 0);
-          }
-        __builtin_amdgcn_s_setprio(0);
       }
+      __builtin_amdgcn_s_setprio(0);
       if (more) put(lds + ((i + 1) % 2) * kBuffer, at + kTok, (i + 1) * (kTok / kRun), runs, clean(i + 1));
       __syncthreads();
     }

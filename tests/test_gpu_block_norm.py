@@ -140,6 +140,15 @@ def test_zero_rows_and_extremes(hip):
         check(hip, layer, y, randn(3, 512, dtype=F), None, None, 1.0, 1.0, h, randn(4, 512, dtype=F), None, F)
 
 
+@pytest.mark.parametrize("width", [2048, 2560, 4096, 4616, 8192])
+def test_a_rows_bits_do_not_depend_on_how_many_there_are(hip, width):
+    y, h, w = randn(1, 1100, width).cuda(), randn(2, 1100, width, dtype=F).cuda(), randn(3, width).cuda()
+    for layer in (False, True):
+        all_h, all_x = call(hip, layer, y, w, None, None, 1.0, 1.0, h, w, None, F, 1e-5)
+        some_h, some_x = call(hip, layer, y[1000:1009], w, None, None, 1.0, 1.0, h[1000:1009], w, None, F, 1e-5)
+        assert torch.equal(some_h, all_h[1000:1009]) and torch.equal(some_x, all_x[1000:1009])
+
+
 def test_a_rows_bits_do_not_depend_on_the_others(hip):
     y, h = randn(1, 40, 4096).cuda(), randn(2, 40, 4096).cuda()
     w = randn(3, 4096).cuda()

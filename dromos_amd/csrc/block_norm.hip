@@ -4,7 +4,7 @@
 // Bytes decide: y, h and the gate are read once, h and x written once, and a row stays in its workgroup's registers between
 // (four vectors of eight values a thread at most, 32768 values a row). A workgroup takes one row. Sums are f32, in
 // an order that goes by the width alone, and with it a row's bits.
-#include "common.h"
+#include "tile_mfma.h"
 
 namespace dro {
 namespace {
@@ -79,7 +79,7 @@ __device__ __forceinline__ void store_values(void* p, int type, int64_t i, const
     u32x4 w;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      w[j] = f32_to_bf16_bits(v[2 * j]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * j + 1])) << 16;
+      w[j] = __builtin_bit_cast(uint32_t, pack_bf16(v[2 * j], v[2 * j + 1]));
     __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i));
   } else {
     f32x4* const q = reinterpret_cast<f32x4*>(static_cast<float*>(p) + i);

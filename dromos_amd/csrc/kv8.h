@@ -38,38 +38,43 @@ __host__ __device__ __forceinline__ int kv8_capacity(const Kv8Batch& b, int page
   return held < b.max_length ? static_cast<int>(held) : b.max_length;
 }
 
-// Its three numbers are asked for at once: no address depends on a branch.
-__host__ __device__ __forceinline__ Kv8Span kv8_span(const Kv8Batch& b, int page, int s) {
-  const int32_t* const rows = b.rows ? b.rows : b.lengths;
-  const int from = rows[s], to = rows[b.rows ? s + 1 : s], length = b.lengths[s];
+__host__ __device__ __forceinline__ Kv8Span kv8_span_of(const Kv8Batch& b, int page, int from, int to, int length) {
   Kv8Span p;
-  p.row0 = clamp_int(b.rows ? from : s, 0, b.T);
-  const int end = clamp_int(b.rows ? to : s + 1, 0, b.T);
+  p.row0 = clamp_int(from, 0, b.T);
+  const int end = clamp_int(to, 0, b.T);
   p.rows = end > p.row0 ? end - p.row0 : 0;
   p.length = clamp_int(length, 0, kv8_capacity(b, page));
   return p;
 }
 
+// The three numbers are asked for at once: no address depends on a branch.
+__host__ __device__ __forceinline__ Kv8Span kv8_span(const Kv8Batch& b, int page, int s) {
+  const int32_t* const rows = b.rows ? b.rows : b.lengths;
+  const int from = rows[s], to = rows[b.rows ? s + 1 : s], length = b.lengths[s];
+  return kv8_span_of(b, page, b.rows ? from : s, b.rows ? to : s + 1, length);
+}
+
 // The part of a block that row r of a call brings to the cache: tokens position .. end - 1 of the block that begins at
 // `begin`, and the row behind them. A row has a part of its own where it is its sequence's first one with a place in the
-// cache, or the first of its block; the others go with one in front of them.
+// cache, or the first of its block; the others go with one in front of them, and rows beyond the caller's max_rows have none.
 struct Kv8Piece {
   int position, begin, end, next;
   bool own;
 };
 
-__host__ __device__ __forceinline__ Kv8Piece kv8_piece(const Kv8Span& span, int block_shift, int r) {
+__host__ __device__ __forceinline__ Kv8Piece kv8_piece(const Kv8Span& span, int max_rows, int block_shift, int r) {
   const int lead = span.length - span.rows;  // the position of the sequence's first row; negative: rows in front of any token
+  const int stop = lead + (span.rows < max_rows ? span.rows : max_rows);
   Kv8Piece p;
   p.position = lead + (r - span.row0);
-  if (p.position < 0) {
+  if (p.position < 0 || p.position >= stop) {
     p.begin = p.end = 0;
-    p.next = span.row0 + (span.length > 0 ? -lead : span.rows);
+    p.next = span.row0 + (p.position < 0 && span.length > 0 ? -lead : span.rows);
     p.own = false;
     return p;
   }
   p.begin = p.position >> block_shift << block_shift;
-  p.end = p.begin + (1 << block_shift) < span.length ? p.begin + (1 << block_shift) : span.length;
+  p.end = p.begin + (1 << block_shift) < stop ? p.begin + (1 << block_shift) : stop;
   p.next = span.row0 + (p.end - lead);
   p.own = p.position == p.begin || p.position == (lead > 0 ? lead : 0);
   return p;
@@ -102,7 +107,7 @@ inline int kv8_check_cache(const lx_kv8* c) {
 }
 
 inline int kv8_check_batch(const lx_kv8_batch* b, int T) {
-  if (!b || T < 0 || T > (1 << 30) || b->seqs < 0 || b->seqs > (1 << 30) || b->max_rows < 0 || b->max_length < 0 || b->ld_table < 0) return kInvalid;
+  if (!b || T < 0 || T >= (1 << 30) || b->seqs < 0 || b->seqs > (1 << 30) || b->max_rows < 0 || b->max_length < 0 || b->ld_table < 0) return kInvalid;
   if (T == 0 || b->seqs == 0) return kOk;
   if (!b->lengths || (b->ld_table > 0 && !b->table)) return kInvalid;
   return kOk;
@@ -115,7 +120,7 @@ inline Kv8Cache kv8_cache(const lx_kv8& c) {
 }
 
 inline Kv8Batch kv8_batch(const lx_kv8_batch& b, int T) {
-  return {b.rows, b.lengths, b.table, b.seqs, b.ld_table, b.max_rows, b.max_length, T};
+  return {b.rows, b.lengths, b.table, b.seqs, b.ld_table, b.max_rows < T ? b.max_rows : T, b.max_length, T};
 }
 
 }  // namespace dro

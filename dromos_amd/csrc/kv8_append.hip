@@ -2,10 +2,15 @@
 // too), and lx_kv8_dequantize, the cache back as bf16.
 //
 // A scale belongs to a block of tokens and a head, so the unit of work is one such block as far as this call writes it: its
-// largest magnitude has to be known before its first code. Tokens of the block from earlier calls keep their codes while
-// their scale still covers the new ones; where it has to grow they are read, rescaled and written again (a block holds 128
-// tokens at most).
+// largest magnitude has to be known before its first code. A workgroup reads it once and holds it in registers (a lane has
+// eight values of a token's head, up to four tokens). Tokens of the block from earlier calls keep their codes while their scale
+// still covers the new ones; where it has to grow they are read, rescaled and written again (a block holds 128 tokens at most).
+// Queries are turned by workgroups of their own, four heads each, so that a model with few heads in its cache has enough of them.
+//
+// A prompt is bound by bytes. A single token is bound by the latency of what it has to follow: the rows' bounds and lengths (every
+// wavefront looks through them by itself), the page table, the block's scale; its values are asked for before the first of them.
 #include "kv8.h"
+#include "tile_mfma.h"
 
 namespace dro {
 namespace {
@@ -19,7 +24,10 @@ struct AppendArgs {
   void* q_out;
   const float* freq;
   int64_t ld_q, ld_k, ld_v, ld_out;
-  int dtype, out_dtype, rot, interleaved, group;
+  int dtype, out_dtype, rot, interleaved, q_heads;
+  int tokens;          // of a block that a call writes at most
+  unsigned queries;    // the first workgroup that turns queries
+  int query_rows;      // rows of one of those
   int rows_per_group;  // rows a workgroup looks at for blocks that begin there
   int wide;            // q, k, v and q_out can be moved 16 (bf16) or 32 (f32) bytes at a time
 };
@@ -41,42 +49,61 @@ __device__ __forceinline__ Unit unit_of(const AppendArgs& p, int u) {
   return n;
 }
 
-// v[0..3] and v[4..7]: the two runs of four, from `at` on.
-__device__ __forceinline__ void load_unit(const void* x, int dtype, bool wide, int64_t at, const Unit& n, float* v) {
-  if (!wide) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = load_as_f32(x, dtype, at + n.a + j);
-      v[4 + j] = load_as_f32(x, dtype, at + n.b + j);
-    }
-  } else if (dtype == LX_BF16) {
+// The eight values as they lie in memory: bf16 (HALF: where they can be moved 8 bytes at a time), or f32.
+template <bool HALF>
+struct RawUnit {
+  u32x4 w[HALF ? 1 : 2];
+};
+
+template <bool HALF>
+__device__ __forceinline__ RawUnit<HALF> load_unit(const void* x, int dtype, bool wide, int64_t at, const Unit& n) {
+  RawUnit<HALF> r;
+  if constexpr (HALF) {
     const uint16_t* const h = static_cast<const uint16_t*>(x) + at;
     const u32x2 lo = *reinterpret_cast<const u32x2*>(h + n.a), hi = *reinterpret_cast<const u32x2*>(h + n.b);
-    decode_dword<LX_W_BF16>(lo.x, v);
-    decode_dword<LX_W_BF16>(lo.y, v + 2);
-    decode_dword<LX_W_BF16>(hi.x, v + 4);
-    decode_dword<LX_W_BF16>(hi.y, v + 6);
-  } else {
+    r.w[0] = u32x4{lo.x, lo.y, hi.x, hi.y};
+  } else if (wide) {
     const float* const f = static_cast<const float*>(x) + at;
-    const f32x4 lo = *reinterpret_cast<const f32x4*>(f + n.a), hi = *reinterpret_cast<const f32x4*>(f + n.b);
+    r.w[0] = *reinterpret_cast<const u32x4*>(f + n.a);
+    r.w[1] = *reinterpret_cast<const u32x4*>(f + n.b);
+  } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[j] = lo[j];
-      v[4 + j] = hi[j];
+      r.w[0][j] = __float_as_uint(load_as_f32(x, dtype, at + n.a + j));
+      r.w[1][j] = __float_as_uint(load_as_f32(x, dtype, at + n.b + j));
+    }
+  }
+  return r;
+}
+
+// v[0 .. 3] and v[4 .. 7]: the two runs of four.
+template <bool HALF>
+__device__ __forceinline__ void values_of(const RawUnit<HALF>& r, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if constexpr (HALF) {
+      const uint32_t two = r.w[0][j / 2];
+      v[j] = __uint_as_float(j % 2 ? two & 0xffff0000u : two << 16);
+    } else {
+      const uint32_t one = r.w[j / 4][j % 4];
+      v[j] = __uint_as_float(one);
     }
   }
 }
 
+template <bool HALF>
 __device__ __forceinline__ void store_unit(void* x, int dtype, bool wide, int64_t at, const Unit& n, const float* v) {
-  if (wide && dtype == LX_BF16) {
-    uint16_t* const h = static_cast<uint16_t*>(x) + at;
-    auto two = [&](int j) { return f32_to_bf16_bits(v[j]) | static_cast<uint32_t>(f32_to_bf16_bits(v[j + 1])) << 16; };
-    *reinterpret_cast<u32x2*>(h + n.a) = u32x2{two(0), two(2)};
-    *reinterpret_cast<u32x2*>(h + n.b) = u32x2{two(4), two(6)};
-  } else if (wide) {
-    float* const f = static_cast<float*>(x) + at;
-    *reinterpret_cast<f32x4*>(f + n.a) = f32x4{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4*>(f + n.b) = f32x4{v[4], v[5], v[6], v[7]};
+  if (HALF || wide) {
+    if (dtype == LX_BF16) {
+      uint16_t* const h = static_cast<uint16_t*>(x) + at;
+      auto two = [&](int j) { return __builtin_bit_cast(uint32_t, pack_bf16(v[j], v[j + 1])); };
+      *reinterpret_cast<u32x2*>(h + n.a) = u32x2{two(0), two(2)};
+      *reinterpret_cast<u32x2*>(h + n.b) = u32x2{two(4), two(6)};
+    } else {
+      float* const f = static_cast<float*>(x) + at;
+      *reinterpret_cast<f32x4*>(f + n.a) = f32x4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4*>(f + n.b) = f32x4{v[4], v[5], v[6], v[7]};
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -86,21 +113,33 @@ __device__ __forceinline__ void store_unit(void* x, int dtype, bool wide, int64_
   }
 }
 
-// The cosines and sines of a unit's four angles position * freq. The product of a 31-bit and a 24-bit number is right to
-// 2^-53 in 64 bits; whole turns are taken off it there, in two steps, so what is left of a far position is as good as of a
-// near one. The rest r is split into an f32 and what that lacks: cos(r + e) = cos r - e sin r.
-__device__ __forceinline__ void angles(const float* freq, int pair, int position, float* c, float* s) {
-  constexpr double kTurn = 6.283185307179586477, kTurnRest = 2.4492935982947064e-16, kPerTurn = 0.15915494309189533577;
+// Quarter turns a position of a unit's four frequencies.
+__device__ __forceinline__ void quarters_of(const AppendArgs& p, const Unit& n, int pair, double (&quarters)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) quarters[j] = n.turned ? static_cast<double>(p.freq[pair + j]) * 0.63661977236758134308 : 0.0;
+}
+
+// The cosines and sines of the four angles at a position. The product of a 31-bit and a 53-bit number is right to 2^-53 in 64 bits;
+// whole quarter turns are taken off it there, so what is left of a far position is as good as of a near one. The rest u, an
+// eighth of a turn at most, goes into Taylor's series in f32 (what they leave off is below 2^-29 and 2^-32).
+__device__ __forceinline__ void angles(const double (&quarters)[4], int position, float* c, float* s) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const double angle = static_cast<double>(position) * static_cast<double>(freq[pair + j]);
-    const double turns = rint(angle * kPerTurn);
-    const double r = fma(-turns, kTurnRest, fma(-turns, kTurn, angle));
-    const float near = static_cast<float>(r), rest = static_cast<float>(r - static_cast<double>(near));
-    float sin_near, cos_near;
-    sincosf(near, &sin_near, &cos_near);
-    c[j] = __builtin_fmaf(-rest, sin_near, cos_near);
-    s[j] = __builtin_fmaf(rest, cos_near, sin_near);
+    const double turned = static_cast<double>(position) * quarters[j], whole = rint(turned);
+    const float u = static_cast<float>((turned - whole) * 1.57079632679489661923), x = u * u;
+    float a = __builtin_fmaf(x, 1.0f / 362880.0f, -1.0f / 5040.0f), b = __builtin_fmaf(x, -1.0f / 3628800.0f, 1.0f / 40320.0f);
+    a = __builtin_fmaf(x, a, 1.0f / 120.0f);
+    b = __builtin_fmaf(x, b, -1.0f / 720.0f);
+    a = __builtin_fmaf(x, a, -1.0f / 6.0f);
+    b = __builtin_fmaf(x, b, 1.0f / 24.0f);
+    a = __builtin_fmaf(x * u, a, u);  // sin u
+    b = __builtin_fmaf(x, b, -0.5f);
+    b = __builtin_fmaf(x, b, 1.0f);  // cos u
+    const int quadrant = static_cast<int>(static_cast<long long>(whole)) & 3;
+    c[j] = quadrant & 1 ? a : b;
+    s[j] = quadrant & 1 ? b : a;
+    if (quadrant == 1 || quadrant == 2) c[j] = -c[j];
+    if (quadrant >= 2) s[j] = -s[j];
   }
 }
 
@@ -144,143 +183,212 @@ __device__ __forceinline__ uint32_t encode_four(const float* v, float inverse) {
   }
 }
 
-// Which sequence row r belongs to, or -1: the sequences' bounds are looked at by all threads at once.
-template <int kThreads>
-__device__ int sequence_of(const Kv8Batch& b, int r, int* found) {
-  if (!b.rows) return r < b.seqs ? r : -1;
-  __syncthreads();
-  if (threadIdx.x == 0) *found = -1;
-  __syncthreads();
-  for (int s = threadIdx.x; s < b.seqs; s += kThreads) {
-    const int first = clamp_int(b.rows[s], 0, b.T), end = clamp_int(b.rows[s + 1], 0, b.T);
-    if (r >= first && r < end) *found = s;
+// The sequence row r belongs to, or -1, and its rows and length: a lane a sequence, in every wavefront by itself.
+__device__ __forceinline__ int sequence_of(const Kv8Batch& b, int page, int r, Kv8Span& span) {
+  if (!b.rows) {
+    if (r >= b.seqs) return -1;
+    span = kv8_span_of(b, page, r, r + 1, b.lengths[r]);
+    return r;
   }
-  __syncthreads();
-  return *found;
+  const int lane = threadIdx.x % kWave;
+  for (int base = 0; base < b.seqs; base += kWave) {
+    const int s = min(base + lane, b.seqs - 1);
+    const int from = b.rows[s], to = b.rows[s + 1], length = b.lengths[s];
+    const uint64_t here = __ballot(base + lane < b.seqs && r >= clamp_int(from, 0, b.T) && r < clamp_int(to, 0, b.T));
+    if (here) {
+      const int l = __builtin_ctzll(here);
+      span = kv8_span_of(b, page, __builtin_amdgcn_readlane(from, l), __builtin_amdgcn_readlane(to, l), __builtin_amdgcn_readlane(length, l));
+      return base + l;
+    }
+  }
+  return -1;
 }
 
-// blockIdx.x: rows; blockIdx.y: the cache's head, whose query heads it rotates too.
-template <int F, int kThreads>
+constexpr int kQueryHeads = 4;  // of a workgroup that turns queries
+
+// The queries of rows first .. stop - 1 (no more than the workgroup has slots), heads q_head .. q_head + heads - 1. A thread's slot is
+// a row, whose angles it makes once for all heads, or (where a workgroup has one row) a head. What it turns is asked for before
+// its row's place is looked up.
+template <int kThreads, bool HALF>
+__device__ __forceinline__ void turn_queries(const AppendArgs& p, int first, int stop, int q_head, int heads) {
+  const int dim = p.c.dim, units = dim / 8, slots = kThreads / units, slot = threadIdx.x / units;
+  const bool one = stop - first == 1;
+  const int base = one ? slot : 0, step = one ? slots : 1, row = one ? first : first + slot;
+  const Unit n = unit_of(p, threadIdx.x % units);
+  double quarters[4];
+  quarters_of(p, n, 4 * (threadIdx.x % units), quarters);
+  RawUnit<HALF> raw[kQueryHeads];
+  const int64_t at = static_cast<int64_t>(q_head) * dim;
+#pragma unroll
+  for (int k = 0; k < kQueryHeads; ++k) {
+    if (k > 0 && k * step >= heads) break;
+    raw[k] = load_unit<HALF>(p.q, p.dtype, p.wide, min(row, p.b.T - 1) * p.ld_q + at + min(base + k * step, heads - 1) * dim, n);
+  }
+  int position = -1;
+  for (int r = first; r < stop;) {
+    Kv8Span span;
+    if (sequence_of(p.b, p.c.page, r, span) < 0) {
+      ++r;
+      continue;
+    }
+    const int end = min(stop, span.row0 + span.rows);
+    if (row >= r && row < end && row - span.row0 < p.b.max_rows) position = span.length - span.rows + (row - span.row0);
+    r = end;
+  }
+  if (position < 0 || slot >= slots) return;
+  float c4[4], s4[4];
+  angles(quarters, position, c4, s4);
+#pragma unroll
+  for (int k = 0; k < kQueryHeads; ++k) {
+    const int head = base + k * step;
+    if (head >= heads) break;
+    float q8[8];
+    values_of(raw[k], q8);
+    if (n.turned) turn(p.interleaved, c4, s4, q8);
+    store_unit<HALF>(p.q_out, p.out_dtype, p.wide, row * p.ld_out + at + head * dim, n, q8);
+    __builtin_amdgcn_sched_barrier(0);  // one head after another: all at once take 210 registers
+  }
+}
+
+// The first workgroups are some rows and one of the cache's heads each, those behind them (from `queries` on) some rows and four
+// query heads. P: tokens of a block that a thread holds values of.
+template <int F, int kThreads, int P, bool HALF>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs p) {
   constexpr float kTop = F == LX_W_INT8 ? 127.0f : 448.0f;
-  __shared__ int found;
   __shared__ float tops[2][kThreads / kWave];
   const Kv8Cache& c = p.c;
-  const int dim = c.dim, units = dim / 8, slots = kThreads / units;
-  const int slot = threadIdx.x / units, head = blockIdx.y;
+  if (blockIdx.x >= p.queries) {
+    const unsigned fours = (p.q_heads + kQueryHeads - 1) / kQueryHeads, which = blockIdx.x - p.queries;
+    const int q_head = which % fours * kQueryHeads, from = which / fours * p.query_rows;
+    turn_queries<kThreads, HALF>(p, from, min(p.b.T, from + p.query_rows), q_head, min(kQueryHeads, p.q_heads - q_head));
+    return;
+  }
+  const int first = blockIdx.x / c.heads * p.rows_per_group, stop = min(p.b.T, first + p.rows_per_group);
+  const int dim = c.dim, units = dim / 8, slots = kThreads / units, slot = threadIdx.x / units, head = blockIdx.x % c.heads;
   const bool busy = slot < slots;
   const Unit n = unit_of(p, threadIdx.x % units);
   const int pair = 4 * (threadIdx.x % units);
-  const int stop = min(p.b.T, static_cast<int>(blockIdx.x + 1) * p.rows_per_group);
-  for (int r = blockIdx.x * p.rows_per_group; r < stop;) {
-    const int s = sequence_of<kThreads>(p.b, r, &found);
+  double quarters[4];
+  quarters_of(p, n, pair, quarters);
+  RawUnit<HALF> keys[P], values[P];
+  auto ask = [&](int row0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if (i > 0 && i * slots >= p.tokens) break;
+      const int64_t row = min(row0 + slot + i * slots, p.b.T - 1);
+      keys[i] = load_unit<HALF>(p.k, p.dtype, p.wide, row * p.ld_k + head * dim, n);
+      values[i] = load_unit<HALF>(p.v, p.dtype, p.wide, row * p.ld_v + head * dim, n);
+    }
+  };
+  const bool early = p.rows_per_group == 1;  // the row is likely to begin a piece
+  if (early) ask(first);
+  for (int r = first; r < stop;) {
+    Kv8Span span;
+    const int s = sequence_of(p.b, c.page, r, span);
     if (s < 0) {
       ++r;
       continue;
     }
-    const Kv8Span span = kv8_span(p.b, c.page, s);
-    const Kv8Piece piece = kv8_piece(span, c.block_shift, r);
+    const Kv8Piece piece = kv8_piece(span, p.b.max_rows, c.block_shift, r);
     if (!piece.own) {
       r = piece.next;
       continue;
     }
-    const int lead = span.length - span.rows, position = piece.position, begin = piece.begin, end = piece.end, next = piece.next;
+    const int position = piece.position, begin = piece.begin, tokens = piece.end - piece.position;
+    if (!early) ask(r);
     const int page = kv8_page(c, p.b, s, begin);
-    float c4[4], s4[4], k8[8], v8[8], top_k = 0.0f, top_v = 0.0f;
-    auto keys = [&](int t) {
-      const int64_t row = span.row0 + (t - lead);
-      load_unit(p.k, p.dtype, p.wide, row * p.ld_k + head * dim, n, k8);
-      load_unit(p.v, p.dtype, p.wide, row * p.ld_v + head * dim, n, v8);
-      if (n.turned) {
-        angles(p.freq, pair, t, c4, s4);
-        turn(p.interleaved, c4, s4, k8);
-      }
-    };
-    for (int t = position + slot; busy && t < end; t += slots) {
-      keys(t);
-      top_k = top_of(k8, top_k);
-      top_v = top_of(v8, top_v);
-      if (p.q) {
-        const int64_t row = span.row0 + (t - lead);
-        for (int g = 0; g < p.group; ++g) {
-          const int at = (head * p.group + g) * dim;
-          float q8[8];
-          load_unit(p.q, p.dtype, p.wide, row * p.ld_q + at, n, q8);
-          if (n.turned) turn(p.interleaved, c4, s4, q8);
-          store_unit(p.q_out, p.out_dtype, p.wide, row * p.ld_out + at, n, q8);
+    r = piece.next;
+    if (page < 0) continue;
+    const int64_t row0 = kv8_row(c, page, head) + begin % c.page;  // the block's first token row
+    float* const scales[2] = {const_cast<float*>(c.k_scale) + (row0 >> c.block_shift), const_cast<float*>(c.v_scale) + (row0 >> c.block_shift)};
+    const bool kept = position > begin;
+    const float held[2] = {*scales[0], *scales[1]};
+    const float old[2] = {kept ? held[0] : 0.0f, kept ? held[1] : 0.0f};
+    float k8[P][8], top[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float v8[8];
+      values_of(keys[i], k8[i]);
+      values_of(values[i], v8);
+      const int token = slot + i * slots;
+      if (busy && token < tokens) {
+        if (n.turned) {
+          float c4[4], s4[4];
+          angles(quarters, position + token, c4, s4);
+          turn(p.interleaved, c4, s4, k8[i]);
         }
+        top[0] = top_of(k8[i], top[0]);
+        top[1] = top_of(v8, top[1]);
       }
     }
-    if (page >= 0) {
-      top_k = wave_max(top_k);
-      top_v = wave_max(top_v);
-      __syncthreads();
-      if (threadIdx.x % kWave == 0) {
-        tops[0][threadIdx.x / kWave] = top_k;
-        tops[1][threadIdx.x / kWave] = top_v;
-      }
-      const int64_t row0 = kv8_row(c, page, head) + begin % c.page;  // the block's first token row
-      const int64_t at = row0 >> c.block_shift;
-      float* const scales[2] = {const_cast<float*>(c.k_scale) + at, const_cast<float*>(c.v_scale) + at};
-      const bool kept = position > begin;
-      const float old[2] = {kept ? *scales[0] : 0.0f, kept ? *scales[1] : 0.0f};
-      __syncthreads();
-      float scale[2], inverse[2];
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        float top = tops[part][0];
+    for (int part = 0; part < 2; ++part) top[part] = wave_max(top[part]);
+    // The barriers also part the scales as every thread has read them from those that one writes.
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) {
+      tops[0][threadIdx.x / kWave] = top[0];
+      tops[1][threadIdx.x / kWave] = top[1];
+    }
+    __syncthreads();
+    float inverse[2];
 #pragma unroll
-        for (int w = 1; w < kThreads / kWave; ++w) top = fmaxf(top, tops[part][w]);
-        scale[part] = top > 0.0f ? fmaxf(top / kTop, 0x1p-126f) : 0.0f;
-        // Every thread has read the old scales before the barrier; one writes the new ones.
-        scale[part] = fmaxf(scale[part], old[part]);
-        inverse[part] = scale[part] > 0.0f ? 1.0f / scale[part] : 0.0f;
-        if (threadIdx.x == 0) *scales[part] = scale[part];
+    for (int part = 0; part < 2; ++part) {
+      float most = tops[part][0];
+#pragma unroll
+      for (int w = 1; w < kThreads / kWave; ++w) most = fmaxf(most, tops[part][w]);
+      const float scale = fmaxf(most > 0.0f ? fmaxf(most / kTop, 0x1p-126f) : 0.0f, old[part]);
+      inverse[part] = scale > 0.0f ? 1.0f / scale : 0.0f;
+      if (threadIdx.x == 0) *scales[part] = scale;
+      if (scale > old[part]) {  // the tokens that stay: none where kept is false
         uint8_t* const codes = const_cast<uint8_t*>(part ? c.v : c.k) + row0 * dim;
-        if (scale[part] > old[part]) {  // the tokens that stay: none where kept is false
-          const float factor = old[part] / scale[part];
-          for (int i = threadIdx.x; i < (position - begin) * units; i += kThreads) {
-            u32x2* const word = reinterpret_cast<u32x2*>(codes) + i;
-            const u32x2 was = *word;
-            float v[8];
-            decode_dword<F>(was.x, v);
-            decode_dword<F>(was.y, v + 4);
-            *word = u32x2{encode_four<F>(v, factor), encode_four<F>(v + 4, factor)};
-          }
+        const float factor = old[part] / scale;
+        for (int i = threadIdx.x; i < (position - begin) * units; i += kThreads) {
+          u32x2* const word = reinterpret_cast<u32x2*>(codes) + i;
+          const u32x2 was = *word;
+          float v[8];
+          decode_dword<F>(was.x, v);
+          decode_dword<F>(was.y, v + 4);
+          *word = u32x2{encode_four<F>(v, factor), encode_four<F>(v + 4, factor)};
         }
       }
-      for (int t = position + slot; busy && t < end; t += slots) {
-        keys(t);
-        const int64_t row = (row0 + (t - begin)) * dim;
-        uint8_t* const kc = const_cast<uint8_t*>(c.k) + row;
-        uint8_t* const vc = const_cast<uint8_t*>(c.v) + row;
-        *reinterpret_cast<uint32_t*>(kc + n.a) = encode_four<F>(k8, inverse[0]);
-        *reinterpret_cast<uint32_t*>(kc + n.b) = encode_four<F>(k8 + 4, inverse[0]);
-        *reinterpret_cast<uint32_t*>(vc + n.a) = encode_four<F>(v8, inverse[1]);
-        *reinterpret_cast<uint32_t*>(vc + n.b) = encode_four<F>(v8 + 4, inverse[1]);
-      }
     }
-    r = next;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int token = slot + i * slots;
+      if (!busy || token >= tokens) continue;
+      float v8[8];
+      values_of(values[i], v8);
+      const int64_t row = (row0 + (position - begin) + token) * dim;
+      uint8_t* const kc = const_cast<uint8_t*>(c.k) + row;
+      uint8_t* const vc = const_cast<uint8_t*>(c.v) + row;
+      *reinterpret_cast<uint32_t*>(kc + n.a) = encode_four<F>(k8[i], inverse[0]);
+      *reinterpret_cast<uint32_t*>(kc + n.b) = encode_four<F>(k8[i] + 4, inverse[0]);
+      *reinterpret_cast<uint32_t*>(vc + n.a) = encode_four<F>(v8, inverse[1]);
+      *reinterpret_cast<uint32_t*>(vc + n.b) = encode_four<F>(v8 + 4, inverse[1]);
+    }
   }
 }
 
-// Sixteen codes a thread: 16 bytes in, 32 out.
+// Sixteen codes a thread: 16 bytes in, 32 out; keys, then values.
 template <int F>
-__global__ void __launch_bounds__(256) dequantize_cache_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scale,
-                                                               uint16_t* __restrict__ out, int64_t pieces, int pieces_per_block_row,
-                                                               int block_shift) {
+__global__ void __launch_bounds__(256) dequantize_cache_kernel(const Kv8Cache c, uint16_t* k, uint16_t* v, int64_t pieces) {
   const int64_t i = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x;
-  if (i >= pieces) return;
-  const u32x4 w = reinterpret_cast<const u32x4*>(codes)[i];
-  const float s = scale[i / pieces_per_block_row >> block_shift];
+  const bool values = blockIdx.y == 1;
+  uint16_t* const out = values ? v : k;
+  if (i >= pieces || !out) return;
+  const u32x4 w = reinterpret_cast<const u32x4*>(values ? c.v : c.k)[i];
+  const int per_row = c.dim / 16;
+  // A head's pieces of a row are few: no division of 64 bits by what is no power of two but 192 / 16.
+  const int64_t row = per_row == 12 ? i / 12 : i >> (per_row == 4 ? 2 : per_row == 8 ? 3 : 4);
+  const float s = (values ? c.v_scale : c.k_scale)[row >> c.block_shift];
   u32x4 out4[2];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    float v[4];
+    float x[4];
     const uint32_t d = w[j];
-    decode_dword<F>(d, v);
-    out4[j / 2][2 * (j & 1)] = f32_to_bf16_bits(v[0] * s) | static_cast<uint32_t>(f32_to_bf16_bits(v[1] * s)) << 16;
-    out4[j / 2][2 * (j & 1) + 1] = f32_to_bf16_bits(v[2] * s) | static_cast<uint32_t>(f32_to_bf16_bits(v[3] * s)) << 16;
+    decode_dword<F>(d, x);
+    out4[j / 2][2 * (j & 1)] = __builtin_bit_cast(uint32_t, pack_bf16(x[0] * s, x[1] * s));
+    out4[j / 2][2 * (j & 1) + 1] = __builtin_bit_cast(uint32_t, pack_bf16(x[2] * s, x[3] * s));
   }
   reinterpret_cast<u32x4*>(out)[2 * i] = out4[0];
   reinterpret_cast<u32x4*>(out)[2 * i + 1] = out4[1];
@@ -290,18 +398,36 @@ bool aligned(const void* p, int64_t ld, int dtype) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (dtype == LX_BF16 ? 2 : 4) % 16 == 0;
 }
 
-// Rows a workgroup looks at: about as many as a sequence has, so that about one block begins there, up to a block's.
+// Rows a workgroup looks at. Short sequences: one, which mostly begins a piece or goes with the one before it (8 sequences of 5 rows
+// by fours: 10.6 us, workgroups that look for several sequences one after another; one by one: 7). Longer ones: about as
+// many as a sequence has, up to a block's, so that about one piece begins there.
 int rows_per_group(int block, int seqs, int T) {
+  const int each = T / (seqs > 0 ? seqs : 1);
   int n = 1;
-  while (n < block && 2 * n <= T / (seqs > 0 ? seqs : 1)) n *= 2;
+  while (each >= 16 && n < block && 2 * n <= each) n *= 2;
   return n;
 }
 
-template <int F>
-int append(const AppendArgs& p, hipStream_t stream) {
-  const dim3 grid((p.b.T + p.rows_per_group - 1) / p.rows_per_group, p.c.heads);
-  hipLaunchKernelGGL((append_kernel<F, 256>), grid, dim3(256), 0, stream, p);
+template <int F, int kThreads, int P, bool HALF>
+int launch(AppendArgs p, hipStream_t stream) {
+  const int slots = kThreads / (p.c.dim / 8);
+  p.query_rows = p.rows_per_group < slots ? p.rows_per_group : slots;
+  const int64_t keys = static_cast<int64_t>((p.b.T + p.rows_per_group - 1) / p.rows_per_group) * p.c.heads;
+  const int64_t queries = static_cast<int64_t>((p.b.T + p.query_rows - 1) / p.query_rows) * ((p.q_heads + kQueryHeads - 1) / kQueryHeads);
+  if (keys + queries > 0x7fffffff) return fail(kInvalid);
+  p.queries = static_cast<unsigned>(keys);
+  hipLaunchKernelGGL((append_kernel<F, kThreads, P, HALF>), dim3(static_cast<unsigned>(keys + queries)), dim3(kThreads), 0, stream, p);
   return status_of(hipGetLastError());
+}
+
+// The fewest threads that hold a block's part in P tokens each.
+template <int F, bool HALF>
+int append(const AppendArgs& p, hipStream_t stream) {
+  const int units = p.c.dim / 8;
+  if (p.tokens <= 64 / units) return launch<F, 64, 1, HALF>(p, stream);
+  if (p.tokens <= 2 * (256 / units)) return launch<F, 256, 2, HALF>(p, stream);
+  if (p.tokens <= 4 * (512 / units)) return launch<F, 512, 4, HALF>(p, stream);
+  return launch<F, 1024, 4, HALF>(p, stream);
 }
 
 }  // namespace
@@ -318,7 +444,7 @@ int lx_kv8_append(const lx_kv8* cache, const lx_kv8_batch* batch, const void* q,
   if (int st = kv8_check_batch(batch, T)) return fail(st);
   if ((dtype != LX_F32 && dtype != LX_BF16) || (q && q_out_dtype != LX_F32 && q_out_dtype != LX_BF16)) return fail(kInvalid);
   if (rot < 0 || rot > cache->dim || rot % 8 != 0) return fail(kInvalid);
-  if (T == 0 || batch->seqs == 0) return kOk;
+  if (T == 0 || batch->seqs == 0 || batch->max_rows == 0) return kOk;
   if (!k || !v || (rot > 0 && !freq) || !q != !q_out) return fail(kInvalid);
   const int64_t kv = static_cast<int64_t>(cache->heads) * cache->dim, width = static_cast<int64_t>(q_heads) * cache->dim;
   if (q && (q_heads < 1 || q_heads % cache->heads != 0 || q_heads > 65536)) return fail(kInvalid);
@@ -329,11 +455,14 @@ int lx_kv8_append(const lx_kv8* cache, const lx_kv8_batch* batch, const void* q,
   p.q = q, p.k = k, p.v = v, p.q_out = q_out, p.freq = freq;
   p.ld_q = ld_q, p.ld_k = ld_k, p.ld_v = ld_v, p.ld_out = ld_q_out;
   p.dtype = dtype, p.out_dtype = q_out_dtype, p.rot = rot, p.interleaved = interleaved != 0;
-  p.group = q ? q_heads / cache->heads : 0;
+  p.q_heads = q ? q_heads : 0;
   p.wide = aligned(k, ld_k, dtype) && aligned(v, ld_v, dtype) && (!q || (aligned(q, ld_q, dtype) && aligned(q_out, ld_q_out, q_out_dtype)));
+  p.tokens = p.b.max_rows < cache->block ? p.b.max_rows : cache->block;
   p.rows_per_group = rows_per_group(cache->block, batch->seqs, T);
   hipStream_t s = as_stream(stream);
-  return cache->type == LX_W_INT8 ? append<LX_W_INT8>(p, s) : append<LX_W_FP8>(p, s);
+  const bool half = p.wide && dtype == LX_BF16;
+  if (cache->type == LX_W_INT8) return half ? append<LX_W_INT8, true>(p, s) : append<LX_W_INT8, false>(p, s);
+  return half ? append<LX_W_FP8, true>(p, s) : append<LX_W_FP8, false>(p, s);
 }
 
 int lx_kv8_dequantize(const lx_kv8* cache, void* k, void* v, void* stream) {
@@ -342,19 +471,14 @@ int lx_kv8_dequantize(const lx_kv8* cache, void* k, void* v, void* stream) {
   const Kv8Cache c = kv8_cache(*cache);
   const int64_t pieces = static_cast<int64_t>(c.pages) * c.heads * c.page * (c.dim / 16);
   if ((pieces + 255) / 256 > 0x7fffffff) return fail(kInvalid);
-  const dim3 grid(static_cast<unsigned>((pieces + 255) / 256));
-  for (int part = 0; part < 2; ++part) {
-    void* const out = part ? v : k;
-    if (!out) continue;
-    auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, as_stream(stream), part ? c.v : c.k, part ? c.v_scale : c.k_scale,
-                         static_cast<uint16_t*>(out), pieces, c.dim / 16, c.block_shift);
-    };
-    if (cache->type == LX_W_INT8) go(dequantize_cache_kernel<LX_W_INT8>);
-    else go(dequantize_cache_kernel<LX_W_FP8>);
-    if (int st = status_of(hipGetLastError())) return st;
-  }
-  return kOk;
+  if (!k && !v) return kOk;
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((pieces + 255) / 256), 2), dim3(256), 0, as_stream(stream), c, static_cast<uint16_t*>(k),
+                       static_cast<uint16_t*>(v), pieces);
+  };
+  if (cache->type == LX_W_INT8) go(dequantize_cache_kernel<LX_W_INT8>);
+  else go(dequantize_cache_kernel<LX_W_FP8>);
+  return status_of(hipGetLastError());
 }
 
 // For tests, on host memory and without a device: what the kernel makes of a call's rows. Every piece that it stores, as
@@ -376,7 +500,7 @@ LX_API int dromos_kv8_pieces(const lx_kv8* cache, const lx_kv8_batch* batch, int
         ++r;
         continue;
       }
-      const Kv8Piece piece = kv8_piece(kv8_span(b, c.page, s), c.block_shift, r);
+      const Kv8Piece piece = kv8_piece(kv8_span(b, c.page, s), b.max_rows, c.block_shift, r);
       if (piece.own) {
         const int five[5] = {s, piece.position, kv8_page(c, b, s, piece.begin), piece.end - piece.position, r};
         for (int i = 0; i < 5 && n < capacity; ++i) out[5 * n + i] = five[i];

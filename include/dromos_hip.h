@@ -239,8 +239,8 @@ LX_API int lx_moe_experts_noalloc(const void* latent, const int32_t* ids, const 
  *            the last sequence belong to nobody and stay as they were); null: one row a sequence, row s
  *   lengths  [seqs] tokens of each sequence in the cache, this call's rows (its last ones) among them; 0 is fine
  *   table    [seqs, ld_table] page number of the tokens [i * page, (i + 1) * page) of a sequence
- *   max_rows, max_length   at least the most rows and the greatest length of any sequence (rows and tokens beyond them are not attended
- *            to). They and T size the launch: a captured call replays with whatever rows, lengths and table hold then, within them.
+ *   max_rows, max_length   at least the most rows and the greatest length of any sequence (rows beyond are left alone, tokens beyond do
+ *            not count). They and T size the launch: a captured call replays with whatever rows, lengths and table hold then, within them.
  * The numbers in device memory are not refused but bounded: a page number outside [0, pages) is a page without tokens (nothing is
  * stored, nothing attended), rows end at T, lengths at max_length and at the table's end; a row in front of position 0 is not
  * stored and attends to nothing.

@@ -177,11 +177,7 @@ __device__ __forceinline__ void store_four(const AttentionArgs& p, int64_t at, f
 template <int F, int DIM, int RT>
 __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const AttentionArgs p) {
   constexpr int kC = DIM / 64, kTiles = DIM / 16, kPerTile = 16 * RT, kRuns = step_runs<DIM>(), kStep = kRuns * kRun;
-  __shared__ int run_of[kMaxRuns];
-  __shared__ float key_scale[kMaxRuns], value_log[kMaxRuns];
   __shared__ float wave_top[kStreamWaves][kPerTile], wave_sum_of[kStreamWaves][kPerTile];
-  __shared__ float scale_top[kStreamWaves];
-  __shared__ int hole_in[kStreamWaves];
   __shared__ float sums[kStreamWaves][16][DIM + 4];
   const Kv8Cache& c = p.c;
   const int head = blockIdx.x % c.heads;
@@ -192,18 +188,16 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
   const int lane = threadIdx.x % kWave, g = lane / 16, i = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 
-  // A part begins at a multiple of its length unless a window moves it, so its line of the page table is asked for together with
-  // the sequence's bounds: a thread's run of the part, and (lanes 0 .. 3) those that its wavefront begins with.
+  // A lane holds one run of its wavefront's: lane kRuns * e + j run j of its step e, so the runs and scales that a step needs
+  // come out of registers. A part begins at a multiple of its length unless a window moves it, so its line of the page table is
+  // asked for together with the sequence's bounds.
+  static_assert(kMaxRuns == kStreamWaves * kWave, "a lane a run");
+  const int mine = (lane / kRuns * kStreamWaves + wave) * kRuns + lane % kRuns;
   const int32_t* const line = p.b.table + static_cast<int64_t>(seq) * p.b.ld_table;
   const int most = p.b.ld_table - 1;
   auto page_of = [&](int64_t token) { return line[min(static_cast<int>(token / c.page), most)]; };
-  const int64_t guess = static_cast<int64_t>(split) * p.chunk;
-  const int mine = threadIdx.x, first_mine = wave * kRuns + lane % kRuns;
-  int page = -1, first_page = -1;
-  if (most >= 0 && p.window == 0) {
-    if (mine < kMaxRuns) page = page_of(guess + kRun * mine);
-    first_page = page_of(guess + kRun * first_mine);
-  }
+  int page = -1;
+  if (most >= 0 && p.window == 0) page = page_of(static_cast<int64_t>(split) * p.chunk + kRun * mine);
   const RowTile t = row_tile(p, seq, tile, kPerTile);
   if (t.count <= 0) return;
   const int64_t start = t.begin + static_cast<int64_t>(split) * p.chunk;
@@ -212,17 +206,9 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
   const int token0 = static_cast<int>(start), stop = static_cast<int>(min(start + p.chunk, static_cast<int64_t>(t.end)));
   const int runs = (stop - token0 + kRun - 1) / kRun;  // none where the rows see nothing
   const int steps = (runs + kRuns - 1) / kRuns;
-  if (p.window > 0) {
-    if (mine < runs) page = page_of(token0 + kRun * mine);
-    if (first_mine < runs) first_page = page_of(token0 + kRun * first_mine);
-  }
-  // The run of 16 tokens number e of the part, -1 where there is none or no page.
-  auto run_at = [&](int e, int page) {
-    if (e >= runs || page < 0 || page >= c.pages) return -1;
-    return static_cast<int>((kv8_row(c, page, head) + (token0 + kRun * e) % c.page) / kRun);
-  };
-
-  const int run = run_at(mine, page);
+  if (p.window > 0 && mine < runs) page = page_of(token0 + kRun * mine);
+  int run = -1;  // where the run lies; none, or none of the cache's pages: no tokens
+  if (mine < runs && page >= 0 && page < c.pages) run = static_cast<int>((kv8_row(c, page, head) + (token0 + kRun * mine) % c.page) / kRun);
   const int64_t scale_at = static_cast<int64_t>(max(run, 0)) * kRun >> c.block_shift;
   const float ks = c.k_scale[scale_at], vs = c.v_scale[scale_at];
   const int key_off = i * DIM + 16 * g, value_off = 4 * g * DIM + i * (DIM / 16);
@@ -237,9 +223,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
     for (int j = 0; j < kRuns; ++j) load_values<DIM>(values[j], c.v + static_cast<int64_t>(max(where(j), 0)) * (kRun * DIM), value_off);
   };
   // Everything the first step needs is on its way before anything is waited for; a wavefront without a step reads run 0.
-  const int first_run = run_at(first_mine, first_page);
-  auto first_where = [&](int j) { return __builtin_amdgcn_readlane(first_run, j); };
-  ask_keys(first_where);
+  auto run_in = [&](int e) { return [&, e](int j) { return __builtin_amdgcn_readlane(run, e * kRuns + j); }; };
+  ask_keys(run_in(0));
   // The rows' queries: row 16 r + i, dims 64 c + 16 g + 8 h .. + 8 (the key's bytes of the same lane group).
   bf16x8 q[RT][2 * kC];
   int pos[RT];
@@ -251,32 +236,15 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
     const int64_t at = have ? (t.span.row0 + token) * p.ld_q + static_cast<int64_t>(head * p.group + flat % p.group) * DIM : 0;
     load_query(p, have, at, [&](int k) { return 64 * (k / 2) + 16 * g + 8 * (k % 2); }, q[r]);
   }
-  ask_values(first_where);
-  // Where the part's runs lie, and their scales.
+  ask_values(run_in(0));
+  // Scales of the runs: of the scores, and (as exponents, relative to the wavefront's largest) of the values and back.
   const float log_here = run >= 0 ? __builtin_amdgcn_logf(fabsf(vs)) : -__builtin_inff();
-  if (mine < runs) {
-    run_of[mine] = run;
-    key_scale[mine] = run >= 0 ? ks * fabsf(p.scale) * 1.4426950408889634f : 0.0f;
-    value_log[mine] = log_here;
-  }
-  const float largest_here = wave_max(log_here);
-  const bool hole = __any(mine < runs && run < 0);
-  if (lane == 0) {
-    scale_top[wave] = largest_here;
-    hole_in[wave] = hole;
-  }
-  __syncthreads();
-  float largest = scale_top[0];  // log2 of the part's largest value scale
-  bool whole = !hole_in[0];
-#pragma unroll
-  for (int w = 1; w < kMaxRuns / kWave; ++w) {
-    largest = fmaxf(largest, scale_top[w]);
-    whole = whole && !hole_in[w];
-  }
+  float largest = wave_max(log_here);
   if (largest == -__builtin_inff()) largest = 0.0f;  // every scale 0
-  auto run_in = [&](int step) {
-    return [&, step](int j) { return __builtin_amdgcn_readfirstlane(run_of[min(step * kRuns + j, runs - 1)]); };
-  };
+  const float key_scale = ks * fabsf(p.scale) * 1.4426950408889634f;
+  const float value_exp = fmaxf(log_here - largest, kLeastScale) + kWeightBits, value_per = __builtin_amdgcn_exp2f(-value_exp);
+  const bool whole = !__any(mine < runs && run < 0);
+  auto from_lane = [](float v, int from) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), from)); };
 
   f32x4 acc[RT][kTiles] = {};
   float top[RT], total[RT];
@@ -285,7 +253,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
     top[r] = -__builtin_inff();
     total[r] = 0.0f;
   }
-  for (int step = wave; step < steps; step += kStreamWaves) {
+  for (int e = 0, step = wave; step < steps; ++e, step += kStreamWaves) {
     const int at = token0 + step * kStep;
     f32x4 s[RT][kRuns];
 #pragma unroll
@@ -302,33 +270,32 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
         }
     }
     const bool more = step + kStreamWaves < steps;
-    if (more) ask_keys(run_in(step + kStreamWaves));
+    if (more) ask_keys(run_in(e + 1));
     // Every token of the step is seen by every row?
     const bool plain = whole && at + kStep - 1 <= t.low_pos && (p.window == 0 || at > t.high_pos - p.window);
     float ks[kRuns], ve[kRuns], per[kRuns];
 #pragma unroll
     for (int j = 0; j < kRuns; ++j) {
-      const int run = min(step * kRuns + j, runs - 1);
-      ks[j] = key_scale[run];
-      ve[j] = fmaxf(value_log[run] - largest, kLeastScale) + kWeightBits;
-      per[j] = __builtin_amdgcn_exp2f(-ve[j]);
+      ks[j] = from_lane(key_scale, e * kRuns + j);
+      ve[j] = from_lane(value_exp, e * kRuns + j);
+      per[j] = from_lane(value_per, e * kRuns + j);
     }
     if (!plain) {
 #pragma unroll
       for (int j = 0; j < kRuns; ++j) {
-        const bool there = step * kRuns + j < runs && run_of[min(step * kRuns + j, runs - 1)] >= 0;
+        const bool there = __builtin_amdgcn_readlane(run, e * kRuns + j) >= 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int token = at + kRun * j + 4 * g + e;
+        for (int k = 0; k < 4; ++k) {
+          const int token = at + kRun * j + 4 * g + k;
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
             const bool hidden = !there || token > pos[r] || (p.window > 0 && token <= pos[r] - p.window);
-            s[r][j][e] = hidden ? -__builtin_inff() : s[r][j][e] * ks[j];
+            s[r][j][k] = hidden ? -__builtin_inff() : s[r][j][k] * ks[j];
           }
           // Codes of places without a token (NaNs perhaps) times a weight of nothing have to be nothing.
           if (!there || token >= t.span.length)
 #pragma unroll
-            for (int d = 0; d < kC; ++d) values[j].w[e][d] = 0;
+            for (int d = 0; d < kC; ++d) values[j].w[k][d] = 0;
         }
         ks[j] = 1.0f;
       }
@@ -394,7 +361,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
           for (int r = 0; r < RT; ++r) acc[r][4 * d + f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, weights[r][j / 2], acc[r][4 * d + f], 0, 0, 0);
         }
       }
-    if (more) ask_values(run_in(step + kStreamWaves));
+    if (more) ask_values(run_in(e + 1));
   }
 
   // The wavefronts' sums together.

@@ -18,7 +18,7 @@ struct Plan {
 
 // Enough parts that the device has about two workgroups a compute unit, none shorter than 256 tokens (a step of each
 // wavefront); one part where sequences and heads alone make a workgroup a unit.
-Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads) {
+Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads, int window) {
   Plan p{};
   const int group = q_heads / c.heads;
   const int64_t most = b.max_rows < T ? b.max_rows : T;
@@ -32,11 +32,21 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads) {
   const int per = p.per_tile;
   p.row_tiles = static_cast<int>((rows + per - 1) / per);
   p.tile_rows = static_cast<int>(rows < per ? rows : per);
+  // What a tile's rows see: all tokens, or the window, the tile's own and the run that the window begins in.
   const int64_t held = static_cast<int64_t>(b.ld_table) * c.page;
-  const int64_t length = held < b.max_length ? held : b.max_length;
+  const int64_t whole = held < b.max_length ? held : b.max_length;
+  int64_t length = whole;
+  const int64_t windowed = static_cast<int64_t>(window) + per / group + 2 + kRun;
+  if (window > 0 && windowed < length) length = windowed;
   const int64_t items = static_cast<int64_t>(b.seqs) * p.row_tiles * c.heads;
-  int64_t want = items > 0 ? (2 * compute_units() + items - 1) / items : 1;
-  if (items >= compute_units()) want = 1;
+  // There are no more tiles with rows than T fills, and one begun for each sequence.
+  const int64_t filled = (static_cast<int64_t>(T) * group / per + b.seqs) * c.heads, busy = items < filled ? items : filled;
+  // One sequence's parts are equally long. Several are of different lengths (which only the device knows): twice as many parts
+  // then even out what the compute units have, 16 streams of up to 8192 tokens 41 -> 38 us, 8 of exactly 8192 33 -> 34. Rows in
+  // two tiles of sixteen leave room for two workgroups a unit only: 8 streams of 5 rows 28.7 us, with twice the parts 34.8.
+  const int each = b.seqs > 1 && per == 16 ? 4 : 2;
+  int64_t want = busy > 0 ? (each * compute_units() + busy - 1) / busy : 1;
+  if (busy >= compute_units()) want = 1;
   int64_t chunk = (length + want - 1) / (want > 0 ? want : 1);
   chunk = (chunk + 255) / 256 * 256;
   // Parts cost a second kernel (about 4 us); one part costs a step of each wavefront more for every 256 tokens (1.6 us).
@@ -48,7 +58,10 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads) {
   p.splits = static_cast<int>((length + chunk - 1) / chunk);
   if (p.splits < 1) p.splits = 1;
   p.workgroups = items * p.splits;
-  p.bytes = p.splits > 1 ? p.workgroups * per * (c.dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+  // The workspace is for any window: one may have as many parts as are wanted of 256 tokens, or of the longest there are.
+  int64_t parts = want < (whole + 255) / 256 ? want : (whole + 255) / 256;
+  if (!p.tiles && parts < (whole + kMaxRuns * kRun - 1) / (kMaxRuns * kRun)) parts = (whole + kMaxRuns * kRun - 1) / (kMaxRuns * kRun);
+  p.bytes = parts > 1 ? items * parts * per * (c.dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
   return p;
 }
 
@@ -98,15 +111,17 @@ int lx_kv8_attention(const void* q, lx_dtype q_dtype, int ld_q, const lx_kv8* ca
   if (T == 0 || batch->seqs == 0 || batch->max_rows == 0) return kOk;
   const int64_t width = static_cast<int64_t>(q_heads) * cache->dim;
   if (!q || !out || (T > 1 && (ld_q < width || ld_out < width))) return fail(kInvalid);
-  const Plan plan = plan_for(*cache, *batch, T, q_heads);
-  if (plan.workgroups > 0x7fffffff / kTileRowsOfGroup || (plan.bytes > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))) return fail(kInvalid);
+  const Plan plan = plan_for(*cache, *batch, T, q_heads, window);
+  if (plan.workgroups > 0x7fffffff / kTileRowsOfGroup || (plan.splits > 1 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))) return fail(kInvalid);
   AttentionArgs a{};
   a.c = kv8_cache(*cache);
   a.b = kv8_batch(*batch, T);
   a.q = q, a.out = out, a.partial = static_cast<float*>(workspace), a.ld_q = ld_q, a.ld_out = ld_out;
-  a.q_dtype = q_dtype, a.out_dtype = out_dtype, a.group = q_heads / cache->heads, a.window = window, a.scale = scale;
+  a.q_dtype = q_dtype, a.out_dtype = out_dtype, a.group = q_heads / cache->heads, a.scale = scale;
+  a.window = window >= batch->max_length ? 0 : window;  // none sees as far
   a.wide_q = q_dtype == LX_BF16 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld_q % 8 == 0;
   a.wide_out = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld_out % 4 == 0;
+  a.fold = batch->seqs == 1 && plan.workgroups <= 2 * compute_units();
   a.row_tiles = plan.row_tiles, a.splits = plan.splits, a.chunk = plan.chunk;
   return cache->type == LX_W_INT8 ? attention<LX_W_INT8>(a, plan, as_stream(stream)) : attention<LX_W_FP8>(a, plan, as_stream(stream));
 }
@@ -114,7 +129,19 @@ int lx_kv8_attention(const void* q, lx_dtype q_dtype, int ld_q, const lx_kv8* ca
 int64_t lx_kv8_attention_workspace_bytes(const lx_kv8* cache, const lx_kv8_batch* batch, int T, int q_heads) {
   if (kv8_check_cache(cache) || kv8_check_batch(batch, T) || T == 0 || batch->seqs == 0 || batch->max_rows == 0) return 0;
   if (q_heads < 1 || q_heads > 65536 || q_heads % cache->heads != 0) return 0;
-  return plan_for(*cache, *batch, T, q_heads).bytes;
+  return plan_for(*cache, *batch, T, q_heads, 0).bytes;
+}
+
+// For tests, without a device (256 compute units): {rows of a tile, tiles a sequence, parts, tokens of a part, workgroups, partial
+// sums' bytes, the workspace's bytes} of a call. Returns 0, or the status that the call is refused with.
+LX_API int dromos_kv8_plan(const lx_kv8* cache, const lx_kv8_batch* batch, int T, int q_heads, int window, int64_t* out) {
+  if (int st = kv8_check_cache(cache)) return st;
+  if (int st = kv8_check_batch(batch, T)) return st;
+  const Plan p = plan_for(*cache, *batch, T, q_heads, window);
+  out[0] = p.per_tile, out[1] = p.row_tiles, out[2] = p.splits, out[3] = p.chunk, out[4] = p.workgroups;
+  out[5] = p.splits > 1 ? p.workgroups * p.per_tile * (cache->dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+  out[6] = lx_kv8_attention_workspace_bytes(cache, batch, T, q_heads);
+  return kOk;
 }
 
 }  // extern "C"

@@ -48,6 +48,7 @@ struct AttentionArgs {
   float scale;
   int wide_q;                    // q is bf16 and can be read 16 bytes at a time
   int wide_out;                  // out can be written 8 (bf16) or 16 (f32) bytes at a time
+  int fold;                      // see kv8_tile.h
   int row_tiles, splits, chunk;  // chunk: tokens of a part, a multiple of 256, 16 * kMaxRuns at most (tiles of 128 rows: any number)
 };
 
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
     const bool more = step + kStreamWaves < steps;
     if (more) ask_keys(run_in(e + 1));
     // Every token of the step is seen by every row?
-    const bool plain = whole && at + kStep - 1 <= t.low_pos && (p.window == 0 || at > t.high_pos - p.window);
+    const bool plain = whole && at + kStep - 1 <= t.low_pos && (p.window == 0 || at > static_cast<int64_t>(t.high_pos) - p.window);
     float ks[kRuns], ve[kRuns], per[kRuns];
 #pragma unroll
     for (int j = 0; j < kRuns; ++j) {

@@ -217,6 +217,18 @@ def test_attention_windows(hip, window, rows):
     attended(hip, "int8", [rows, rows], [400, rows], window=window, dim=64, page=32, block=32)
 
 
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 2, 1 << 30])
+def test_attention_windows_wider_than_anything(hip, window):
+    for rows in ([5, 40], [1, 200]):
+        attended(hip, "fp8", rows, [3, 150], window=window, dim=64)
+
+
+def test_attention_windows_of_long_sequences(hip):
+    """Parts of a window that lies far behind the first token; tiles of few and of many rows."""
+    for rows in (1, 5, 150):
+        attended(hip, "int8", [rows, rows, 0], [9000, 700 + rows, 50], window=2100, dim=64, heads=1, group=2, spoil=False)
+
+
 @pytest.mark.parametrize("q_dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows", [1, 40])

@@ -152,3 +152,28 @@ def test_nonsense_stays_inside(lx, seed):
         assert 0 <= s < n and tokens > 0 and 0 <= row and row + tokens <= T
         assert 0 <= position and position + tokens <= min(width * page, limit) and -1 <= p < 7
         assert position // block == (position + tokens - 1) // block
+
+
+@pytest.mark.parametrize("seed", range(300))
+def test_parts_cover_what_rows_see_and_fit_the_workspace(lx, seed):
+    """How a call is cut up, on random sizes: every token that a row may see lies in one of the parts, whatever the window, and
+    the partial sums fit the workspace, whose size does not ask for the window."""
+    rng = random.Random(seed)
+    log = lambda a, b: int(round(2 ** rng.uniform(a, b)))
+    dim, block = rng.choice([64, 128, 192, 256]), rng.choice([16, 32, 64])
+    page, heads, group = block * rng.choice([1, 2, 4]), log(0, 4), rng.choice([1, 2, 4, 5, 8, 16, 17])
+    seqs, most, longest = log(0, 8), rng.choice([1, 1, log(0, 4), log(0, 13)]), log(0, 18)
+    T = min(1 << 29, rng.randint(most, most * seqs))
+    window = rng.choice([0, 0, log(0, 14), 2**31 - 1])
+    ld = rng.choice([-(-longest // page), -(-longest // page) + 3, max(0, longest // page - 1)])
+    c = cache(dim=dim, block=block, page=page, heads=heads)
+    b = batch(seqs=seqs, ld_table=ld, max_rows=most, max_length=longest)
+    out = (ctypes.c_int64 * 7)()
+    assert lx.lib.dromos_kv8_plan(c, b, T, heads * group, window, out) == 0
+    per, tiles, parts, chunk, workgroups, partial, workspace = out
+    rows, length = min(most, T) * group, min(longest, ld * page)
+    assert per in (16, 32, 128) and tiles * per >= rows and (tiles - 1) * per < rows
+    seen = length if window == 0 else min(length, window + -(-per // group) + 16)  # the tile's rows and the run it begins in
+    assert parts * chunk >= seen and chunk % 256 == 0 and (per == 128 or chunk <= 4096)
+    assert workgroups == seqs * tiles * heads * parts and partial <= workspace
+    assert parts == 1 or workspace > 0

@@ -61,8 +61,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
   constexpr int kTok = tile_tokens<DIM>(), kKeyPitch = 2 * DIM, kValuePitch = 2 * kTok;
   constexpr int kKeyBytes = kTok * kKeyPitch, kBuffer = 2 * kKeyBytes;
   extern __shared__ __attribute__((aligned(256))) uint8_t lds[];  // two buffers of keys and values
-  __shared__ int run_of[kMaxRuns];
-  __shared__ float key_scale[kMaxRuns], value_exp[kMaxRuns], value_per[kMaxRuns];
+  __shared__ __attribute__((aligned(32))) float key_scale[kMaxRuns], value_exp[kMaxRuns], value_per[kMaxRuns];
   __shared__ float scale_top[kTileWaves];
   __shared__ int holes;
   const Kv8Cache& c = p.c;
@@ -71,7 +70,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
   const int split = static_cast<int>(rest % p.splits);
   rest /= p.splits;
   // Later rows see more tokens: they go first. Where all workgroups are resident at once, two a compute unit, the second of them
-  // starts from the other end, so that a unit has a long one and a short one (16 heads of 64, 4096 rows: 75 -> 6x us).
+  // starts from the other end, so that a unit has a long one and a short one (2048 rows of 32 heads of 128: 67 -> 59 us).
   const int turn = static_cast<int>(rest % p.row_tiles), seq = static_cast<int>(rest / p.row_tiles);
   const int half = (p.row_tiles + 1) / 2;
   const int tile = p.fold && turn >= half ? turn - half : p.row_tiles - 1 - turn;
@@ -107,21 +106,23 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
   const int value_half = lane / (DIM / 4) % 2, quad = lane % (DIM / 4);
   u32x4 key_codes[kKeyLoads];
   uint32_t value_codes[8];
-  // The tile's codes on their way; it begins with run run0 of the window.
-  auto ask = [&](int run0, int runs) {
-    auto place = [&](int run) { return static_cast<int64_t>(max(__builtin_amdgcn_readfirstlane(run_of[min(run0 + run, runs - 1)]), 0)) * (kRun * DIM); };
+  // Lane kRunsOfWave * i + e holds where the wavefront's run e of the window's tile i lies: -1 where it has none, or no page.
+  constexpr int kTileRuns = kTok / kRun, kRunsOfWave = kTileRuns / kTileWaves;
+  static_assert(kMaxRuns == kWave * kTileWaves, "a lane a run");
+  int my_run = -1;
+  // The codes of the window's tile i on their way.
+  auto ask = [&](int i) {
+    auto place = [&](int e) { return static_cast<int64_t>(max(__builtin_amdgcn_readlane(my_run, kRunsOfWave * i + e), 0)) * (kRun * DIM); };
 #pragma unroll
-    for (int e = 0; e < kKeyLoads; ++e) {
-      key_codes[e] = *reinterpret_cast<const u32x4*>(c.k + place(key_run(e)) + 16 * key_piece(e));
-    }
-    const uint8_t* at = c.v + place(DIM == 64 ? 2 * wave : value_run);
-    if constexpr (DIM == 64) at = lane < 32 ? at : c.v + place(2 * wave + 1);
+    for (int e = 0; e < kKeyLoads; ++e) key_codes[e] = *reinterpret_cast<const u32x4*>(c.k + place(DIM == 64 ? e : 0) + 16 * key_piece(e));
+    const uint8_t* at = c.v + place(0);
+    if constexpr (DIM == 64) at = lane < 32 ? at : c.v + place(1);
     at += 4 * value_half * DIM + 4 * quad;
 #pragma unroll
     for (int k = 0; k < 8; ++k) value_codes[k] = *reinterpret_cast<const uint32_t*>(at + (k % 4 + 8 * (k / 4)) * DIM);
   };
   // The codes asked for into LDS. `first`: the tile's first token; `clean`: every place of the tile holds a token.
-  auto put = [&](uint8_t* buffer, int first, int run0, int runs, bool clean) {
+  auto put = [&](uint8_t* buffer, int i, int first, bool clean) {
 #pragma unroll
     for (int e = 0; e < kKeyLoads; ++e) {
       const int row = kRun * key_run(e) + key_piece(e) / (DIM / 16), column = key_piece(e) % (DIM / 16);
@@ -130,7 +131,8 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
       *reinterpret_cast<bf16x8*>(at + key_place<DIM>(row, 2 * column + 1)) = weight_fragment<F>(key_codes[e], 0, 1);
     }
     if (!clean) {  // codes of places without a token (NaNs perhaps) times a weight of nothing have to be nothing
-      const bool there = run0 + value_run < runs && run_of[min(run0 + value_run, runs - 1)] >= 0;
+      bool there = __builtin_amdgcn_readlane(my_run, kRunsOfWave * i) >= 0;
+      if constexpr (DIM == 64) there = lane < 32 ? there : __builtin_amdgcn_readlane(my_run, kRunsOfWave * i + 1) >= 0;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (!there || first + kRun * value_run + 4 * value_half + k % 4 + 8 * (k / 4) >= t.span.length) value_codes[k] = 0;
@@ -161,33 +163,30 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
     __syncthreads();
     if (threadIdx.x == 0) holes = 0;
     __syncthreads();
-    float most = 0.0f, vs = 0.0f;
-    if (static_cast<int>(threadIdx.x) < runs) {
-      const int token = window + kRun * threadIdx.x, page = kv8_page(c, p.b, seq, token);
-      float ks = 0.0f;
-      int run = -1;
+    const int mine = lane / kRunsOfWave * kTileRuns + kRunsOfWave * wave + lane % kRunsOfWave;  // the lane's run of the window
+    float ks = 0.0f, vs = 0.0f;
+    my_run = -1;
+    if (mine < runs) {
+      const int token = window + kRun * mine, page = kv8_page(c, p.b, seq, token);
       if (page >= 0) {
         const int64_t at = kv8_row(c, page, head) + token % c.page;
-        run = static_cast<int>(at / kRun);
+        my_run = static_cast<int>(at / kRun);
         ks = c.k_scale[at >> c.block_shift] * fabsf(p.scale) * 1.4426950408889634f;
         vs = fabsf(c.v_scale[at >> c.block_shift]);
       } else {
         holes = 1;
       }
-      run_of[threadIdx.x] = run;
-      key_scale[threadIdx.x] = ks;
-      most = vs;
     }
+    key_scale[mine] = my_run >= 0 ? ks : __builtin_nanf("");  // a NaN: nothing of the run is seen
+    float most = vs;
     most = wave_max(most);
     if (lane == 0) scale_top[wave] = most;
     __syncthreads();
     most = fmaxf(fmaxf(fmaxf(scale_top[0], scale_top[1]), fmaxf(scale_top[2], scale_top[3])), largest);
     // Scales as exponents relative to the largest so far; one under 2^-60 of it counts as that.
-    if (static_cast<int>(threadIdx.x) < runs) {
-      const float e = most > 0.0f ? fmaxf(__builtin_amdgcn_logf(vs / most), kLeastScale) + kWeightBits : 0.0f;
-      value_exp[threadIdx.x] = e;
-      value_per[threadIdx.x] = __builtin_amdgcn_exp2f(-e);
-    }
+    const float e = most > 0.0f ? fmaxf(__builtin_amdgcn_logf(vs / most), kLeastScale) + kWeightBits : 0.0f;
+    value_exp[mine] = e;
+    value_per[mine] = __builtin_amdgcn_exp2f(-e);
     if (largest < most && largest > 0.0f) {
       const float less = largest / most;
 #pragma unroll
@@ -197,15 +196,22 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
     const bool whole = !holes;
     const int tiles = (runs * kRun + kTok - 1) / kTok;
     auto clean = [&](int i) { return whole && window + (i + 1) * kTok <= min(stop, t.span.length); };
-    ask(0, runs);
-    put(lds, window, 0, runs, clean(0));
+    ask(0);
+    put(lds, 0, window, clean(0));
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
       const uint8_t* const keys = lds + (i % 2) * kBuffer;
       const uint8_t* const values = keys + kKeyBytes;
       const int at = window + i * kTok;
       const bool more = i + 1 < tiles;
-      if (more) ask((i + 1) * (kTok / kRun), runs);
+      if (more) ask(i + 1);
+      float ks[kTileRuns], ve[kTileRuns], per[kTileRuns];
+#pragma unroll
+      for (int j = 0; j < kTileRuns; ++j) {
+        ks[j] = key_scale[i * kTileRuns + j];
+        ve[j] = value_exp[i * kTileRuns + j];
+        per[j] = value_per[i * kTileRuns + j];
+      }
       const bool some = my_count > 0 && at <= high_pos && (p.window == 0 || at + kTok > static_cast<int64_t>(low_pos) - p.window + 1);
       if (some) {
         // The wavefronts of a SIMD take turns: the one that feeds the matrix cores goes first (176 -> 169 us on a 4096-row prompt).
@@ -229,19 +235,10 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
         __builtin_amdgcn_sched_group_barrier(kMatrix, 6, 0);
         __builtin_amdgcn_s_setprio(0);
         const bool plain = clean(i) && at + kTok - 1 <= low_pos && (p.window == 0 || at > static_cast<int64_t>(high_pos) - p.window);
-        float ks[kTok / kRun], ve[kTok / kRun], per[kTok / kRun];
-#pragma unroll
-        for (int j = 0; j < kTok / kRun; ++j) {
-          const int run = min(i * (kTok / kRun) + j, runs - 1);
-          ks[j] = key_scale[run];
-          ve[j] = value_exp[run];
-          per[j] = value_per[run];
-        }
         if (!plain) {
 #pragma unroll
           for (int j = 0; j < kTok / kRun; ++j) {
-            const int run = i * (kTok / kRun) + j;
-            const bool there = run < runs && run_of[min(run, runs - 1)] >= 0;
+            const bool there = ks[j] == ks[j];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const int token = at + kRun * j + 8 * (e / 4) + 4 * h + e % 4;
@@ -301,7 +298,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      if (more) put(lds + ((i + 1) % 2) * kBuffer, at + kTok, (i + 1) * (kTok / kRun), runs, clean(i + 1));
+      if (more) put(lds + ((i + 1) % 2) * kBuffer, i + 1, at + kTok, clean(i + 1));
       __syncthreads();
     }
   }

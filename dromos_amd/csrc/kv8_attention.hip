@@ -46,7 +46,9 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads, int wi
   // two tiles of sixteen leave room for two workgroups a unit only: 8 streams of 5 rows 28.7 us, with twice the parts 34.8.
   const int each = b.seqs > 1 && per == 16 ? 4 : 2;
   int64_t want = busy > 0 ? (each * compute_units() + busy - 1) / busy : 1;
-  if (busy >= compute_units()) want = 1;
+  // One part where there is a workgroup a unit. Tiles of 128 rows need a quarter more: a unit with one of them alone is half idle
+  // (1024 rows behind 7168 tokens, 264 workgroups: 208 us, in two parts 152).
+  if (4 * busy >= (p.tiles ? 5 : 4) * compute_units()) want = 1;
   int64_t chunk = (length + want - 1) / (want > 0 ? want : 1);
   chunk = (chunk + 255) / 256 * 256;
   // Parts cost a second kernel (about 4 us); one part costs a step of each wavefront more for every 256 tokens (1.6 us).

@@ -24,6 +24,7 @@ struct NormArgs {
   int64_t ld_y, ld_gate, ld_h, ld_x;
   int y_type, h_type, w_type, x_type;
   float alpha, beta, eps;
+  int64_t row0;
   int H;
   int layer;
 };
@@ -158,7 +159,7 @@ template <int V, int N>
 __global__ void __launch_bounds__(1024, V * N == 32 ? 4 : 8) block_norm_kernel(const NormArgs a) {
   __shared__ __attribute__((aligned(16))) float shared[32];
   if (threadIdx.x < 32) shared[threadIdx.x] = 0.0f;
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.row0 + blockIdx.x;
   bool in[N];
   int at[N];
 #pragma unroll
@@ -216,11 +217,17 @@ bool aligned(const void* p, int64_t ld, int type) {
 
 // As many threads as the row has vectors for N each, up to 1024; of single values half as many each where there are threads for it.
 template <int V, int N>
-int launch(const NormArgs& a, int T, hipStream_t s) {
+int launch(NormArgs a, int T, hipStream_t s) {
   constexpr int kEach = V == 1 ? N / 2 : V * N;
   const int wanted = ((a.H + kEach - 1) / kEach + kWave - 1) / kWave * kWave, threads = wanted < 1024 ? wanted : 1024;
-  hipLaunchKernelGGL((block_norm_kernel<V, N>), dim3(T), dim3(threads), 0, s, a);
-  return status_of(hipGetLastError());
+  const int most = static_cast<int>(kMaxGridThreads / threads);  // rows of a launch
+  for (int row = 0; row < T; row += most) {
+    a.row0 = row;
+    hipLaunchKernelGGL((block_norm_kernel<V, N>), dim3(T - row < most ? T - row : most), dim3(threads), 0, s, a);
+    if (int st = status_of(hipGetLastError())) return st;
+    if (T - row <= most) break;
+  }
+  return kOk;
 }
 
 }  // namespace

@@ -296,6 +296,9 @@ __device__ __forceinline__ float weight_element(int type, const void* data, cons
   }
 }
 
+// A launch has at most this many threads along x.
+constexpr int64_t kMaxGridThreads = 0xffffffff;
+
 // f32 -> e4m3fn, nearest even, saturating at 448, NaN -> 0x7f with the sign (engine/cpu/quant.cpp:20-39).
 __device__ __forceinline__ uint32_t e4m3_encode(float f) {
   uint32_t u = __float_as_uint(f);

@@ -156,3 +156,19 @@ def test_a_rows_bits_do_not_depend_on_the_others(hip):
     for i in (0, 17, 39):
         one_h, one_x = call(hip, True, y[i:i + 1], w, None, None, 1.0, 1.0, h[i:i + 1], w, None, H, 1e-5)
         assert torch.equal(one_h[0], all_h[i]) and torch.equal(one_x[0], all_x[i])
+
+
+def test_more_rows_than_a_launch_has_threads_for(hip):
+    """Heads as rows: 2^26 + 5 rows of eight values, a wavefront each. The rows around the end of the first launch, and the last."""
+    T, width = (1 << 26) + 5, 8
+    y = torch.ones(T, width, dtype=H, device="cuda")
+    edges = [slice(0, 9), slice((1 << 26) - 70, T)]
+    for i, at in enumerate(edges):
+        y[at] = randn(i, y[at].shape[0], width).cuda()
+    w = randn(3, width).cuda()
+    _, x = call(hip, False, None, None, None, None, 1.0, 1.0, y, w, None, H, 1e-5)
+    for at in edges:
+        _, some = call(hip, False, None, None, None, None, 1.0, 1.0, y[at].contiguous(), w, None, H, 1e-5)
+        assert torch.equal(x[at], some)
+    _, one = call(hip, False, None, None, None, None, 1.0, 1.0, y[1000:1001].contiguous(), w, None, H, 1e-5)
+    assert bool((x[9:(1 << 26) - 70] == one).all())

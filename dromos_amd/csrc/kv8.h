@@ -106,10 +106,12 @@ inline int kv8_check_cache(const lx_kv8* c) {
   return kOk;
 }
 
-inline int kv8_check_batch(const lx_kv8_batch* b, int T) {
+// Positions, and what is added to them on the way, stay below 2^31: no sequence has room for more than 2^30 tokens.
+inline int kv8_check_batch(const lx_kv8_batch* b, int T, const lx_kv8& c) {
   if (!b || T < 0 || T >= (1 << 30) || b->seqs < 0 || b->seqs > (1 << 30) || b->max_rows < 0 || b->max_length < 0 || b->ld_table < 0) return kInvalid;
   if (T == 0 || b->seqs == 0) return kOk;
   if (!b->lengths || (b->ld_table > 0 && !b->table)) return kInvalid;
+  if (b->max_length > (1 << 30) && static_cast<int64_t>(b->ld_table) * c.page > (1 << 30)) return kInvalid;
   return kOk;
 }
 

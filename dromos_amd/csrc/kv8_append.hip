@@ -369,10 +369,10 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs p) {
   }
 }
 
-// Sixteen codes a thread: 16 bytes in, 32 out; keys, then values.
+// Sixteen codes a thread: 16 bytes in, 32 out; keys, then values. What one grid line does not hold goes to the next.
 template <int F>
 __global__ void __launch_bounds__(256) dequantize_cache_kernel(const Kv8Cache c, uint16_t* k, uint16_t* v, int64_t pieces) {
-  const int64_t i = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x;
+  const int64_t i = (blockIdx.z * static_cast<int64_t>(gridDim.x) + blockIdx.x) * 256 + threadIdx.x;
   const bool values = blockIdx.y == 1;
   uint16_t* const out = values ? v : k;
   if (i >= pieces || !out) return;
@@ -414,7 +414,7 @@ int launch(AppendArgs p, hipStream_t stream) {
   p.query_rows = p.rows_per_group < slots ? p.rows_per_group : slots;
   const int64_t keys = static_cast<int64_t>((p.b.T + p.rows_per_group - 1) / p.rows_per_group) * p.c.heads;
   const int64_t queries = static_cast<int64_t>((p.b.T + p.query_rows - 1) / p.query_rows) * ((p.q_heads + kQueryHeads - 1) / kQueryHeads);
-  if (keys + queries > 0x7fffffff) return fail(kInvalid);
+  if ((keys + queries) * kThreads > kMaxGridThreads) return fail(kInvalid);
   p.queries = static_cast<unsigned>(keys);
   hipLaunchKernelGGL((append_kernel<F, kThreads, P, HALF>), dim3(static_cast<unsigned>(keys + queries)), dim3(kThreads), 0, stream, p);
   return status_of(hipGetLastError());
@@ -441,7 +441,7 @@ int lx_kv8_append(const lx_kv8* cache, const lx_kv8_batch* batch, const void* q,
                   int ld_k, int ld_v, void* q_out, lx_dtype q_out_dtype, int ld_q_out, const float* freq, int rot, int interleaved, int T,
                   int q_heads, void* stream) {
   if (int st = kv8_check_cache(cache)) return fail(st);
-  if (int st = kv8_check_batch(batch, T)) return fail(st);
+  if (int st = kv8_check_batch(batch, T, *cache)) return fail(st);
   if ((dtype != LX_F32 && dtype != LX_BF16) || (q && q_out_dtype != LX_F32 && q_out_dtype != LX_BF16)) return fail(kInvalid);
   if (rot < 0 || rot > cache->dim || rot % 8 != 0) return fail(kInvalid);
   if (T == 0 || batch->seqs == 0 || batch->max_rows == 0) return kOk;
@@ -470,11 +470,11 @@ int lx_kv8_dequantize(const lx_kv8* cache, void* k, void* v, void* stream) {
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 != 0) return fail(kInvalid);
   const Kv8Cache c = kv8_cache(*cache);
   const int64_t pieces = static_cast<int64_t>(c.pages) * c.heads * c.page * (c.dim / 16);
-  if ((pieces + 255) / 256 > 0x7fffffff) return fail(kInvalid);
   if (!k && !v) return kOk;
+  const int64_t groups = (pieces + 255) / 256, line = groups < (1 << 23) ? groups : 1 << 23;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((pieces + 255) / 256), 2), dim3(256), 0, as_stream(stream), c, static_cast<uint16_t*>(k),
-                       static_cast<uint16_t*>(v), pieces);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(line), 2, static_cast<unsigned>((groups + line - 1) / line)), dim3(256), 0, as_stream(stream), c,
+                       static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), pieces);
   };
   if (cache->type == LX_W_INT8) go(dequantize_cache_kernel<LX_W_INT8>);
   else go(dequantize_cache_kernel<LX_W_FP8>);
@@ -484,7 +484,7 @@ int lx_kv8_dequantize(const lx_kv8* cache, void* k, void* v, void* stream) {
 // For tests, on host memory and without a device: what the kernel makes of a call's rows. Every piece that it stores, as
 // {sequence, first token, its page or -1, tokens, first row}, `capacity` of them at most; returns how many there are.
 LX_API int dromos_kv8_pieces(const lx_kv8* cache, const lx_kv8_batch* batch, int T, int* out, int capacity) {
-  if (kv8_check_cache(cache) || kv8_check_batch(batch, T)) return -1;
+  if (kv8_check_cache(cache) || kv8_check_batch(batch, T, *cache)) return -1;
   const Kv8Cache c = kv8_cache(*cache);
   const Kv8Batch b = kv8_batch(*batch, T);
   const int per = rows_per_group(cache->block, batch->seqs, T);

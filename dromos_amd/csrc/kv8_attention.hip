@@ -12,8 +12,9 @@ struct Plan {
   int row_tiles;       // tiles a sequence
   int tile_rows;       // rows of its fullest tile
   int splits, chunk;
-  int64_t workgroups;
-  int64_t bytes;       // workspace
+  int64_t workgroups, combiners;  // of the attention, and of the sums of its parts
+  int64_t bytes;                  // workspace
+  bool fits;                      // the device can be asked for that many
 };
 
 // Enough parts that the device has about two workgroups a compute unit, none shorter than 256 tokens (a step of each
@@ -30,7 +31,9 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads, int wi
   p.tiles = rows > 96 && c.dim <= 128;
   p.per_tile = p.tiles ? kTileRowsOfGroup : rows <= 16 || c.dim == 256 ? 16 : 32;
   const int per = p.per_tile;
-  p.row_tiles = static_cast<int>((rows + per - 1) / per);
+  const int64_t row_tiles = (rows + per - 1) / per, limit = kMaxGridThreads / 256;
+  if (row_tiles > limit || row_tiles * b.seqs > limit || row_tiles * b.seqs * c.heads > limit) return p;
+  p.row_tiles = static_cast<int>(row_tiles);
   p.tile_rows = static_cast<int>(rows < per ? rows : per);
   // What a tile's rows see: all tokens, or the window, the tile's own and the run that the window begins in.
   const int64_t held = static_cast<int64_t>(b.ld_table) * c.page;
@@ -60,6 +63,9 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads, int wi
   p.splits = static_cast<int>((length + chunk - 1) / chunk);
   if (p.splits < 1) p.splits = 1;
   p.workgroups = items * p.splits;
+  const int64_t combined = items * p.tile_rows, each_time = p.splits <= kFewParts ? 1024 / c.dim : 1;
+  p.combiners = p.splits > 1 ? (combined + each_time - 1) / each_time : 0;
+  p.fits = p.workgroups <= limit && p.combiners <= limit;
   // The workspace is for any window: one may have as many parts as are wanted of 256 tokens, or of the longest there are.
   int64_t parts = want < (whole + 255) / 256 ? want : (whole + 255) / 256;
   if (!p.tiles && parts < (whole + kMaxRuns * kRun - 1) / (kMaxRuns * kRun)) parts = (whole + kMaxRuns * kRun - 1) / (kMaxRuns * kRun);
@@ -82,8 +88,7 @@ int stream(const AttentionArgs& a, const Plan& p, hipStream_t s) {
   }
   if (int st = status_of(hipGetLastError())) return st;
   if (p.splits == 1) return kOk;
-  const int64_t rows = p.workgroups / p.splits * p.tile_rows, per = p.splits <= kFewParts ? 1024 / DIM : 1;
-  hipLaunchKernelGGL((combine_kernel<DIM>), dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, s, a, p.per_tile, p.tile_rows);
+  hipLaunchKernelGGL((combine_kernel<DIM>), dim3(static_cast<unsigned>(p.combiners)), dim3(256), 0, s, a, p.per_tile, p.tile_rows);
   return status_of(hipGetLastError());
 }
 
@@ -107,14 +112,14 @@ extern "C" {
 int lx_kv8_attention(const void* q, lx_dtype q_dtype, int ld_q, const lx_kv8* cache, const lx_kv8_batch* batch, void* out,
                      lx_dtype out_dtype, int ld_out, int T, int q_heads, float scale, int window, void* workspace, void* stream) {
   if (int st = kv8_check_cache(cache)) return fail(st);
-  if (int st = kv8_check_batch(batch, T)) return fail(st);
+  if (int st = kv8_check_batch(batch, T, *cache)) return fail(st);
   if ((q_dtype != LX_F32 && q_dtype != LX_BF16) || (out_dtype != LX_F32 && out_dtype != LX_BF16) || window < 0) return fail(kInvalid);
   if (q_heads < 1 || q_heads > 65536 || q_heads % cache->heads != 0) return fail(kInvalid);
   if (T == 0 || batch->seqs == 0 || batch->max_rows == 0) return kOk;
   const int64_t width = static_cast<int64_t>(q_heads) * cache->dim;
   if (!q || !out || (T > 1 && (ld_q < width || ld_out < width))) return fail(kInvalid);
   const Plan plan = plan_for(*cache, *batch, T, q_heads, window);
-  if (plan.workgroups > 0x7fffffff / kTileRowsOfGroup || (plan.splits > 1 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))) return fail(kInvalid);
+  if (!plan.fits || (plan.splits > 1 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))) return fail(kInvalid);
   AttentionArgs a{};
   a.c = kv8_cache(*cache);
   a.b = kv8_batch(*batch, T);
@@ -129,7 +134,7 @@ int lx_kv8_attention(const void* q, lx_dtype q_dtype, int ld_q, const lx_kv8* ca
 }
 
 int64_t lx_kv8_attention_workspace_bytes(const lx_kv8* cache, const lx_kv8_batch* batch, int T, int q_heads) {
-  if (kv8_check_cache(cache) || kv8_check_batch(batch, T) || T == 0 || batch->seqs == 0 || batch->max_rows == 0) return 0;
+  if (kv8_check_cache(cache) || kv8_check_batch(batch, T, *cache) || T == 0 || batch->seqs == 0 || batch->max_rows == 0) return 0;
   if (q_heads < 1 || q_heads > 65536 || q_heads % cache->heads != 0) return 0;
   return plan_for(*cache, *batch, T, q_heads, 0).bytes;
 }
@@ -138,8 +143,9 @@ int64_t lx_kv8_attention_workspace_bytes(const lx_kv8* cache, const lx_kv8_batch
 // sums' bytes, the workspace's bytes} of a call. Returns 0, or the status that the call is refused with.
 LX_API int dromos_kv8_plan(const lx_kv8* cache, const lx_kv8_batch* batch, int T, int q_heads, int window, int64_t* out) {
   if (int st = kv8_check_cache(cache)) return st;
-  if (int st = kv8_check_batch(batch, T)) return st;
+  if (int st = kv8_check_batch(batch, T, *cache)) return st;
   const Plan p = plan_for(*cache, *batch, T, q_heads, window);
+  if (!p.fits) return kInvalid;
   out[0] = p.per_tile, out[1] = p.row_tiles, out[2] = p.splits, out[3] = p.chunk, out[4] = p.workgroups;
   out[5] = p.splits > 1 ? p.workgroups * p.per_tile * (cache->dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
   out[6] = lx_kv8_attention_workspace_bytes(cache, batch, T, q_heads);

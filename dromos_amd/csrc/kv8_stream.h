@@ -1,7 +1,7 @@
 // lx_kv8_attention for few rows a sequence: the cache is streamed once, so its bytes decide.
 //
-// Mathematics. o = sum_t w_t v_t / sum_t w_t with w_t = 2^(c_t - m), c_t = (q . k_t) * scale * log2 e, m the largest c so far:
-// one pass over the keys, sums and values rescaled by 2^(m_old - m_new) where a larger score comes. Scores are taken the other
+// Mathematics. o = sum_t w_t v_t / sum_t w_t with w_t = 2^(c_t - m), c_t = (q . k_t) * scale * log2 e, m a score near the
+// largest c so far: one pass over the keys, sums and values rescaled by 2^(m_old - m_new) where a much larger score comes. Scores are taken the other
 // way round, S^T = K Q^T, sixteen keys (A) by sixteen rows (B): a lane then holds the scores of one row (lane % 16) and four
 // keys, which is the layout in which O^T = V^T P^T wants its B operand, so weights never change lanes, and a row's
 // rescaling is its lanes' own. The matrix instruction sums over k in any order that both operands agree on: keys are read 16
@@ -17,9 +17,14 @@
 // at most, one 2^-21 of the reference's still a normal number, and most steps leave the sums as they are.
 //
 // Split. A workgroup takes one sequence, 16 RT rows of one of the cache's heads (rows of a head: its tokens' query heads,
-// token after token) and up to kMaxRuns runs of 16 tokens of it. Its four wavefronts take 64 tokens at a time in turn (32 of heads wider than 128) and keep
-// sums of their own; the workgroup adds them up at its end, in order. Where a sequence has several such parts they leave
-// their sums in the workspace, and a second kernel adds those, in order.
+// token after token) and up to kMaxRuns runs of 16 tokens of it. Its four wavefronts take 64 tokens at a time in turn (32 of
+// heads wider than 128) and keep sums of their own; the workgroup adds them up at its end, in order. Where a sequence has several
+// such parts they leave their sums in the workspace, and a second kernel adds those, in order.
+//
+// What bounds it (heads of 128, int8 or fp8). One sequence of 131072 tokens: 50.0 us for 268 MB, 5.4 TB/s, the rate of a copy.
+// 32 of up to 4096 tokens, as uneven as they come: 35 us where their bytes want 27, the longest one's workgroups end last. 8 of 5 rows
+// (20 a head, two tiles' worth of registers): 23.8 us against 12.6, two workgroups a unit wait for memory. 517 tokens: 10 us, two
+// steps of a wavefront whose every load follows one before it.
 #pragma once
 
 #include "kv8.h"

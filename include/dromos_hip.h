@@ -243,7 +243,8 @@ LX_API int lx_moe_experts_noalloc(const void* latent, const int32_t* ids, const 
  *            not count). They and T size the launch: a captured call replays with whatever rows, lengths and table hold then, within them.
  * The numbers in device memory are not refused but bounded: a page number outside [0, pages) is a page without tokens (nothing is
  * stored, nothing attended), rows end at T, lengths at max_length and at the table's end; a row in front of position 0 is not
- * stored and attends to nothing.
+ * stored and attends to nothing. T < 2^30; a table with room for more than 2^30 tokens a sequence wants a max_length that is no more,
+ * and a call of more workgroups than a launch can have (2^32 threads) is refused.
  *
  * lx_kv8_append: row i of a sequence of n rows and length L is its token p = L - n + i. k and v [T, heads * dim] and q [T, q_heads * dim]
  * (q may be null, then q_out is too), all f32 or all bf16, row strides in elements; q_out f32 or bf16, q itself allowed where type
@@ -251,9 +252,9 @@ LX_API int lx_moe_experts_noalloc(const void* latent, const int32_t* ids, const 
  *   rotation   the first `rot` values of a head (a multiple of 8, 0 for none) of q and k, by the angles p * freq[i], i < rot / 2 (freq
  *              f32 on the device; the angles are formed and reduced in 64 bits, so far positions lose nothing): pairs (i, i + rot / 2),
  *              or (2 i, 2 i + 1) where `interleaved`; (a, b) -> (a cos - b sin, b cos + a sin). v is stored unrotated.
- *   codes      per block and head, keys and values apart, qmax 127 or 448: s = max(|finite values of this call in the block|) / qmax, and at
- *              least the scale the block has while tokens of it in front of this call's stay; code = rne(x * (1 / s)), clamped to +-qmax
- *              (infinities too; a NaN is 0). Where s grew, the codes that stay become rne(code * (s_old / s)).
+ *   codes      per block and head, keys and values apart, qmax 127 or 448: s = max(|finite values of this call in the block|) / qmax
+ *              (2^-126 or more unless they are all 0), and at least the scale the block has while tokens of it in front of this call's
+ *              stay; code = rne(x * (1 / s)), clamped to +-qmax (infinities too; a NaN is 0). Where s grew, the codes that stay become rne(code * (s_old / s)).
  *              A block of zeros has scale 0. Codes of places behind the sequence's last token stay as they were.
  * A block may be written by one sequence of a call only; pages that sequences share are read by all of them.
  *
@@ -262,9 +263,10 @@ LX_API int lx_moe_experts_noalloc(const void* latent, const int32_t* ids, const 
  * lx_kv8_attention: out[row, h] = sum_t softmax_t(scale * q[row, h] . k[t]) v[t] over the tokens p - window < t <= p of the row's own
  * sequence (window 0: all up to p), p as above; query head h reads the cache's head h / (q_heads / heads). Rows without a token are 0.
  * q f32 (rounded to bf16, as lx_gemm_w's BF16 math does) or bf16, out f32 or bf16, row strides in elements; products on the matrix
- * cores (weights rounded to f16), sums and softmax in f32, one pass over the keys. Contents of the cache where no token lies (NaNs too) have no
- * part in it; where one lies its codes and scales are numbers, as lx_kv8_append writes them. The workspace (lx_kv8_attention_workspace_bytes for the same cache, batch, T and q_heads; 0: none, may be null) holds
- * partial sums of long sequences, may hold garbage, and belongs to one call at a time. */
+ * cores (weights rounded to f16), sums and softmax in f32, one pass over the keys. Contents of the cache where no token lies (NaNs
+ * too) have no part in it; where one lies its codes and scales are numbers, as lx_kv8_append writes them. The workspace
+ * (lx_kv8_attention_workspace_bytes for the same cache, batch, T and q_heads, whatever the window; 0: none, may be null) holds partial
+ * sums of long sequences, 16-byte aligned, may hold garbage, and belongs to one call at a time. */
 typedef struct {
   lx_wtype type;
   void* k;

@@ -326,3 +326,56 @@ def test_attention_beyond_31_bits(hip):
     batch.pages = 6
     check_appended(cache, after, batch, x[:, :heads * dim].cpu(), x[:, heads * dim:].cpu(), frequencies(dim), dim, False)
     assert not bool(big.codes[:, :pages - 6].any())
+
+
+# ---- numbers in device memory beyond what the caller has said -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("group", [4, 40])
+def test_no_table_at_all(hip, group):
+    """ld_table 0: no sequence has a place for a token. Nothing is stored, rows attend to nothing."""
+    batch = Batch([3, 1], [3, 40], 32)
+    cache = Cache("fp8", batch.pages, 1, 32, 16, 64).fill(1).to("cuda")
+    before, q = cache.codes.clone(), randn(2, 4, group * 64).cuda()
+    on = batch.to("cuda")
+    b = on.lx()
+    b.table, b.ld_table = None, 0
+    c = cache.lx()
+    out = torch.full_like(q, 7.0)
+    at = ctypes.pointer
+    hip("kv8_attention", q, BF16, group * 64, at(c), at(b), out, BF16, group * 64, 4, group, 0.1, 0, None)
+    assert bool((out == 0).all())
+    k = randn(3, 4, 64).cuda()
+    hip("kv8_append", at(c), at(b), None, k, k, BF16, 0, 64, 64, None, BF16, 0, None, 0, 0, 4, 0)
+    assert torch.equal(cache.codes, before)
+
+
+def test_lengths_beyond_the_callers_bound(hip):
+    """Tokens behind max_length do not count: a sequence ends there, and its rows with it."""
+    for rows in ([3, 5], [40, 70]):
+        more, less = Batch(rows, [200, 300], 32), Batch(rows, [150, 150], 32)
+        less.table, less.pages = more.table, more.pages
+        more.max_length = 150
+        cache = Cache("int8", more.pages, 2, 32, 16, 64).fill(1)
+        q, kv = randn(2, more.T, 8 * 64), randn(3, 2, more.T, 2 * 64)
+        got = attention(hip, q.cuda(), cache.to("cuda"), more.to("cuda"), 8, 0.1)
+        check_attention(got, q, cache, less, 8, 0.1)
+        held = cache.to("cuda")
+        append(hip, held, more.to("cuda"), None, kv[0].cuda(), kv[1].cuda(), frequencies(64).cuda(), 64)
+        check_appended(cache, held.to("cpu"), less, kv[0], kv[1], frequencies(64), 64, False)
+
+
+def test_more_rows_than_the_callers_bound(hip):
+    """Rows of a sequence behind max_rows are left alone; those in front of them are what they are without them."""
+    more, less = Batch([3, 5], [200, 300], 32), Batch([3, 4], [200, 299], 32)
+    less.table, less.pages = more.table, more.pages
+    more.max_rows = 4
+    cache = Cache("fp8", more.pages, 2, 32, 16, 64).fill(1)
+    q, kv = randn(2, 8, 8 * 64), randn(3, 2, 8, 2 * 64)
+    out = torch.full((8, 8 * 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    attention(hip, q.cuda(), cache.to("cuda"), more.to("cuda"), 8, 0.1, out=out)
+    check_attention(out[:7], q[:7], cache, less, 8, 0.1)
+    assert bool((out[7] == 7.0).all())
+    held = cache.to("cuda")
+    append(hip, held, more.to("cuda"), None, kv[0].cuda(), kv[1].cuda(), frequencies(64).cuda(), 64)
+    check_appended(cache, held.to("cpu"), less, kv[0, :7], kv[1, :7], frequencies(64), 64, False)

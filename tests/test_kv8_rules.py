@@ -177,3 +177,27 @@ def test_parts_cover_what_rows_see_and_fit_the_workspace(lx, seed):
     assert parts * chunk >= seen and chunk % 256 == 0 and (per == 128 or chunk <= 4096)
     assert workgroups == seqs * tiles * heads * parts and partial <= workspace
     assert parts == 1 or workspace > 0
+
+
+def test_sequences_of_more_than_2_30_tokens_refused(lx):
+    """A table may name one page many times, and so have room for more tokens than positions can count."""
+    plan = lambda b: lx.lib.dromos_kv8_plan(cache(), b, 2, 8, 0, (ctypes.c_int64 * 7)())
+    wide = (1 << 24) + 1  # pages of 64
+    for call in (append, attention):
+        assert call(lx, b=batch(ld_table=wide, max_length=2**31 - 1)) == 1
+        assert call(lx, b=batch(ld_table=wide, max_length=(1 << 30) + 1)) == 1
+    assert plan(batch(ld_table=wide, max_length=(1 << 30) + 1)) == 1
+    assert plan(batch(ld_table=wide, max_length=1 << 30)) == 0 and plan(batch(ld_table=3, max_length=2**31 - 1)) == 0
+
+
+@pytest.mark.parametrize("seqs,heads,group,T,rows,length", [(1 << 30, 1024, 1, 1 << 29, 1, 64), (1, 1, 65536, (1 << 30) - 1, 1 << 30, 64), (1 << 30, 1, 65536, (1 << 30) - 1, 1 << 30, 64),
+                                                          (1 << 14, 1024, 1, 1 << 14, 1, 64), (1 << 22, 2, 8, 1 << 22, 1, 65536)])
+def test_calls_of_more_workgroups_than_a_launch_refused(lx, seqs, heads, group, T, rows, length):
+    """Not started, and never taken for a smaller one: neither a number of workgroups nor its bytes wraps around."""
+    c, b = cache(heads=heads), batch(seqs=seqs, max_rows=rows, max_length=length, ld_table=1024)
+    width = heads * group * 128
+    assert lx.lib.dromos_kv8_plan(c, b, T, heads * group, 0, (ctypes.c_int64 * 7)()) == 1
+    # The last would have its 16 parts of 4096 tokens (a window might make it fit); of the others no part fits.
+    most = seqs * heads * 16 * 16 * (128 + 2) * 4 if length > 64 else 0
+    assert lx.size("kv8_attention_workspace_bytes", c, b, T, heads * group) == most
+    assert attention(lx, c=c, b=b, T=T, q_heads=heads * group, ld_q=width, ld_out=width) == 1

@@ -379,3 +379,28 @@ def test_more_rows_than_the_callers_bound(hip):
     held = cache.to("cuda")
     append(hip, held, more.to("cuda"), None, kv[0].cuda(), kv[1].cuda(), frequencies(64).cuda(), 64)
     check_appended(cache, held.to("cpu"), less, kv[0, :7], kv[1, :7], frequencies(64), 64, False)
+
+
+@pytest.mark.parametrize("rows", [2, 60])
+def test_pages_that_sequences_share(hip, rows):
+    """A prefix of 96 tokens that three sequences have in common: read by all, written by none, each goes on in pages of its own."""
+    batch = Batch([rows, rows, 1], [96 + rows, 130 + rows, 97], 32)
+    batch.table[1, :3] = batch.table[2, :3] = batch.table[0, :3]
+    cache = Cache("fp8", batch.pages, 2, 32, 16, 128).fill(1)
+    held, on = cache.to("cuda"), batch.to("cuda")
+    T = batch.T
+    q, kv = randn(2, T, 8 * 128), randn(3, 2, T, 2 * 128)
+    append(hip, held, on, None, kv[0].cuda(), kv[1].cuda(), frequencies(128).cuda(), 128)
+    after = held.to("cpu")
+    check_appended(cache, after, batch, kv[0], kv[1], frequencies(128), 128, False)
+    got = attention(hip, q.cuda(), held, on, 8, 0.09)
+    check_attention(got, q, after, batch, 8, 0.09)
+
+
+def test_one_page_many_times(hip):
+    """A table that names the same page again and again: its tokens count as often."""
+    batch = Batch([3], [400], 32)
+    batch.table[0, :] = batch.table[0, 0]
+    cache = Cache("int8", batch.pages, 1, 32, 32, 64).fill(1)
+    q = randn(2, 3, 4 * 64)
+    check_attention(attention(hip, q.cuda(), cache.to("cuda"), batch.to("cuda"), 4, 0.1), q, cache, batch, 4, 0.1)

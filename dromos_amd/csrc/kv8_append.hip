@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs p) {
   }
 }
 
-// Sixteen codes a thread: 16 bytes in, 32 out; keys, then values. What one grid line does not hold goes to the next.
+// Sixteen codes a thread: 16 bytes in, 32 out; keys, then values. What one grid line does not hold goes to the next. Stored past the caches
+// (4288 tokens of 8 heads of 128 7.4 -> 6.5 us, 6336 of them 11.4 -> 9.5).
 template <int F>
 __global__ void __launch_bounds__(256) dequantize_cache_kernel(const Kv8Cache c, uint16_t* k, uint16_t* v, int64_t pieces) {
   const int64_t i = (blockIdx.z * static_cast<int64_t>(gridDim.x) + blockIdx.x) * 256 + threadIdx.x;
@@ -391,8 +392,8 @@ __global__ void __launch_bounds__(256) dequantize_cache_kernel(const Kv8Cache c,
     out4[j / 2][2 * (j & 1)] = __builtin_bit_cast(uint32_t, pack_bf16(x[0] * s, x[1] * s));
     out4[j / 2][2 * (j & 1) + 1] = __builtin_bit_cast(uint32_t, pack_bf16(x[2] * s, x[3] * s));
   }
-  reinterpret_cast<u32x4*>(out)[2 * i] = out4[0];
-  reinterpret_cast<u32x4*>(out)[2 * i + 1] = out4[1];
+  __builtin_nontemporal_store(out4[0], reinterpret_cast<u32x4*>(out) + 2 * i);
+  __builtin_nontemporal_store(out4[1], reinterpret_cast<u32x4*>(out) + 2 * i + 1);
 }
 
 bool aligned(const void* p, int64_t ld, int dtype) {

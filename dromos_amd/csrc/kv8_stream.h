@@ -8,13 +8,14 @@
 // bytes a lane as they lie, and a lane's slots of a sum over tokens are the four of one run of 16 and the four of the next
 // that it holds weights of. Values are read DIM / 16 bytes a lane and token (16 lanes a row) and transposed by bytes in
 // registers, two permutations for four tokens' pairs. Key codes become bf16 exactly, as the queries are; value codes become
-// f16 exactly. A key block's scale multiplies its scores; a value block's goes into its weights as an exponent: a weight is
-// 2^(score * key scale + (log2 of the value scale - m)), one multiply-add and one exponential, rounded to f16 for the matrix
-// cores: three more bits than bf16, so the roundings of the weights (2^-11 of each term) stay well below the result's own.
-// The sum of weights adds up the rounded ones, by twos, in f32, and takes the value scale off again once per run. f16's range is
-// made enough: value scales are taken relative to the part's largest one (under 2^-60 of it they count as that), weights are
-// held times 2^7, and the reference m follows a row's largest score only where that is 2^8 ahead: the largest weight is 2^15
-// at most, one 2^-21 of the reference's still a normal number, and most steps leave the sums as they are.
+// f16 exactly. A key block's scale multiplies its scores; a value block's scale u goes into its weights as an exponent: the
+// matrix cores take terms 2^(c + log2 u - n), one multiply-add and one exponential, rounded to f16: three more bits than bf16, so
+// these roundings (2^-11 of each term) stay well below the result's own. n is a row's reference for c + log2 u, as m is for c, so
+// f16's range is spent on what the row sees and on nothing else. Either follows only where a token is 2^8 ahead of it. Terms are held
+// times 2^7: the largest is 2^15 at most, one 2^-21 of the reference's still a normal number, one under 2^-32 nothing, and most
+// steps leave the sums as they are. A token counts in the sum of weights however small its values are: that adds up the terms
+// before they are rounded, in f32, and takes log2 u off again once per run. A block's exponent is 2^-60 of its weights' at least,
+// so its terms are numbers in f32 (and nothing in f16) where its scale is 0.
 //
 // Split. A workgroup takes one sequence, 16 RT rows of one of the cache's heads (rows of a head: its tokens' query heads,
 // token after token) and up to kMaxRuns runs of 16 tokens of it. Its four wavefronts take 64 tokens at a time in turn (32 of
@@ -140,9 +141,13 @@ __device__ __forceinline__ uint32_t flipped(uint32_t d) {
 
 __device__ __forceinline__ f16x2 pack_f16(float a, float b) { return f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)}; }
 
-constexpr float kWeightBits = 7.0f;   // weights are held times 2^7
-constexpr float kSlack = 8.0f;        // how far a score may be ahead of its row's reference (log2)
-constexpr float kLeastScale = -60.0f; // of a value block, relative to the largest (log2)
+// Row references less 7 (terms and weights are held times 2^7); how far a score or a term may be ahead of them before they follow;
+// and what they are until a row sees a token.
+constexpr float kTermBits = 7.0f, kSlack = 8.0f + kTermBits, kNothing = -1e30f;
+constexpr float kLeastLift = -60.0f;  // a term over its weight, at least (log2)
+
+// Terms times this, twice, are relative to the reference `base`, as the sum of weights is (scales from 2^-126 to 2^121 come back so).
+__device__ __forceinline__ float term_root(float term_base, float base) { return __builtin_amdgcn_exp2f(0.5f * (term_base - base)); }
 
 // N eights of a query's values, `stride` values apart from `at` on, as the matrix instruction's operands; f32 ones are rounded to
 // bf16 here. A negative scale's sign goes to them, so that the scales of the scores never turn a largest one into a smallest.
@@ -243,20 +248,17 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
     load_query(p, have, at, [&](int k) { return 64 * (k / 2) + 16 * g + 8 * (k % 2); }, q[r]);
   }
   ask_values(run_in(0));
-  // Scales of the runs: of the scores, and (as exponents, relative to the wavefront's largest) of the values and back.
-  const float log_here = run >= 0 ? __builtin_amdgcn_logf(fabsf(vs)) : -__builtin_inff();
-  float largest = wave_max(log_here);
-  if (largest == -__builtin_inff()) largest = 0.0f;  // every scale 0
+  // Scales of the runs: of the scores, and of the values (a run that is none may have any there).
   const float key_scale = ks * fabsf(p.scale) * 1.4426950408889634f;
-  const float value_exp = fmaxf(log_here - largest, kLeastScale) + kWeightBits, value_per = __builtin_amdgcn_exp2f(-value_exp);
+  const float value_log = run >= 0 ? __builtin_amdgcn_logf(fabsf(vs)) : -__builtin_inff();
   const bool whole = !__any(mine < runs && run < 0);
   auto from_lane = [](float v, int from) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), from)); };
 
   f32x4 acc[RT][kTiles] = {};
-  float top[RT], total[RT];
+  float base[RT], term_base[RT], total[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    top[r] = -__builtin_inff();
+    base[r] = term_base[r] = kNothing;
     total[r] = 0.0f;
   }
   for (int e = 0, step = wave; step < steps; ++e, step += kStreamWaves) {
@@ -279,12 +281,11 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
     if (more) ask_keys(run_in(e + 1));
     // Every token of the step is seen by every row?
     const bool plain = whole && at + kStep - 1 <= t.low_pos && (p.window == 0 || at > static_cast<int64_t>(t.high_pos) - p.window);
-    float ks[kRuns], ve[kRuns], per[kRuns];
+    float ks[kRuns], vl[kRuns];
 #pragma unroll
     for (int j = 0; j < kRuns; ++j) {
       ks[j] = from_lane(key_scale, e * kRuns + j);
-      ve[j] = from_lane(value_exp, e * kRuns + j);
-      per[j] = from_lane(value_per, e * kRuns + j);
+      vl[j] = from_lane(value_log, e * kRuns + j);
     }
     if (!plain) {
 #pragma unroll
@@ -306,43 +307,50 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
         ks[j] = 1.0f;
       }
     }
-    f16x8 weights[RT][kRuns / 2];
-    const f16x2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+    f16x8 terms[RT][kRuns / 2];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      float m = -__builtin_inff();
+      float m = -__builtin_inff(), n = m;
 #pragma unroll
-      for (int j = 0; j < kRuns; ++j)
-        m = fmaxf(m, fmaxf(fmaxf(s[r][j][0], s[r][j][1]), fmaxf(s[r][j][2], s[r][j][3])) * ks[j]);
-      float a, b;
-      swap_halves<true>(m, a, b);
-      m = fmaxf(a, b);
-      swap_halves<false>(m, a, b);
-      m = fmaxf(a, b);
-      if (__any(m > top[r] + kSlack)) {
-        m = fmaxf(m, top[r]);
-        const float keep = __builtin_amdgcn_exp2f(top[r] - (m == -__builtin_inff() ? 0.0f : m));
+      for (int j = 0; j < kRuns; ++j) {
+        const float most = fmaxf(fmaxf(s[r][j][0], s[r][j][1]), fmaxf(s[r][j][2], s[r][j][3])) * ks[j];
+        m = fmaxf(m, most);
+        n = fmaxf(n, most + vl[j]);
+      }
+      if (__any(m > base[r] + kSlack || n > term_base[r] + kSlack)) {
+        auto of_row = [](float v) {
+          float a, b;
+          swap_halves<true>(v, a, b);
+          v = fmaxf(a, b);
+          swap_halves<false>(v, a, b);
+          return fmaxf(a, b);
+        };
+        m = fmaxf(of_row(m) - kTermBits, base[r]);
+        n = fmaxf(of_row(n) - kTermBits, term_base[r]);
+        total[r] *= __builtin_amdgcn_exp2f(base[r] - m);
+        const float keep = __builtin_amdgcn_exp2f(term_base[r] - n);
 #pragma unroll
         for (int f = 0; f < kTiles; ++f) acc[r][f] *= keep;
-        total[r] *= keep;
-        top[r] = m;
+        base[r] = m;
+        term_base[r] = n;
       }
-      const float base = top[r] == -__builtin_inff() ? 0.0f : top[r];
+      const float least = kLeastLift - base[r];
 #pragma unroll
       for (int j = 0; j < kRuns; j += 2) {
         f16x2 v[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float lift = ve[j + e] - base;
+          const float lift = fmaxf(vl[j + e] - term_base[r], least);
           float w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][j + e][k], ks[j + e], lift));
           v[2 * e] = pack_f16(w[0], w[1]);
           v[2 * e + 1] = pack_f16(w[2], w[3]);
-          const float sum = __builtin_amdgcn_fdot2(v[2 * e + 1], ones, __builtin_amdgcn_fdot2(v[2 * e], ones, 0.0f, false), false);
-          total[r] = __builtin_fmaf(sum, per[j + e], total[r]);
+          const float per = __builtin_amdgcn_exp2f(-base[r] - lift);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) total[r] = __builtin_fmaf(w[k], per, total[r]);
         }
-        weights[r][j / 2] = __builtin_bit_cast(f16x8, v);
+        terms[r][j / 2] = __builtin_bit_cast(f16x8, v);
       }
     }
 #pragma unroll
@@ -364,7 +372,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
           for (int e = 0; e < 4; ++e) v[e] = f % 2 ? pair_of<F, true>(two[e][f / 2]) : pair_of<F, false>(two[e][f / 2]);
           const f16x8 a = __builtin_bit_cast(f16x8, v);
 #pragma unroll
-          for (int r = 0; r < RT; ++r) acc[r][4 * d + f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, weights[r][j / 2], acc[r][4 * d + f], 0, 0, 0);
+          for (int r = 0; r < RT; ++r) acc[r][4 * d + f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, terms[r][j / 2], acc[r][4 * d + f], 0, 0, 0);
         }
       }
     if (more) ask_values(run_in(e + 1));
@@ -378,12 +386,11 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
     const float w = a + b;
     swap_halves<false>(w, a, b);
     if (g == 0) {
-      wave_top[wave][16 * r + i] = top[r];
+      wave_top[wave][16 * r + i] = base[r];
       wave_sum_of[wave][16 * r + i] = a + b;
     }
   }
   __syncthreads();
-  const float to_value = __builtin_amdgcn_exp2f(largest - kWeightBits);  // the sums are of weights times 2^7 and scales over the largest
   auto row_top = [&](int row) {
     float m = wave_top[0][row];
 #pragma unroll
@@ -396,7 +403,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
     if (16 * r >= t.count) break;
     const int row = 16 * r + i;
     const float m = row_top(row);
-    const float keep = top[r] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top[r] - m) * to_value;
+    const float root = term_root(term_base[r], m);
     if (r > 0) __syncthreads();
     // Tile f of a lane: dims kTiles * (4 g + e) + f.
 #pragma unroll
@@ -404,7 +411,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
 #pragma unroll
       for (int f = 0; f < kTiles; f += 4) {
         f32x4 v = {acc[r][f][e], acc[r][f + 1][e], acc[r][f + 2][e], acc[r][f + 3][e]};
-        *reinterpret_cast<f32x4*>(&sums[wave][i][kTiles * (4 * g + e) + f]) = v * keep;
+        *reinterpret_cast<f32x4*>(&sums[wave][i][kTiles * (4 * g + e) + f]) = v * root * root;
       }
     __syncthreads();
     for (int e = threadIdx.x; e < 16 * (DIM / 4); e += kStreamThreads) {

@@ -9,7 +9,7 @@
 //
 // What bounds it. 4096 rows of 32 heads of 128: 137 GFLOP in 150 .. 165 us, 830 .. 915 TFLOP/s where a large plain product reaches
 // 1220. A wavefront has 1024 cycles of matrix work a tile and takes about 4500, reads, scores' arithmetic (one maximum, one
-// multiply-add, one exponential, half a conversion and half a sum a score) and matrix work one after another; two a SIMD fill one
+// multiply-add, one exponential, half a conversion and one sum a score) and matrix work one after another; two a SIMD fill one
 // another's gaps in part: the matrix cores are busy 40 % of the time, vector arithmetic half of it. Heads of 64 have twice the
 // exponentials for a matrix instruction and are bound by them.
 // LDS rows are swizzled by 16-byte pieces so that the 32 rows of a read fall on all banks.
@@ -65,8 +65,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
   constexpr int kTok = tile_tokens<DIM>(), kKeyPitch = 2 * DIM, kValuePitch = 2 * kTok;
   constexpr int kKeyBytes = kTok * kKeyPitch, kBuffer = 2 * kKeyBytes;
   extern __shared__ __attribute__((aligned(256))) uint8_t lds[];  // two buffers of keys and values
-  __shared__ __attribute__((aligned(32))) float key_scale[kMaxRuns], value_exp[kMaxRuns], value_per[kMaxRuns];
-  __shared__ float scale_top[kTileWaves];
+  __shared__ __attribute__((aligned(32))) float key_scale[kMaxRuns], value_log[kMaxRuns];
   __shared__ int holes;
   const Kv8Cache& c = p.c;
   const int head = blockIdx.x % c.heads;
@@ -99,7 +98,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
     load_query(p, n < my_count, at, [&](int k) { return 16 * k + 8 * h; }, q);
   }
   f32x16 acc[DIM / 32] = {};
-  float top = -__builtin_inff(), total = 0.0f, largest = 0.0f;
+  float base = kNothing, term_base = kNothing, total = 0.0f;
 
   // What a wavefront brings of a tile: a run, or two of heads of 64: its key rows 16 bytes a lane and load, and eight tokens by
   // four dims of its values a lane.
@@ -182,21 +181,8 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
       }
     }
     key_scale[mine] = my_run >= 0 ? ks : __builtin_nanf("");  // a NaN: nothing of the run is seen
-    float most = vs;
-    most = wave_max(most);
-    if (lane == 0) scale_top[wave] = most;
+    value_log[mine] = __builtin_amdgcn_logf(vs);
     __syncthreads();
-    most = fmaxf(fmaxf(fmaxf(scale_top[0], scale_top[1]), fmaxf(scale_top[2], scale_top[3])), largest);
-    // Scales as exponents relative to the largest so far; one under 2^-60 of it counts as that.
-    const float e = most > 0.0f ? fmaxf(__builtin_amdgcn_logf(vs / most), kLeastScale) + kWeightBits : 0.0f;
-    value_exp[mine] = e;
-    value_per[mine] = __builtin_amdgcn_exp2f(-e);
-    if (largest < most && largest > 0.0f) {
-      const float less = largest / most;
-#pragma unroll
-      for (int f = 0; f < DIM / 32; ++f) acc[f] *= less;
-    }
-    largest = most;
     const bool whole = !holes;
     const int tiles = (runs * kRun + kTok - 1) / kTok;
     auto clean = [&](int i) { return whole && window + (i + 1) * kTok <= min(stop, t.span.length); };
@@ -209,12 +195,11 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
       const int at = window + i * kTok;
       const bool more = i + 1 < tiles;
       if (more) ask(i + 1);
-      float ks[kTileRuns], ve[kTileRuns], per[kTileRuns];
+      float ks[kTileRuns], vl[kTileRuns];
 #pragma unroll
       for (int j = 0; j < kTileRuns; ++j) {
         ks[j] = key_scale[i * kTileRuns + j];
-        ve[j] = value_exp[i * kTileRuns + j];
-        per[j] = value_per[i * kTileRuns + j];
+        vl[j] = value_log[i * kTileRuns + j];
       }
       const bool some = my_count > 0 && at <= high_pos && (p.window == 0 || at + kTok > static_cast<int64_t>(low_pos) - p.window + 1);
       if (some) {
@@ -252,28 +237,30 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
             ks[j] = 1.0f;
           }
         }
-        float m = -__builtin_inff();
+        float m = -__builtin_inff(), most_term = m;
 #pragma unroll
         for (int j = 0; j < kTok / kRun; ++j) {
           float r = s[j / 2][8 * (j % 2)];
 #pragma unroll
           for (int e = 1; e < 8; ++e) r = fmaxf(r, s[j / 2][8 * (j % 2) + e]);
-          m = fmaxf(m, r * ks[j]);
+          r *= ks[j];
+          m = fmaxf(m, r);
+          most_term = fmaxf(most_term, r + vl[j]);
         }
-        float x0, x1;
-        swap_halves<false>(m, x0, x1);
-        m = fmaxf(x0, x1);
-        if (__any(m > top + kSlack)) {
-          m = fmaxf(m, top);
-          const float base = m == -__builtin_inff() ? 0.0f : m;
-          const float keep = __builtin_amdgcn_exp2f(top - base);
+        if (__any(m > base + kSlack || most_term > term_base + kSlack)) {
+          float x0, x1;
+          swap_halves<false>(m, x0, x1);
+          m = fmaxf(fmaxf(x0, x1) - kTermBits, base);
+          swap_halves<false>(most_term, x0, x1);
+          most_term = fmaxf(fmaxf(x0, x1) - kTermBits, term_base);
+          total *= __builtin_amdgcn_exp2f(base - m);
+          const float keep = __builtin_amdgcn_exp2f(term_base - most_term);
 #pragma unroll
           for (int f = 0; f < DIM / 32; ++f) acc[f] *= keep;
-          total *= keep;
-          top = m;
+          base = m;
+          term_base = most_term;
         }
-        const float base = top == -__builtin_inff() ? 0.0f : top;
-        const f16x2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+        const float least = kLeastLift - base;
         // A run's weights are made while the matrix cores work on the one before it, from values that were read before that.
         f16x8 a[2][DIM / 32];
         auto read_values = [&](int j, f16x8 (&to)[DIM / 32]) {
@@ -288,17 +275,18 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
 #pragma unroll
         for (int j = 0; j < kTok / kRun; ++j) {
           if (j + 1 < kTok / kRun) read_values(j + 1, a[(j + 1) % 2]);
-          const float lift = ve[j] - base;
-          float w[8], sum = 0.0f;
+          const float lift = fmaxf(vl[j] - term_base, least);
+          float w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 2][8 * (j % 2) + e], ks[j], lift));
           const f16x2 v[4] = {pack_f16(w[0], w[1]), pack_f16(w[2], w[3]), pack_f16(w[4], w[5]), pack_f16(w[6], w[7])};
+          float sum = w[0];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_fdot2(v[e], ones, sum, false);
-          total = __builtin_fmaf(sum, per[j], total);
-          const f16x8 weights = __builtin_bit_cast(f16x8, v);
+          for (int e = 1; e < 8; ++e) sum += w[e];
+          total = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-base - lift), total);
+          const f16x8 terms = __builtin_bit_cast(f16x8, v);
 #pragma unroll
-          for (int f = 0; f < DIM / 32; ++f) acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[j % 2][f], weights, acc[f], 0, 0, 0);
+          for (int f = 0; f < DIM / 32; ++f) acc[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[j % 2][f], terms, acc[f], 0, 0, 0);
         }
       }
       __builtin_amdgcn_s_setprio(0);
@@ -311,17 +299,17 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
   swap_halves<false>(total, x0, x1);
   const float sum = x0 + x1;
   if (n >= my_count) return;
-  const float to_value = largest * 0x1p-7f;  // kWeightBits
+  const float root = term_root(term_base, base);
   if (alone) {
     const int flat = my_first + n;
     const int64_t at = (t.span.row0 + flat / p.group) * p.ld_out + static_cast<int64_t>(head * p.group + flat % p.group) * DIM;
-    const float factor = sum > 0.0f ? to_value / sum : sum == 0.0f ? 0.0f : sum;
+    const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
 #pragma unroll
     for (int a = 0; a < DIM / 64; ++a)
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) store_four(p, at + 4 * (16 * a + 8 * b + 4 * h + k), four_dims<DIM>(acc, a, b, k) * factor);
+        for (int k = 0; k < 4; ++k) store_four(p, at + 4 * (16 * a + 8 * b + 4 * h + k), four_dims<DIM>(acc, a, b, k) * root * (root * inverse));
   } else {
     float* const part = partial_at<DIM>(p, (static_cast<int64_t>(seq) * p.row_tiles + tile) * c.heads + head, split, kTileRowsOfGroup);
     const int row = kTileRowsOfWave * wave + n;
@@ -331,9 +319,9 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<f32x4*>(part + row * DIM + 4 * (16 * a + 8 * b + 4 * h + k)) = four_dims<DIM>(acc, a, b, k) * to_value;
+          *reinterpret_cast<f32x4*>(part + row * DIM + 4 * (16 * a + 8 * b + 4 * h + k)) = four_dims<DIM>(acc, a, b, k) * root * root;
     if (h == 0) {
-      part[kTileRowsOfGroup * DIM + 2 * row] = top;
+      part[kTileRowsOfGroup * DIM + 2 * row] = base;
       part[kTileRowsOfGroup * DIM + 2 * row + 1] = sum;
     }
   }

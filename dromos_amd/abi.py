@@ -163,10 +163,12 @@ class Kernels:
         else:
             torch.cuda.synchronize()
 
-    def _lower(self, value):
+    def _lower(self, value, ld=None):
+        """``ld``: the row stride that the call gives for the tensor, where it gives one."""
         if isinstance(value, torch.Tensor):
-            if value.device.type != self.device or not value.is_contiguous():
-                raise ValueError(f"kernels take contiguous {self.device} tensors, not {value.device} / strides {value.stride()}")
+            rows = ld is not None and value.dim() == 2 and value.stride(1) == 1 and value.stride(0) == ld
+            if value.device.type != self.device or not (value.is_contiguous() or rows):
+                raise ValueError(f"kernels take contiguous {self.device} tensors, or columns of one with its row stride, not {value.device} / strides {value.stride()}")
             return value.data_ptr()
         return int(value) if isinstance(value, bool) else value
 
@@ -175,8 +177,11 @@ class Kernels:
         parameter, when it is the stream and was left out, is the current stream."""
         symbol = "lx_" + name
         fn = getattr(self.lib, symbol)
-        lowered = [self._lower(a) for a in args]
         params = self._params.get(symbol)
+        given = {name: a for (name, _), a in zip(params or (), args) if name.startswith("ld_")}
+        names = [name for name, _ in params or ()] + [""] * len(args)
+        # h_out has the stride of h, ld_h; other outputs have one of their own.
+        lowered = [self._lower(a, given.get("ld_" + name, given.get("ld_" + name.removesuffix("_out")))) for name, a in zip(names, args)]
         if params is None:  # not in the header: ctypes' own conversions, the stream behind the arguments
             if stream:
                 lowered.append(self.stream)

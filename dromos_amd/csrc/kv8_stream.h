@@ -146,8 +146,12 @@ __device__ __forceinline__ f16x2 pack_f16(float a, float b) { return f16x2{stati
 constexpr float kTermBits = 7.0f, kSlack = 8.0f + kTermBits, kNothing = -1e30f;
 constexpr float kLeastLift = -60.0f;  // a term over its weight, at least (log2)
 
-// Terms times this, twice, are relative to the reference `base`, as the sum of weights is (scales from 2^-126 to 2^121 come back so).
-__device__ __forceinline__ float term_root(float term_base, float base) { return __builtin_amdgcn_exp2f(0.5f * (term_base - base)); }
+// Sums of terms times this, twice, are relative to the reference `base`, as the sum of weights is, and held times 2^-32: sums over 2^17
+// tokens of values of f32's whole range (which their mean may have) are in it then, and values from 2^-101 on.
+__device__ __forceinline__ float term_root(float term_base, float base) { return __builtin_amdgcn_exp2f(0.5f * (term_base - base) - 16.0f); }
+
+// What such a sum has to be multiplied by. No token: 0; no number: that.
+__device__ __forceinline__ float over_weights(float sum) { return sum > 0.0f ? 0x1p32f / sum : sum == 0.0f ? 0.0f : sum; }
 
 // N eights of a query's values, `stride` values apart from `at` on, as the matrix instruction's operands; f32 ones are rounded to
 // bf16 here. A negative scale's sign goes to them, so that the scales of the scores never turn a largest one into a smallest.
@@ -429,8 +433,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) stream_kernel(const Attenti
       if (alone) {
         const int flat = t.first + row;
         const int64_t at = (t.span.row0 + flat / p.group) * p.ld_out + static_cast<int64_t>(head * p.group + flat % p.group) * DIM + d;
-        const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-        store_four(p, at, v * inverse);
+        store_four(p, at, v * over_weights(sum));
       } else {
         *reinterpret_cast<f32x4*>(part + row * DIM + d) = v;
         if (d == 0) {
@@ -518,8 +521,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttentionArgs p, int
   }
   const int flat = t.first + row;
   const int64_t at = (t.span.row0 + flat / p.group) * p.ld_out + static_cast<int64_t>(head * p.group + flat % p.group) * DIM + 4 * lane;
-  const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-  store_four(p, at, v * inverse);
+  store_four(p, at, v * over_weights(sum));
 }
 
 }  // namespace dro

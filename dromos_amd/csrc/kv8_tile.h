@@ -303,13 +303,13 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(const AttentionArgs p) {
   if (alone) {
     const int flat = my_first + n;
     const int64_t at = (t.span.row0 + flat / p.group) * p.ld_out + static_cast<int64_t>(head * p.group + flat % p.group) * DIM;
-    const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+    const float factor = root * over_weights(sum);
 #pragma unroll
     for (int a = 0; a < DIM / 64; ++a)
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) store_four(p, at + 4 * (16 * a + 8 * b + 4 * h + k), four_dims<DIM>(acc, a, b, k) * root * (root * inverse));
+        for (int k = 0; k < 4; ++k) store_four(p, at + 4 * (16 * a + 8 * b + 4 * h + k), four_dims<DIM>(acc, a, b, k) * root * factor);
   } else {
     float* const part = partial_at<DIM>(p, (static_cast<int64_t>(seq) * p.row_tiles + tile) * c.heads + head, split, kTileRowsOfGroup);
     const int row = kTileRowsOfWave * wave + n;

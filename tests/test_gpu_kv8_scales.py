@@ -143,3 +143,16 @@ def test_tokens_of_zeros_appended(hip, fmt, rows):
     after = cache.to("cpu")
     assert bool((after.scales[1] == 0).any())
     check(got, q, after, batch, 4, 0.1)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("rows,lengths", [([1, 6], [700, 90]), ([1, 6], [3000, 64]), ([150, 70], [700, 70]), ([150, 100], [3000, 400])])
+def test_values_of_the_types_range(hip, fmt, rows, lengths):
+    """Values up to 2^127, whose sum over the tokens is beyond f32 though their mean is not."""
+    batch = Batch(rows, lengths, 64)
+    cache = Cache(fmt, batch.pages, 2, 64, 32, 64).fill(1)
+    cache.scales[1] *= 2.0**125
+    cache.codes[1] = cache.codes[1] & 0x7F if fmt == "fp8" else cache.codes[1].view(torch.int8).abs().view(torch.uint8)
+    q = torch.randn(batch.T, 4 * 64, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    got = attention(hip, q.cuda(), cache.to("cuda"), batch.to("cuda"), 4, 0.125, out_dtype=torch.float32)
+    check(got, q, cache, batch, 4, 0.125)

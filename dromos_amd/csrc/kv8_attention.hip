@@ -13,9 +13,40 @@ struct Plan {
   int tile_rows;       // rows of its fullest tile
   int splits, chunk;
   int64_t workgroups, combiners;  // of the attention, and of the sums of its parts
-  int64_t bytes;                  // workspace
   bool fits;                      // the device can be asked for that many
 };
+
+// Whether `rows` rows (tokens times query heads of a head of the cache) are taken in tiles of 128 by kv8_tile.h's kernel. Below 97
+// rows a sequence tiles of 32 rows that stream the cache (again from L2 for each) are ahead: 8 streams of up to 8191
+// tokens at 40 / 64 / 96 / 128 rows 41.3 / 42.1 / 50.3 / 62.8 us, in tiles of 128 rows 47.6 / 48.9 / 52.1 / 54.3. Sums of 32 rows of
+// heads wider than 128 leave the tile kernel's wavefronts too few registers (2048 rows of 256: 246 us against 352).
+bool in_tiles(int64_t rows, int dim) { return rows > 96 && dim <= 128; }
+
+// Heads of 256 leave no registers for the sums of 32 rows.
+int rows_per_tile(int64_t rows, int dim) { return in_tiles(rows, dim) ? kTileRowsOfGroup : rows <= 16 || dim == 256 ? 16 : 32; }
+
+// Tiles with rows, of all heads: no more than T fills, and one begun for each sequence.
+int64_t busy_tiles(int64_t seqs, int64_t row_tiles, int per, int heads, int64_t T, int group) {
+  const int64_t items = seqs * row_tiles * heads, filled = (T * group / per + seqs) * heads;
+  return items < filled ? items : filled;
+}
+
+// One part where there is a workgroup a unit. Tiles of 128 rows need a quarter more: a unit with one of them alone is half idle
+// (1024 rows behind 7168 tokens, 264 workgroups: 208 us, in two parts 152).
+bool one_part(int64_t busy, bool tiles, int units) { return 4 * busy >= (tiles ? 5 : 4) * units; }
+
+// One sequence's parts are equally long. Several are of different lengths (which only the device knows): twice as many parts
+// then even out what the compute units have, 16 streams of up to 8192 tokens 41 -> 38 us, 8 of exactly 8192 33 -> 34. Rows in
+// two tiles of sixteen leave room for two workgroups a unit only: 8 streams of 5 rows 28.7 us, with twice the parts 34.8.
+int64_t parts_wanted(int64_t busy, bool tiles, int64_t seqs, int per, int units) {
+  const int each = seqs > 1 && per == 16 ? 4 : 2;
+  return busy <= 0 || one_part(busy, tiles, units) ? 1 : (each * units + busy - 1) / busy;
+}
+
+int64_t tokens_held(const lx_kv8& c, const lx_kv8_batch& b) {
+  const int64_t held = static_cast<int64_t>(b.ld_table) * c.page;
+  return held < b.max_length ? held : b.max_length;
+}
 
 // Enough parts that the device has about two workgroups a compute unit, none shorter than 256 tokens (a step of each
 // wavefront); one part where sequences and heads alone make a workgroup a unit.
@@ -24,35 +55,20 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads, int wi
   const int group = q_heads / c.heads;
   const int64_t most = b.max_rows < T ? b.max_rows : T;
   const int64_t rows = most * group;
-  // Heads of 256 leave no registers for the sums of 32 rows.
-  // Below 97 rows a sequence tiles of 32 rows that stream the cache (again from L2 for each) are ahead: 8 streams of up to 8191
-  // tokens at 40 / 64 / 96 / 128 rows 41.3 / 42.1 / 50.3 / 62.8 us, in tiles of 128 rows 47.6 / 48.9 / 52.1 / 54.3. Sums of 32 rows of
-  // heads wider than 128 leave the tile kernel's wavefronts too few registers (2048 rows of 256: 246 us against 352).
-  p.tiles = rows > 96 && c.dim <= 128;
-  p.per_tile = p.tiles ? kTileRowsOfGroup : rows <= 16 || c.dim == 256 ? 16 : 32;
+  p.tiles = in_tiles(rows, c.dim);
+  p.per_tile = rows_per_tile(rows, c.dim);
   const int per = p.per_tile;
   const int64_t row_tiles = (rows + per - 1) / per, limit = kMaxGridThreads / 256;
   if (row_tiles > limit || row_tiles * b.seqs > limit || row_tiles * b.seqs * c.heads > limit) return p;
   p.row_tiles = static_cast<int>(row_tiles);
   p.tile_rows = static_cast<int>(rows < per ? rows : per);
   // What a tile's rows see: all tokens, or the window, the tile's own and the run that the window begins in.
-  const int64_t held = static_cast<int64_t>(b.ld_table) * c.page;
-  const int64_t whole = held < b.max_length ? held : b.max_length;
-  int64_t length = whole;
+  int64_t length = tokens_held(c, b);
   const int64_t windowed = static_cast<int64_t>(window) + per / group + 2 + kRun;
   if (window > 0 && windowed < length) length = windowed;
   const int64_t items = static_cast<int64_t>(b.seqs) * p.row_tiles * c.heads;
-  // There are no more tiles with rows than T fills, and one begun for each sequence.
-  const int64_t filled = (static_cast<int64_t>(T) * group / per + b.seqs) * c.heads, busy = items < filled ? items : filled;
-  // One sequence's parts are equally long. Several are of different lengths (which only the device knows): twice as many parts
-  // then even out what the compute units have, 16 streams of up to 8192 tokens 41 -> 38 us, 8 of exactly 8192 33 -> 34. Rows in
-  // two tiles of sixteen leave room for two workgroups a unit only: 8 streams of 5 rows 28.7 us, with twice the parts 34.8.
-  const int each = b.seqs > 1 && per == 16 ? 4 : 2;
-  int64_t want = busy > 0 ? (each * compute_units() + busy - 1) / busy : 1;
-  // One part where there is a workgroup a unit. Tiles of 128 rows need a quarter more: a unit with one of them alone is half idle
-  // (1024 rows behind 7168 tokens, 264 workgroups: 208 us, in two parts 152).
-  if (4 * busy >= (p.tiles ? 5 : 4) * compute_units()) want = 1;
-  int64_t chunk = (length + want - 1) / (want > 0 ? want : 1);
+  const int64_t want = parts_wanted(busy_tiles(b.seqs, p.row_tiles, per, c.heads, T, group), p.tiles, b.seqs, per, compute_units());
+  int64_t chunk = (length + want - 1) / want;
   chunk = (chunk + 255) / 256 * 256;
   // Parts cost a second kernel (about 4 us); one part costs a step of each wavefront more for every 256 tokens (1.6 us).
   if (length <= 768) chunk = 768;
@@ -66,11 +82,50 @@ Plan plan_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads, int wi
   const int64_t combined = items * p.tile_rows, each_time = p.splits <= kFewParts ? 1024 / c.dim : 1;
   p.combiners = p.splits > 1 ? (combined + each_time - 1) / each_time : 0;
   p.fits = p.workgroups <= limit && p.combiners <= limit;
-  // The workspace is for any window: one may have as many parts as are wanted of 256 tokens, or of the longest there are.
-  int64_t parts = want < (whole + 255) / 256 ? want : (whole + 255) / 256;
-  if (!p.tiles && parts < (whole + kMaxRuns * kRun - 1) / (kMaxRuns * kRun)) parts = (whole + kMaxRuns * kRun - 1) / (kMaxRuns * kRun);
-  p.bytes = parts > 1 ? items * parts * per * (c.dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
   return p;
+}
+
+// Bytes of partial sums of `row_tiles` tiles of `per` rows a sequence at most, whatever the window: it may have as many parts as are
+// wanted of 256 tokens, or of the longest there are.
+int64_t partial_bytes(int64_t seqs, int64_t row_tiles, int per, bool tiles, int heads, int dim, int64_t whole, int64_t want) {
+  const int64_t runs = (whole + 255) / 256, longest = (whole + kMaxRuns * kRun - 1) / (kMaxRuns * kRun);
+  int64_t parts = want < runs ? want : runs;
+  if (!tiles && parts < longest) parts = longest;
+  return parts > 1 ? seqs * row_tiles * heads * parts * per * (dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+}
+
+// The workspace of a call and of every smaller one: fewer rows or sequences fill fewer compute units, are cut into more parts for
+// it, and may leave more partial sums than the call itself. From one part on those only grow with rows and sequences; in front of
+// that there are few numbers of tiles and sequences to look at (about as many tiles, of all heads and sequences, as compute units).
+int64_t workspace_for(const lx_kv8& c, const lx_kv8_batch& b, int T, int q_heads) {
+  const int group = q_heads / c.heads, units = compute_units();
+  const int64_t rows = static_cast<int64_t>(b.max_rows < T ? b.max_rows : T) * group, whole = tokens_held(c, b), limit = kMaxGridThreads / 256;
+  int64_t most = 0;
+  // The rows that have tiles of one height, from the last on.
+  for (int64_t last = rows, first; last > 0; last = first - 1) {
+    const int per = rows_per_tile(last, c.dim);
+    const bool tiles = in_tiles(last, c.dim);
+    first = tiles ? 97 : per == 32 ? 17 : 1;
+    // n tiles a sequence, in calls of as few rows as have them. Whether one part is enough.
+    auto look_at = [&](int64_t seqs, int64_t n) {
+      const int64_t least = n * per - per + 1 > first ? n * per - per + 1 : first;
+      const int64_t busy = busy_tiles(seqs, n, per, c.heads, (least + group - 1) / group, group);
+      if (n <= limit && n * seqs <= limit && n * seqs * c.heads <= limit) {
+        const int64_t bytes = partial_bytes(seqs, n, per, tiles, c.heads, c.dim, whole, parts_wanted(busy, tiles, seqs, per, units));
+        most = bytes > most ? bytes : most;
+      }
+      return one_part(busy, tiles, units);
+    };
+    const int64_t most_tiles = (last + per - 1) / per;
+    for (int64_t n = (first + per - 1) / per; n <= most_tiles;) {
+      const bool alone = look_at(1, n);
+      bool enough = alone;
+      for (int64_t seqs = 2; seqs <= b.seqs && !enough; ++seqs) enough = look_at(seqs, n);
+      look_at(b.seqs, n);
+      n = alone && n < most_tiles ? most_tiles : n + 1;
+    }
+  }
+  return most;
 }
 
 template <int F, int DIM>
@@ -136,7 +191,7 @@ int lx_kv8_attention(const void* q, lx_dtype q_dtype, int ld_q, const lx_kv8* ca
 int64_t lx_kv8_attention_workspace_bytes(const lx_kv8* cache, const lx_kv8_batch* batch, int T, int q_heads) {
   if (kv8_check_cache(cache) || kv8_check_batch(batch, T, *cache) || T == 0 || batch->seqs == 0 || batch->max_rows == 0) return 0;
   if (q_heads < 1 || q_heads > 65536 || q_heads % cache->heads != 0) return 0;
-  return plan_for(*cache, *batch, T, q_heads, 0).bytes;
+  return workspace_for(*cache, *batch, T, q_heads);
 }
 
 // For tests, without a device (256 compute units): {rows of a tile, tiles a sequence, parts, tokens of a part, workgroups, partial

@@ -265,10 +265,11 @@ LX_API int lx_moe_experts_noalloc(const void* latent, const int32_t* ids, const 
  * q f32 (rounded to bf16, as lx_gemm_w's BF16 math does) or bf16, out f32 or bf16, row strides in elements; products on the matrix
  * cores (a weight times its block's value scale is rounded to f16, and perhaps to nothing under 2^-32 of its row's largest), sums
  * and softmax in f32 (of the weights themselves: what a token weighs does not depend on its values; values under 2^-101 may count as
- * zeros), one pass over the keys. Contents of the cache where no token lies (NaNs
- * too) have no part in it; where one lies its codes and scales are numbers, as lx_kv8_append writes them. The workspace
- * (lx_kv8_attention_workspace_bytes for the same cache, batch, T and q_heads, whatever the window; 0: none, may be null) holds partial
- * sums of long sequences, 16-byte aligned, may hold garbage, and belongs to one call at a time. */
+ * zeros), one pass over the keys. Contents of the cache where no token lies (NaNs too) have no part in it; where one lies its codes
+ * and scales are numbers, as lx_kv8_append writes them. The workspace holds partial sums of long sequences, 16-byte aligned, may hold
+ * garbage, and belongs to one call at a time. lx_kv8_attention_workspace_bytes (0: none, may be null) answers for the call of these
+ * sizes and for every one with no larger T, seqs, max_rows, max_length and ld_table on the same cache and q_heads, whatever the window:
+ * smaller calls can want more than the largest one. */
 typedef struct {
   lx_wtype type;
   void* k;

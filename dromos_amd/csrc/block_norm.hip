@@ -3,7 +3,8 @@
 //
 // Bytes decide: y, h and the gate are read once, h and x written once, and a row stays in its workgroup's registers between
 // (four vectors of eight values a thread at most, 32768 values a row). A workgroup takes one row. Sums are f32, in
-// an order that goes by the width alone, and with it a row's bits.
+// an order that goes by the width and by whether all rows and vectors can be moved 16 bytes at a time, and with it a row's bits: they
+// do not depend on how many rows there are.
 #include "tile_mfma.h"
 
 namespace dro {
@@ -215,6 +216,8 @@ bool aligned(const void* p, int64_t ld, int type) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (type == LX_BF16 ? 2 : 4) % 16 == 0;
 }
 
+// Rows that cannot be moved 16 bytes at a time are read a value a lane: 4096 rows of 8191 values 159 us, of 8192 51. Four vectors a
+// thread (more than 16384 values) leave four wavefronts a SIMD: 1024 rows of 32768 63 us, 2048 of 16384 52.
 // As many threads as the row has vectors for N each, up to 1024; of single values half as many each where there are threads for it.
 template <int V, int N>
 int launch(NormArgs a, int T, hipStream_t s) {

@@ -19,7 +19,8 @@ struct Plan {
 // Whether `rows` rows (tokens times query heads of a head of the cache) are taken in tiles of 128 by kv8_tile.h's kernel. Below 97
 // rows a sequence tiles of 32 rows that stream the cache (again from L2 for each) are ahead: 8 streams of up to 8191
 // tokens at 40 / 64 / 96 / 128 rows 41.3 / 42.1 / 50.3 / 62.8 us, in tiles of 128 rows 47.6 / 48.9 / 52.1 / 54.3. Sums of 32 rows of
-// heads wider than 128 leave the tile kernel's wavefronts too few registers (2048 rows of 256: 246 us against 352).
+// heads wider than 128 leave the tile kernel's wavefronts too few registers
+// (2048 rows of 16 heads of 256 behind 2048 tokens: 246 us against 352; 260 with sums of unrounded terms).
 bool in_tiles(int64_t rows, int dim) { return rows > 96 && dim <= 128; }
 
 // Heads of 256 leave no registers for the sums of 32 rows.

@@ -22,10 +22,11 @@
 // heads wider than 128) and keep sums of their own; the workgroup adds them up at its end, in order. Where a sequence has several
 // such parts they leave their sums in the workspace, and a second kernel adds those, in order.
 //
-// What bounds it (heads of 128, int8 or fp8). One sequence of 131072 tokens: 50.0 us for 268 MB, 5.4 TB/s, the rate of a copy.
-// 32 of up to 4096 tokens, as uneven as they come: 35 us where their bytes want 27, the longest one's workgroups end last. 8 of 5 rows
-// (20 a head, two tiles' worth of registers): 23.8 us against 12.6, two workgroups a unit wait for memory. 517 tokens: 10 us, two
-// steps of a wavefront whose every load follows one before it.
+// What bounds it (heads of 128, int8 or fp8). One sequence of 131072 tokens: 50.6 us for 268 MB, 5.3 TB/s, the rate of a copy.
+// 32 of up to 4096 tokens, as uneven as they come: 35.9 us where their bytes want 27, the longest one's workgroups end last. 8 of 5 rows
+// (20 a head, two tiles' worth of registers): 23.0 us where their bytes want 12.6; parts are cut by the longest possible sequence, so
+// 256 of 512 workgroups find a token, one a unit, and its four wavefronts wait for memory in each of four steps. 517 tokens: 9.5 us,
+// two steps of a wavefront whose every load follows one before it.
 #pragma once
 
 #include "kv8.h"

@@ -7,11 +7,11 @@
 // scores of one row, tokens 8 a + 4 h + b (h = lane / 32), and a sum over 16 tokens takes its eight of them as they
 // lie, so the value columns are stored in that order and weights never change lanes.
 //
-// What bounds it. 4096 rows of 32 heads of 128: 137 GFLOP in 150 .. 165 us, 830 .. 915 TFLOP/s where a large plain product reaches
-// 1220. A wavefront has 1024 cycles of matrix work a tile and takes about 4500, reads, scores' arithmetic (one maximum, one
+// What bounds it. 4096 rows of 32 heads of 128: 137 GFLOP in 158 .. 176 us (devices differ), 780 .. 870 TFLOP/s where a large plain product
+// reaches 1220. A wavefront has 1024 cycles of matrix work a tile and takes about 4600, reads, scores' arithmetic (one maximum, one
 // multiply-add, one exponential, half a conversion and one sum a score) and matrix work one after another; two a SIMD fill one
 // another's gaps in part: the matrix cores are busy 40 % of the time, vector arithmetic half of it. Heads of 64 have twice the
-// exponentials for a matrix instruction and are bound by them.
+// score arithmetic for a matrix instruction: 4096 rows of 32 heads 105 us, 655 TFLOP/s.
 // LDS rows are swizzled by 16-byte pieces so that the 32 rows of a read fall on all banks.
 #pragma once
 

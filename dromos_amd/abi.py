@@ -22,6 +22,9 @@ DTYPE = {torch.float32: F32, torch.bfloat16: BF16}
 W_BF16, W_INT8, W_FP8, W_NVFP4, W_BF16X = 0, 1, 2, 3, 4
 MATH_BF16, MATH_INT8, MATH_FP8, MATH_FP4 = 0, 1, 2, 3
 NORM_RMS, NORM_LAYER = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS, ROPE_WAVES = 0, 1, 2, 3, 4
+ACT_NONE, ACT_SILU = 0, 1
+DECAY_HEAD, DECAY_LOG, DECAY_STEP = 0, 1, 2
 NOT_SUPPORTED = 801
 FORMATS = {"bf16": W_BF16, "int8": W_INT8, "fp8": W_FP8, "nvfp4": W_NVFP4}
 
@@ -69,6 +72,25 @@ class LxKv8Batch(ctypes.Structure):
         ("ld_table", ctypes.c_int),
         ("max_rows", ctypes.c_int),
         ("max_length", ctypes.c_int),
+    ]
+
+
+class LxStates(ctypes.Structure):
+    """lx_states (include/dromos_hip.h): what sequences keep between calls of lx_causal_conv and lx_linear_attention."""
+
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("count", ctypes.c_int)]
+
+
+class LxDecay(ctypes.Structure):
+    """lx_decay (include/dromos_hip.h): how a linear attention's state fades."""
+
+    _fields_ = [
+        ("kind", ctypes.c_int),
+        ("x", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("ld", ctypes.c_int),
+        ("rate", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
     ]
 
 

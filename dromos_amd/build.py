@@ -18,7 +18,8 @@ SOURCES = ["runtime.hip", "quant.hip", "gemv.hip", "gemv_bf16.hip", "gemv_int8.h
            "gemm_ring_bf16.hip", "gemm_ring_int8.hip", "gemm_ring_fp8.hip", "gemm_ring_nvfp4.hip",
            "gemm_block_bf16.hip", "gemm_block_int8.hip", "gemm_block_fp8.hip", "gemm_block_nvfp4.hip", "gemm_block_int8_math.hip", "gemm_block_fp8_math.hip",
            "moe.hip", "moe_grouped.hip", "moe_block_bf16.hip", "moe_block_int8.hip", "moe_block_fp8.hip", "moe_block_nvfp4.hip", "router.hip", "checkpoint.hip",
-           "kv8_append.hip", "kv8_attention.hip", "block_norm.hip"]
+           "kv8_append.hip", "kv8_attention.hip", "block_norm.hip",
+           "rotate.hip", "causal_conv.hip", "linear_attention.hip"]
 
 # -ffp-contract=off: the epilogues and the ordered sums are written as separate multiplies and adds, as the
 # CPU reference computes them; fused operations are spelled __builtin_fmaf where they are meant.

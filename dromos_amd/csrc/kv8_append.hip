@@ -10,6 +10,7 @@
 // A prompt is bound by bytes. A single token is bound by the latency of what it has to follow: the rows' bounds and lengths (every
 // wavefront looks through them by itself), the page table, the block's scale; its values are asked for before the first of them.
 #include "kv8.h"
+#include "rotation.h"
 #include "tile_mfma.h"
 
 namespace dro {
@@ -118,30 +119,6 @@ __device__ __forceinline__ void store_unit(void* x, int dtype, bool wide, int64_
 __device__ __forceinline__ void quarters_of(const AppendArgs& p, const Unit& n, int pair, double (&quarters)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) quarters[j] = n.turned ? static_cast<double>(p.freq[pair + j]) * 0.63661977236758134308 : 0.0;
-}
-
-// The cosines and sines of the four angles at a position. The product of a 31-bit and a 53-bit number is right to 2^-53 in 64 bits;
-// whole quarter turns are taken off it there, so what is left of a far position is as good as of a near one. The rest u, an
-// eighth of a turn at most, goes into Taylor's series in f32 (what they leave off is below 2^-29 and 2^-32).
-__device__ __forceinline__ void angles(const double (&quarters)[4], int position, float* c, float* s) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const double turned = static_cast<double>(position) * quarters[j], whole = rint(turned);
-    const float u = static_cast<float>((turned - whole) * 1.57079632679489661923), x = u * u;
-    float a = __builtin_fmaf(x, 1.0f / 362880.0f, -1.0f / 5040.0f), b = __builtin_fmaf(x, -1.0f / 3628800.0f, 1.0f / 40320.0f);
-    a = __builtin_fmaf(x, a, 1.0f / 120.0f);
-    b = __builtin_fmaf(x, b, -1.0f / 720.0f);
-    a = __builtin_fmaf(x, a, -1.0f / 6.0f);
-    b = __builtin_fmaf(x, b, 1.0f / 24.0f);
-    a = __builtin_fmaf(x * u, a, u);  // sin u
-    b = __builtin_fmaf(x, b, -0.5f);
-    b = __builtin_fmaf(x, b, 1.0f);  // cos u
-    const int quadrant = static_cast<int>(static_cast<long long>(whole)) & 3;
-    c[j] = quadrant & 1 ? a : b;
-    s[j] = quadrant & 1 ? b : a;
-    if (quadrant == 1 || quadrant == 2) c[j] = -c[j];
-    if (quadrant >= 2) s[j] = -s[j];
-  }
 }
 
 __device__ __forceinline__ void turn(bool interleaved, const float* c, const float* s, float* v) {

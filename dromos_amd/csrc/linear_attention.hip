@@ -1,0 +1,78 @@
+// lx_linear_attention: linear attention with a decay for each head, a state of each sequence and head kept between calls.
+#include "linear_step.h"
+
+namespace dro {
+namespace {
+
+constexpr int kMaxDk = 256, kMaxDv = 512, kMaxHeads = 4096;
+
+template <int COLS, int ROWS>
+int launch_step(const LinearArgs& p, hipStream_t s) {
+  const int64_t waves = static_cast<int64_t>(p.b.seqs) * p.heads * ((p.dv + 4 * COLS - 1) / (4 * COLS));
+  const int64_t groups = (waves + 3) / 4;
+  if (groups * 256 > kMaxGridThreads) return kInvalid;
+  hipLaunchKernelGGL((linear_step_kernel<COLS, ROWS>), dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, p);
+  return status_of(hipGetLastError());
+}
+
+int steps(const LinearArgs& p, hipStream_t s) {
+  if (p.dk <= 64) return launch_step<8, 8>(p, s);
+  // 16 columns a wavefront where 32 leave the device short of wavefronts.
+  const bool few = static_cast<int64_t>(p.b.seqs) * p.heads * ((p.dv + 31) / 32) < 4 * compute_units();
+  if (p.dk <= 128) return few ? launch_step<4, 8>(p, s) : launch_step<8, 16>(p, s);
+  return few ? launch_step<4, 16>(p, s) : launch_step<8, 32>(p, s);
+}
+
+bool sizes_known(int T, int heads, int k_heads, int dk, int dv) {
+  return T >= 0 && T < (1 << 30) && k_heads >= 1 && heads >= k_heads && heads <= kMaxHeads && heads % k_heads == 0 && dk >= 8 && dk <= kMaxDk &&
+         dk % 8 == 0 && dv >= 8 && dv <= kMaxDv && dv % 8 == 0;
+}
+
+}  // namespace
+}  // namespace dro
+
+using namespace dro;
+
+extern "C" {
+
+int64_t lx_linear_attention_workspace_bytes(const lx_kv8_batch* batch, int T, int heads, int k_heads, int dk, int dv) {
+  if (!batch || !sizes_known(T, heads, k_heads, dk, dv)) return -1;
+  return 0;
+}
+
+int lx_linear_attention(const void* q, const void* k, const void* v, lx_dtype dtype, int ld_q, int ld_k, int ld_v, const lx_decay* decay,
+                        const float* skip, const void* gate, lx_dtype gate_dtype, int ld_gate, const lx_kv8_batch* batch,
+                        const lx_states* states, void* out, lx_dtype out_dtype, int ld_out, int T, int heads, int k_heads, int dk, int dv,
+                        float scale, void* workspace, void* stream) {
+  if (!sizes_known(T, heads, k_heads, dk, dv)) return fail(kInvalid);
+  if (int st = mix_check(batch, T)) return fail(st);
+  if (int st = mix_check_states(states)) return fail(st);
+  if (!mix_type(dtype) || !mix_type(out_dtype) || (gate && !mix_type(gate_dtype))) return fail(kInvalid);
+  if (!decay || (decay->kind != LX_DECAY_HEAD && decay->kind != LX_DECAY_LOG && decay->kind != LX_DECAY_STEP)) return fail(kInvalid);
+  if (states && (reinterpret_cast<uintptr_t>(states->in) | reinterpret_cast<uintptr_t>(states->out)) % 16 != 0) return fail(kInvalid);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(kInvalid);
+  const bool by_token = decay->kind != LX_DECAY_HEAD;
+  if (by_token && !mix_type(decay->dtype)) return fail(kInvalid);
+  if (T == 0 || batch->seqs == 0) return kOk;
+  if (!q || !k || !v || !out || (by_token ? !decay->x : !decay->rate)) return fail(kInvalid);
+  const int64_t keys = static_cast<int64_t>(k_heads) * dk, values = static_cast<int64_t>(heads) * dv;
+  if (T > 1 && (ld_q < keys || ld_k < keys || ld_v < values || ld_out < values || (gate && ld_gate < values) || (by_token && decay->ld < heads)))
+    return fail(kInvalid);
+  LinearArgs p{};
+  p.q = q, p.k = k, p.v = v, p.x = by_token ? decay->x : nullptr, p.rate = decay->rate;
+  p.bias = decay->kind == LX_DECAY_STEP ? decay->bias : nullptr;
+  p.skip = skip, p.gate = gate, p.out = out;
+  p.ld_q = ld_q, p.ld_k = ld_k, p.ld_v = ld_v, p.ld_x = decay->ld, p.ld_gate = ld_gate, p.ld_out = ld_out;
+  p.type = dtype, p.x_type = decay->dtype, p.gate_type = gate_dtype, p.out_type = out_dtype;
+  p.kind = decay->kind, p.heads = heads, p.k_heads = k_heads, p.group = heads / k_heads, p.dk = dk, p.dv = dv;
+  auto in16 = [&](const void* t, int ld, int type) { return mix_aligned(t, T > 1 ? ld : 0, type, 16); };
+  p.wide = in16(q, ld_q, dtype) && in16(k, ld_k, dtype) && in16(v, ld_v, dtype) && (!gate || in16(gate, ld_gate, gate_dtype)) && in16(out, ld_out, out_dtype);
+  p.scale = scale;
+  p.b = mix_batch(*batch, T);
+  p.states = mix_states(states);
+  if (p.b.max_rows == 0 || p.b.seqs == 0) return kOk;
+  if (int st = steps(p, as_stream(stream))) return fail(st);
+  return kOk;
+}
+
+}  // extern "C"

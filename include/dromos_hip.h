@@ -308,6 +308,88 @@ LX_API int lx_block_norm(lx_norm norm, const void* y, lx_dtype y_dtype, int ld_y
                          const void* weight, const void* bias, lx_dtype w_dtype, void* x, lx_dtype x_dtype, int ld_x, float eps, int T,
                          int H, void* stream);
 
+/* ---- a linear-attention mixer's step between its products (this library's own too) -------------------------------------------------
+ * x = lx_block_norm(...); z = lx_gemm_w(x); lx_causal_conv(z); lx_rotate(q, k); lx_linear_attention(q, k, v); lx_block_norm(...); lx_gemm_w
+ *
+ * The rows of a call are an lx_kv8_batch's, the one that an attention layer of the same model takes; of it these calls read seqs, rows,
+ * lengths and max_rows (table, ld_table and max_length may be anything). Row i of a sequence of n rows and length L is its token
+ * p = L - n + i. Rows from max_rows on, in front of position 0 and behind the last sequence belong to nobody: what stands there is not
+ * used and their outputs stay as they were. lengths may be null in lx_causal_conv and lx_linear_attention (no sequence begins with
+ * this call, every row counts) and in lx_rotate with positions of its own. Numbers in device memory are bounded as lx_kv8's are.
+ *
+ * What a sequence keeps between calls is a slot of a caller's tensor:
+ *   in     where states come from, null: every sequence starts from zeros; a sequence whose first token is among the call's rows (L <= n)
+ *          starts from zeros too, whatever its slot holds
+ *   out    where they go, null: nowhere; `in` itself, or apart from it (drafted tokens that may be refused leave the states as they are)
+ *   slots  [seqs] slot of each sequence, null: sequence s has slot s. One outside [0, count) is none: zeros come from it, nothing goes to it.
+ * A sequence without a row in the call leaves its slot of `out` alone. A slot belongs to one sequence of a call. */
+typedef struct {
+  const void* in;
+  void* out;
+  const int32_t* slots;
+  int count;
+} lx_states;
+/* lx_rotate: y[t, h, :rot] = amplitude * x[t, h, :rot] turned by the angles p * freq[i], i < rot / 2 (f32 on the device; formed and reduced in
+ * 64 bits), pairs (i, i + rot / 2), or (2 i, 2 i + 1) where `interleaved`: (a, b) -> (a cos - b sin, b cos + a sin); the values behind them as
+ * they are. rot even (0: a copy), dim up to 1024. p is positions[t] (any int32; batch may be null then and every row counts) or, where positions is
+ * null, the batch's. x and y f32 or bf16, row strides in elements (heads behind one another); y may be x where type and stride agree.
+ * Queries and keys that lie side by side in a row are one call. T * heads < 2^31.
+ *
+ * lx_rotary_frequencies: on the host, freq[rot / 2] and the amplitude of a scaled rotation (host pointers; either may be null), by f_i = base^(-2 i / rot) and
+ * `original`, the tokens a model was trained on:
+ *   LX_ROPE_PLAIN    f_i
+ *   LX_ROPE_LINEAR   f_i / factor
+ *   LX_ROPE_BASE     f_i of the base base * factor^(rot / (rot - 2)), rot 4 or more
+ *   LX_ROPE_PARTS    f_i (k_i + (1 - k_i) / factor), k_i = 1 below dimension d(high), 0 from d(low) on, a line between them;
+ *                    d(r) = rot ln(original / (2 pi r)) / (2 ln base), d(high) rounded down to 0 at least, d(low) up to rot - 1 at most (r turns in the
+ *                    original context; low 1, high 32 are usual); amplitude 0.1 ln(factor) + 1
+ *   LX_ROPE_WAVES    the same form with k_i = (original f_i / (2 pi) - low) / (high - low) within 0 .. 1 (low 1, high 4 are usual)
+ * The amplitude is 1 where nothing else is said. factor >= 1, base > 1, original > 0, 0 < low < high where they are used. lx_kv8_append takes such
+ * frequencies too; it has no amplitude, whose square is a factor of lx_kv8_attention's scale where all of a head is turned.
+ *
+ * lx_causal_conv: y[t, c] = act(bias[c] + sum_j weight[c, j] x[t - (width - 1) + j, c]) along each sequence, width 2 .. 8 taps, sums in f32; weight
+ * [C, width] and bias [C] (or null) in w_dtype. In front of a sequence's rows stand the kept ones: states [count, width - 1, C] in x's type,
+ * the oldest first, and afterwards the sequence's last width - 1 rows, bits as they were. x and y f32 or bf16, y apart from x.
+ * LX_ACT_SILU: v / (1 + exp(-v)).
+ *
+ * lx_linear_attention: a state S [dk, dv] of each sequence and head, token after token
+ *   S = exp(g) S + b k v^T,  out = (scale S^T q + skip[h] v) silu(gate)
+ * q and k [T, k_heads * dk] (head h reads head h / (heads / k_heads)), v, gate and out [T, heads * dv]; skip f32 [heads] or null (0), gate f32 or bf16
+ * or null (1). dk a multiple of 8 up to 256, dv a multiple of 8 up to 512, heads up to 4096. The decay (a host struct, x [T, heads] and rate, bias [heads] on the
+ * device), g at most 0, minus infinity a fresh start (g counts as at least -10000):
+ *   LX_DECAY_HEAD  g = rate[h], b = 1
+ *   LX_DECAY_LOG   g = x[t, h] * rate[h] (rate null: 1), b = 1
+ *   LX_DECAY_STEP  d = log(1 + exp(x[t, h] + bias[h])) (bias null: 0), g = d * rate[h] (rate null: -1), b = d
+ * q, k and v all bf16 or all f32 (rounded to bf16, as lx_gemm_w's BF16 math does), out f32 or bf16, row strides in elements; states f32
+ * [count, heads, dk, dv], 16-byte aligned, or null. Calls of few rows a sequence go token by token in f32, longer ones by
+ * chunks of 64 tokens on the matrix cores: there f32 factors (weights of tokens, values times their decay, the state) enter products as two
+ * bf16 (16 bits are kept) and sums are f32. Neither form's bits depend on the other sequences of the call; which form a call takes depends on max_rows, and where
+ * a long sequence is cut on T and the sizes. The workspace
+ * holds states in front of the parts of long sequences, 16-byte aligned, may hold garbage, and belongs to one call at a time;
+ * lx_linear_attention_workspace_bytes (0: none, may be null) answers for the call of these sizes and for every one with no larger T. */
+typedef enum { LX_ROPE_PLAIN = 0, LX_ROPE_LINEAR = 1, LX_ROPE_BASE = 2, LX_ROPE_PARTS = 3, LX_ROPE_WAVES = 4 } lx_rope;
+typedef enum { LX_ACT_NONE = 0, LX_ACT_SILU = 1 } lx_act;
+typedef enum { LX_DECAY_HEAD = 0, LX_DECAY_LOG = 1, LX_DECAY_STEP = 2 } lx_decay_kind;
+typedef struct {
+  lx_decay_kind kind;
+  const void* x;
+  lx_dtype dtype;
+  int ld;
+  const float* rate;
+  const float* bias;
+} lx_decay;
+LX_API int lx_rotary_frequencies(lx_rope kind, double base, int rot, double factor, double original, double low, double high, float* freq,
+                                 float* amplitude);
+LX_API int lx_rotate(const void* x, lx_dtype x_dtype, int ld_x, void* y, lx_dtype y_dtype, int ld_y, const lx_kv8_batch* batch,
+                     const int32_t* positions, const float* freq, float amplitude, int rot, int interleaved, int T, int heads, int dim, void* stream);
+LX_API int lx_causal_conv(const void* x, lx_dtype x_dtype, int ld_x, const void* weight, const void* bias, lx_dtype w_dtype, int width, lx_act act,
+                          const lx_kv8_batch* batch, const lx_states* states, void* y, lx_dtype y_dtype, int ld_y, int T, int C, void* stream);
+LX_API int lx_linear_attention(const void* q, const void* k, const void* v, lx_dtype dtype, int ld_q, int ld_k, int ld_v, const lx_decay* decay,
+                               const float* skip, const void* gate, lx_dtype gate_dtype, int ld_gate, const lx_kv8_batch* batch,
+                               const lx_states* states, void* out, lx_dtype out_dtype, int ld_out, int T, int heads, int k_heads, int dk, int dv,
+                               float scale, void* workspace, void* stream);
+LX_API int64_t lx_linear_attention_workspace_bytes(const lx_kv8_batch* batch, int T, int heads, int k_heads, int dk, int dv);
+
 /* ---- runtime (replaces engine/cuda/kernels.h:308-381 on the HIP runtime) --------------------------- */
 typedef struct {
   char name[256];

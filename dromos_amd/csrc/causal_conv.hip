@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(256) conv_kernel(const ConvArgs p) {
         for (int t = 0; t < kTaps; ++t) last = t == kept ? weight[t][c] : last;
       }
       y[c] = __builtin_fmaf(last, now[c], y[c]);
-      if (p.silu) y[c] = silu(y[c]);
+      if (p.silu) y[c] = quick_silu(y[c]);
 #pragma unroll
       for (int t = 0; t + 1 < kTaps; ++t) {
         if (t + 1 < kept) seen[t][c] = seen[t + 1][c];

@@ -58,7 +58,7 @@ __device__ __forceinline__ void finish_four(const LinearArgs& p, int64_t row, in
   if (p.gate) {
     const f32x4 z = load_four(p.gate, p.gate_type, p.wide, row * p.ld_gate + at);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] *= silu(z[j]);
+    for (int j = 0; j < 4; ++j) o[j] *= quick_silu(z[j]);
   }
   store_four(p.out, p.out_type, p.wide, row * p.ld_out + at, o);
 }

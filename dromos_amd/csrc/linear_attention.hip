@@ -1,10 +1,12 @@
 // lx_linear_attention: linear attention with a decay for each head, a state of each sequence and head kept between calls.
+#include "linear_chunk.h"
 #include "linear_step.h"
 
 namespace dro {
 namespace {
 
 constexpr int kMaxDk = 256, kMaxDv = 512, kMaxHeads = 4096;
+constexpr int kMostSteps = 16;  // rows of a sequence that go token by token
 
 template <int COLS, int ROWS>
 int launch_step(const LinearArgs& p, hipStream_t s) {
@@ -23,6 +25,78 @@ int steps(const LinearArgs& p, hipStream_t s) {
   return few ? launch_step<4, 16>(p, s) : launch_step<8, 32>(p, s);
 }
 
+// How a call of chunks is cut: heads (or columns of wide ones) by workgroups, long sequences into parts of `size` rows.
+struct Cut {
+  int waves, teams;  // of a head's columns, heads of a workgroup
+  int across;        // workgroups of a key head
+  int size, places;  // rows of a part; parts of long sequences there may be
+};
+
+constexpr int kLeastPart = 256;
+
+Cut cut_of(int T, int max_rows, int heads, int k_heads, int dk, int dv) {
+  Cut c;
+  const int group = heads / k_heads;
+  c.waves = dv <= 64 ? 2 : 4;
+  c.teams = dv <= 64 && group > 1 ? 2 : 1;
+  c.across = c.teams > 1 ? (group + 1) / 2 : group * ((dv + 32 * c.waves - 1) / (32 * c.waves));
+  // As many parts as fill the device once: a part costs a second look at its keys and values.
+  const int64_t places = static_cast<int64_t>(dk > 128 ? 1 : 2) * compute_units(), columns = static_cast<int64_t>(c.across) * k_heads;
+  const int64_t even = (T * columns + places - 1) / places, size = (even + kChunk - 1) / kChunk * kChunk;
+  c.size = static_cast<int>(size < kLeastPart ? kLeastPart : size);
+  // No call of T rows or fewer has more: a part is no shorter than T columns / places.
+  const int64_t most = T / kLeastPart < places / columns ? T / kLeastPart : places / columns;
+  c.places = static_cast<int>(2 * most);
+  if (max_rows <= c.size) c.size = (max_rows + kChunk - 1) / kChunk * kChunk;
+  return c;
+}
+
+int64_t sum_bytes(const Cut& c, int heads, int dk, int dv) { return 4 * static_cast<int64_t>(c.places) * heads * dk * dv; }
+
+template <int DK, int TW, int TEAMS, bool OUT>
+int launch_chunks(ChunkArgs a, int64_t numbers, hipStream_t s) {
+  using L = ChunkTiles<DK, TW, TEAMS>;
+  constexpr int kLds = OUT ? L::kBytes : L::kSumBytes;
+  a.numbers = numbers;
+  const int64_t groups = (numbers * a.l.k_heads + 7) / 8 * 8 * a.across;
+  if (groups * L::kThreads > kMaxGridThreads) return kInvalid;
+  const auto kernel = linear_chunk_kernel<DK, TW, TEAMS, OUT>;
+  allow_lds(reinterpret_cast<const void*>(kernel), kLds);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(L::kThreads), kLds, s, a);
+  return status_of(hipGetLastError());
+}
+
+template <int DK, int TW, int TEAMS>
+int chunks_of(const ChunkArgs& a, hipStream_t s) {
+  const MixBatch& b = a.l.b;
+  if (!a.single) {
+    const int64_t places = 2 * static_cast<int64_t>(b.T / a.size);
+    if (int st = launch_chunks<DK, TW, TEAMS, false>(a, places, s)) return st;
+    const int64_t fours = static_cast<int64_t>(a.l.heads) * a.l.dk * a.l.dv / 4, groups = (fours + 255) / 256 * (places / 2);
+    if (groups * 256 > kMaxGridThreads) return kInvalid;
+    hipLaunchKernelGGL(linear_parts_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, a);
+    if (int st = status_of(hipGetLastError())) return st;
+  }
+  return launch_chunks<DK, TW, TEAMS, true>(a, mix_piece_count(b, MixPieces{a.size, a.single}), s);
+}
+
+template <int DK>
+int chunks_by(const ChunkArgs& a, const Cut& c, hipStream_t s) {
+  return c.waves == 4 ? chunks_of<DK, 4, 1>(a, s) : c.teams == 2 ? chunks_of<DK, 2, 2>(a, s) : chunks_of<DK, 2, 1>(a, s);
+}
+
+int chunks(const LinearArgs& p, void* workspace, hipStream_t s) {
+  const Cut c = cut_of(p.b.T, p.b.max_rows, p.heads, p.k_heads, p.dk, p.dv);
+  ChunkArgs a{};
+  a.l = p, a.size = c.size, a.single = mix_pieces(p.b, c.size).single, a.across = c.across;
+  if (!a.single) {
+    if (!workspace) return kInvalid;
+    a.sums = static_cast<float*>(workspace);
+    a.logs = reinterpret_cast<double*>(static_cast<char*>(workspace) + sum_bytes(c, p.heads, p.dk, p.dv));
+  }
+  return p.dk <= 64 ? chunks_by<64>(a, c, s) : p.dk <= 128 ? chunks_by<128>(a, c, s) : chunks_by<256>(a, c, s);
+}
+
 bool sizes_known(int T, int heads, int k_heads, int dk, int dv) {
   return T >= 0 && T < (1 << 30) && k_heads >= 1 && heads >= k_heads && heads <= kMaxHeads && heads % k_heads == 0 && dk >= 8 && dk <= kMaxDk &&
          dk % 8 == 0 && dv >= 8 && dv <= kMaxDv && dv % 8 == 0;
@@ -37,7 +111,8 @@ extern "C" {
 
 int64_t lx_linear_attention_workspace_bytes(const lx_kv8_batch* batch, int T, int heads, int k_heads, int dk, int dv) {
   if (!batch || !sizes_known(T, heads, k_heads, dk, dv)) return -1;
-  return 0;
+  const Cut c = cut_of(T, T, heads, k_heads, dk, dv);
+  return sum_bytes(c, heads, dk, dv) + 8 * static_cast<int64_t>(c.places) * heads;
 }
 
 int lx_linear_attention(const void* q, const void* k, const void* v, lx_dtype dtype, int ld_q, int ld_k, int ld_v, const lx_decay* decay,
@@ -71,8 +146,8 @@ int lx_linear_attention(const void* q, const void* k, const void* v, lx_dtype dt
   p.b = mix_batch(*batch, T);
   p.states = mix_states(states);
   if (p.b.max_rows == 0 || p.b.seqs == 0) return kOk;
-  if (int st = steps(p, as_stream(stream))) return fail(st);
-  return kOk;
+  const int st = p.b.max_rows <= kMostSteps ? steps(p, as_stream(stream)) : chunks(p, workspace, as_stream(stream));
+  return st ? fail(st) : kOk;
 }
 
 }  // extern "C"

@@ -68,26 +68,19 @@ __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 4) linear_step_kernel(co
     const float now = log;
     if (i + 1 < span.stop) ask(i + 1);
     f32x4 o = {};
-    auto step = [&](auto fade) __attribute__((always_inline)) {
+    // e^g in two parts: rounded, near 1, it is off to the same side token after token (after 4096 tokens of a memory as long, 3e-4 were
+    // missing).
+    const float less = expm1f(now), slow = 1.0f + less, fade = now > -0.5f ? slow : expf(now), left = now > -0.5f ? less - (slow - 1.0f) : 0.0f;
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        const uint32_t two_k = ks[r / 8][r % 8 / 2], two_q = qs[r / 8][r % 8 / 2];
-        const float k = __uint_as_float(r % 2 ? two_k & 0xffff0000u : two_k << 16), q = __uint_as_float(r % 2 ? two_q & 0xffff0000u : two_q << 16);
+    for (int r = 0; r < ROWS; ++r) {
+      const uint32_t two_k = ks[r / 8][r % 8 / 2], two_q = qs[r / 8][r % 8 / 2];
+      const float k = __uint_as_float(r % 2 ? two_k & 0xffff0000u : two_k << 16), q = __uint_as_float(r % 2 ? two_q & 0xffff0000u : two_q << 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          state[r][j] = __builtin_fmaf(k, v[j], fade(state[r][j]));
-          o[j] = __builtin_fmaf(q, state[r][j], o[j]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        state[r][j] = __builtin_fmaf(state[r][j], fade, __builtin_fmaf(state[r][j], left, k * v[j]));
+        o[j] = __builtin_fmaf(q, state[r][j], o[j]);
       }
-    };
-    // Slow decays by what is lost: e^g near 1 is rounded to the same side token after token (after 4096 tokens of a memory as long 3e-4
-    // were missing), e^g - 1 is not.
-    if (__builtin_amdgcn_readfirstlane(now > -0.5f)) {
-      const float less = expm1f(now);
-      step([&](float x) { return __builtin_fmaf(x, less, x); });
-    } else {
-      const float fade = expf(now);
-      step([&](float x) { return x * fade; });
+      if (r % 2) __builtin_amdgcn_sched_barrier(0);  // left alone, products of all rows are made before the first sum, in registers that are not there
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -49,30 +49,46 @@ struct MixPieces {
 inline MixPieces mix_pieces(const MixBatch& b, int size) { return {size, !b.rows || b.max_rows <= size}; }
 inline int64_t mix_piece_count(const MixBatch& b, const MixPieces& p) { return p.single ? b.seqs : static_cast<int64_t>(b.T) / p.size + b.seqs; }
 
-// The sequence and the number in it of piece w, as every wavefront finds them for itself: the last sequence whose first piece is not behind
-// w, 64 candidates at a time. False where there is none.
+// The last sequence whose number is not behind w, as every wavefront finds it for itself, 64 candidates at a time; -1 where there is none. Numbers
+// ascend.
+template <typename Number>
+__device__ __forceinline__ int mix_last(int seqs, int64_t w, Number number) {
+  const int lane = threadIdx.x % kWave;
+  int low = 0, count = seqs;
+  while (true) {
+    const int step = (count + kWave - 1) / kWave, at = lane * step;
+    const bool here = at < count && number(low + (at < count ? at : 0)) <= w;
+    const uint64_t set = __ballot(here);
+    if (!set) return -1;
+    const int last = (kWave - 1 - __builtin_clzll(set)) * step;
+    low += last;
+    count = count - last < step ? count - last : step;
+    if (count <= 1) return __builtin_amdgcn_readfirstlane(low);
+  }
+}
+
+// The sequence of piece w and the piece's number in it; false where there is none.
 __device__ __forceinline__ bool mix_find(const MixBatch& b, const MixPieces& p, int64_t w, int& s, int& j) {
   if (p.single) {
     s = static_cast<int>(w), j = 0;
     return w < b.seqs;
   }
-  const int lane = threadIdx.x % kWave;
   auto number = [&](int i) { return static_cast<int64_t>(mix_clamp(b.rows[i], 0, b.T) / p.size) + i; };
-  int low = 0, count = b.seqs;
-  while (true) {
-    const int step = (count + kWave - 1) / kWave, at = lane * step;
-    const bool here = at < count && number(low + (at < count ? at : 0)) <= w;
-    const uint64_t set = __ballot(here);
-    if (!set) return false;
-    const int last = (kWave - 1 - __builtin_clzll(set)) * step;
-    low += last;
-    count = count - last < step ? count - last : step;
-    if (count <= 1) break;
-  }
-  s = __builtin_amdgcn_readfirstlane(low);
-  const int64_t of = w - number(s);
+  s = mix_last(b.seqs, w, number);
+  const int64_t of = s < 0 ? w : w - number(s);
   j = static_cast<int>(of);
-  return of < (1 << 30);
+  return s >= 0 && of <= b.T / p.size;
+}
+
+// The same among the sequences of more than one piece alone, which start more than `size` rows apart: piece j of sequence s is number
+// 2 (rows[s] / size) + j, which a sequence of n > size rows, (rows[s] + n) / size - rows[s] / size >= 1 whole sizes apart from the next one, does not
+// exceed, and all of them are fewer than 2 (T / size). The last sequence that starts in a size is the one, if any is.
+__device__ __forceinline__ bool mix_find_long(const MixBatch& b, int size, int64_t w, int& s, int& j) {
+  auto number = [&](int i) { return 2 * static_cast<int64_t>(mix_clamp(b.rows[i], 0, b.T) / size); };
+  s = mix_last(b.seqs, w, number);
+  const int64_t of = s < 0 ? w : w - number(s);
+  j = static_cast<int>(of);
+  return s >= 0 && of <= b.T / size;
 }
 
 struct MixStates {
@@ -86,6 +102,15 @@ struct MixStates {
 __device__ __forceinline__ int mix_slot(const MixStates& t, int s) {
   const int slot = t.slots ? t.slots[s] : s;
   return slot >= 0 && slot < t.count ? slot : -1;
+}
+
+// v / (1 + exp(-v)), right to 2^-21: the exponent's product in two parts, one reciprocal in place of a division.
+__device__ __forceinline__ float quick_silu(float v) {
+  const float x = -fmaxf(v, -87.0f), t = x * 1.44269502f;
+  const float rest = __builtin_fmaf(x, 1.44269502f, -t);  // what t's rounding left, exactly
+  float e = __builtin_amdgcn_exp2f(t);
+  e = __builtin_fmaf(e, __builtin_fmaf(x, 1.334976e-8f, rest * 0.693147181f), e);  // log2(e) - 1.44269502 is 1.92596e-8
+  return v * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
 inline bool mix_type(lx_dtype t) { return t == LX_F32 || t == LX_BF16; }

@@ -41,18 +41,8 @@ __device__ __forceinline__ bool position_of(const RotateArgs& p, int t, int& pos
     s = t;
     if (s >= p.b.seqs) return false;
   } else {
-    const int lane = threadIdx.x % kWave;
-    int low = 0, count = p.b.seqs;
-    while (true) {
-      const int step = (count + kWave - 1) / kWave, at = lane * step;
-      const uint64_t set = __ballot(at < count && p.b.rows[low + (at < count ? at : 0)] <= t);
-      if (!set) return false;
-      const int last = (kWave - 1 - __builtin_clzll(set)) * step;
-      low += last;
-      count = count - last < step ? count - last : step;
-      if (count <= 1) break;
-    }
-    s = low;
+    s = mix_last(p.b.seqs, t, [&](int i) { return p.b.rows[i]; });
+    if (s < 0) return false;
   }
   const MixSpan span = mix_span(p.b, s);
   j = t - span.row0;

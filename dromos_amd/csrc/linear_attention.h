@@ -1,4 +1,4 @@
-// The arguments of lx_linear_attention's kernels, and what they share: the decay of a token and the epilogue of an output.
+// The arguments of lx_linear_attention's kernels, and what they share: the decay of a token.
 #pragma once
 
 #include "mixer.h"
@@ -45,22 +45,6 @@ __device__ __forceinline__ void decay_of(const LinearArgs& p, int64_t row, int h
     }
   }
   log = log < kForgotten ? kForgotten : log;
-}
-
-// Four outputs of a row from the state's part: skip, gate, store.
-__device__ __forceinline__ void finish_four(const LinearArgs& p, int64_t row, int head, int column, f32x4 o, float skip) {
-  const int64_t at = static_cast<int64_t>(head) * p.dv + column;
-  if (p.skip) {
-    const f32x4 v = load_four(p.v, p.type, p.wide, row * p.ld_v + at);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(skip, p.type == LX_BF16 ? v[j] : bf16_bits_to_f32(f32_to_bf16_bits(v[j])), o[j]);
-  }
-  if (p.gate) {
-    const f32x4 z = load_four(p.gate, p.gate_type, p.wide, row * p.ld_gate + at);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] *= quick_silu(z[j]);
-  }
-  store_four(p.out, p.out_type, p.wide, row * p.ld_out + at, o);
 }
 
 }  // namespace dro

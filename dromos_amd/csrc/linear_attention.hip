@@ -13,7 +13,8 @@ int launch_step(const LinearArgs& p, hipStream_t s) {
   const int64_t waves = static_cast<int64_t>(p.b.seqs) * p.heads * ((p.dv + 4 * COLS - 1) / (4 * COLS));
   const int64_t groups = (waves + 3) / 4;
   if (groups * 256 > kMaxGridThreads) return kInvalid;
-  hipLaunchKernelGGL((linear_step_kernel<COLS, ROWS>), dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, p);
+  const auto kernel = p.type == LX_BF16 && p.wide && (!p.gate || p.gate_type == LX_BF16) ? linear_step_kernel<COLS, ROWS, true> : linear_step_kernel<COLS, ROWS, false>;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, p);
   return status_of(hipGetLastError());
 }
 

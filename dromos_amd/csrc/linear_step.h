@@ -6,79 +6,113 @@
 // 64 / COLS parts of the rows. The columns' sums over the rows cross the lanes once a token.
 #pragma once
 
+#include <type_traits>
+
 #include "linear_attention.h"
 
 namespace dro {
 
-// COLS lanes side by side in a row of the state; ROWS rows of it a lane.
-template <int COLS, int ROWS>
-__global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 4) linear_step_kernel(const LinearArgs p) {
+// COLS lanes side by side in a row of the state; ROWS rows of it a lane. PLAIN: queries, keys, values and gates bf16 that can be moved 16 bytes at
+// a time (everything else in its own kernel: the registers of its loads would be missing here).
+template <int COLS, int ROWS, bool PLAIN>
+__global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 3) linear_step_kernel(const LinearArgs p) {
   static_assert(COLS == 4 || COLS == 8, "lanes of a row");
   static_assert(ROWS % 8 == 0, "keys are read eight at a time");
   const int lane = threadIdx.x % kWave;
-  const int blocks = (p.dv + 4 * COLS - 1) / (4 * COLS);
-  const int64_t wave = static_cast<int64_t>(blockIdx.x) * (blockDim.x / kWave) + threadIdx.x / kWave;
-  const int64_t unit = wave / blocks;
-  const int s = static_cast<int>(unit / p.heads), head = static_cast<int>(unit % p.heads);
+  const unsigned blocks = (p.dv + 4 * COLS - 1) / (4 * COLS);
+  const unsigned wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), unit = wave / blocks;
+  const int s = unit / p.heads, head = unit % p.heads;
   if (s >= p.b.seqs) return;
   const MixSpan span = mix_span(p.b, s);
   if (span.first >= span.stop) return;
-  const int column = static_cast<int>(wave % blocks) * (4 * COLS) + lane % COLS * 4;
+  const int column = wave % blocks * (4 * COLS) + lane % COLS * 4;
   const int row0 = lane / COLS * ROWS;  // of the state
   const bool mine = column < p.dv;
-  const int slot = mix_slot(p.states, s);
-  const int64_t size = static_cast<int64_t>(p.dk) * p.dv;
-  const int64_t at = (static_cast<int64_t>(slot) * p.heads + head) * size + static_cast<int64_t>(row0) * p.dv + column;
+  const int slot = __builtin_amdgcn_readfirstlane(mix_slot(p.states, s));
+  const int64_t size = static_cast<int64_t>(p.dk) * p.dv, base = (static_cast<int64_t>(slot) * p.heads + head) * size;
+  const unsigned from = static_cast<unsigned>(row0 * p.dv + column);  // rows are told apart by what all lanes share
 
   f32x4 state[ROWS];
   const bool reads = p.states.in && slot >= 0 && !span.begins && mine;
 #pragma unroll
-  for (int i = 0; i < ROWS; i += 8)
+  for (int i = 0; i < ROWS; i += 8) {
+    const float* const rows = static_cast<const float*>(p.states.in) + base + static_cast<int64_t>(i) * p.dv;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      state[i + j] = reads && row0 + i < p.dk ? *reinterpret_cast<const f32x4*>(static_cast<const float*>(p.states.in) + at + static_cast<int64_t>(i + j) * p.dv) : f32x4{};
-
-  const int k_head = head / p.group;
-  const float skip = p.skip ? p.skip[head] : 0.0f;
-  u32x4 key[ROWS / 8], query[ROWS / 8];
-  f32x4 value;
-  float log, weight;
-  auto ask = [&](int i) {
-    const int64_t row = span.row0 + i;
-    const int64_t k_at = static_cast<int64_t>(k_head) * p.dk + row0;
+    for (int j = 0; j < 8; ++j) state[i + j] = f32x4{};
+    if (reads && row0 + i < p.dk) {
 #pragma unroll
-    for (int r = 0; r < ROWS / 8; ++r) {
-      const bool in = row0 + 8 * r < p.dk;
-      key[r] = in ? load_eight_bf16(p.k, p.type, p.wide, row * p.ld_k + k_at + 8 * r) : u32x4{};
-      query[r] = in ? load_eight_bf16(p.q, p.type, p.wide, row * p.ld_q + k_at + 8 * r) : u32x4{};
+      for (int j = 0; j < 8; ++j) state[i + j] = *reinterpret_cast<const f32x4*>(rows + static_cast<int64_t>(j) * p.dv + from);
     }
-    value = mine ? load_four(p.v, p.type, p.wide, row * p.ld_v + static_cast<int64_t>(head) * p.dv + column) : f32x4{};
-    if (p.type != LX_BF16) {
+  }
+
+  const int k_head = head / p.group, rows = span.stop - span.first;
+  const int64_t first = static_cast<int64_t>(span.row0) + span.first, k_at = static_cast<int64_t>(k_head) * p.dk + row0, v_at = static_cast<int64_t>(head) * p.dv + column;
+  // What a token brings, one token ahead on its way. The gate too: asked for at an output's end, each token would wait for it.
+  // Numbers are made of it where they are used: here they would be waited for.
+  u32x4 key[ROWS / 8], query[ROWS / 8];
+  using Four = std::conditional_t<PLAIN, u32x2, f32x4>;
+  Four value, gate = {};
+  auto ask = [&](int i) {
+    const int64_t row = first + i;
+#pragma unroll
+    for (int r = 0; r < ROWS / 8; ++r) {  // places behind the state's last row are read somewhere else, and count nothing
+      const int64_t at = row0 + 8 * r < p.dk ? k_at + 8 * r : static_cast<int64_t>(k_head) * p.dk;
+      key[r] = load_eight_bf16(p.k, PLAIN ? LX_BF16 : p.type, PLAIN || p.wide, row * p.ld_k + at);
+      query[r] = load_eight_bf16(p.q, PLAIN ? LX_BF16 : p.type, PLAIN || p.wide, row * p.ld_q + at);
+    }
+    const int64_t at = mine ? v_at : static_cast<int64_t>(head) * p.dv;
+    if constexpr (PLAIN) {
+      value = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p.v) + row * p.ld_v + at);
+      if (p.gate) gate = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p.gate) + row * p.ld_gate + at);
+    } else {
+      value = load_four(p.v, p.type, p.wide, row * p.ld_v + at);
+      if (p.gate) gate = load_four(p.gate, p.gate_type, p.wide, row * p.ld_gate + at);
 #pragma unroll
       for (int j = 0; j < 4; ++j) value[j] = bf16_bits_to_f32(f32_to_bf16_bits(value[j]));
     }
-    decay_of(p, row, head, log, weight);
   };
-  ask(span.first);
-  for (int i = span.first; i < span.stop; ++i) {
+  auto four_of = [](const Four& x) {
+    if constexpr (PLAIN) {
+      const uint32_t a = x.x, b = x.y;
+      return f32x4{__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)};
+    } else {
+      return x;
+    }
+  };
+  ask(0);
+
+  // The decays, a token a lane. e^g in two parts: rounded, near 1, it is off to the same side token after token (after 4096 tokens of a
+  // memory as long, 3e-4 were missing).
+  const float skip = p.skip ? p.skip[head] : 0.0f;
+  float fades, lefts, weights = 1.0f;
+  {
+    float log = 0.0f;
+    if (lane < rows) decay_of(p, first + lane, head, log, weights);
+    const float less = expm1f(log), slow = 1.0f + less;
+    fades = log > -0.5f ? slow : expf(log), lefts = log > -0.5f ? less - (slow - 1.0f) : 0.0f;
+  }
+  auto of_token = [&](float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); };
+
+  for (int i = 0; i < rows; ++i) {
     u32x4 ks[ROWS / 8], qs[ROWS / 8];
 #pragma unroll
-    for (int r = 0; r < ROWS / 8; ++r) ks[r] = key[r], qs[r] = query[r];
-    const f32x4 v = value * weight;
-    const float now = log;
-    if (i + 1 < span.stop) ask(i + 1);
+    for (int r = 0; r < ROWS / 8; ++r) ks[r] = row0 + 8 * r < p.dk ? key[r] : u32x4{}, qs[r] = row0 + 8 * r < p.dk ? query[r] : u32x4{};
+    const float fade = of_token(fades, i), left = of_token(lefts, i), weight = of_token(weights, i);
+    const f32x4 raw = four_of(value), z = four_of(gate), v = raw * weight;
+    if (i + 1 < rows) ask(i + 1);
     f32x4 o = {};
-    // e^g in two parts: rounded, near 1, it is off to the same side token after token (after 4096 tokens of a memory as long, 3e-4 were
-    // missing).
-    const float less = expm1f(now), slow = 1.0f + less, fade = now > -0.5f ? slow : expf(now), left = now > -0.5f ? less - (slow - 1.0f) : 0.0f;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const uint32_t two_k = ks[r / 8][r % 8 / 2], two_q = qs[r / 8][r % 8 / 2];
       const float k = __uint_as_float(r % 2 ? two_k & 0xffff0000u : two_k << 16), q = __uint_as_float(r % 2 ? two_q & 0xffff0000u : two_q << 16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        state[r][j] = __builtin_fmaf(state[r][j], fade, __builtin_fmaf(state[r][j], left, k * v[j]));
-        o[j] = __builtin_fmaf(q, state[r][j], o[j]);
+        // In place: the compiler would make the new state in registers of its own.
+        const float add = __builtin_fmaf(state[r][j], left, k * v[j]);
+        float in = state[r][j];
+        asm("v_fma_f32 %0, %0, %1, %2" : "+v"(in) : "s"(fade), "v"(add));
+        state[r][j] = in;
+        o[j] = __builtin_fmaf(q, in, o[j]);
       }
       if (r % 2) __builtin_amdgcn_sched_barrier(0);  // left alone, products of all rows are made before the first sum, in registers that are not there
     }
@@ -92,15 +126,24 @@ __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 4) linear_step_kernel(co
       swap_halves<false>(half, a, b);
       o[j] = (a + b) * p.scale;
     }
-    if (mine && lane < COLS) finish_four(p, span.row0 + i, head, column, o, skip);
+    if (mine && lane < COLS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[j] = __builtin_fmaf(skip, raw[j], o[j]);
+        if (p.gate) o[j] *= quick_silu(z[j]);
+      }
+      store_four(p.out, p.out_type, p.wide, (first + i) * p.ld_out + v_at, o);
+    }
   }
   if (!p.states.out || slot < 0 || !mine) return;
 #pragma unroll
-  for (int i = 0; i < ROWS; i += 8)
+  for (int i = 0; i < ROWS; i += 8) {
+    float* const rows = static_cast<float*>(p.states.out) + base + static_cast<int64_t>(i) * p.dv;
     if (row0 + i < p.dk) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) *reinterpret_cast<f32x4*>(static_cast<float*>(p.states.out) + at + static_cast<int64_t>(i + j) * p.dv) = state[i + j];
+      for (int j = 0; j < 8; ++j) *reinterpret_cast<f32x4*>(rows + static_cast<int64_t>(j) * p.dv + from) = state[i + j];
     }
+  }
 }
 
 }  // namespace dro

@@ -6,6 +6,7 @@ namespace dro {
 namespace {
 
 constexpr int kMaxDk = 256, kMaxDv = 512, kMaxHeads = 4096;
+constexpr int kMaxStride = 1 << 24;  // values: rows of a chunk are told apart in 32 bits
 constexpr int kMostSteps = 16;  // rows of a sequence that go token by token
 
 template <int COLS, int ROWS>
@@ -61,7 +62,8 @@ int launch_chunks(ChunkArgs a, int64_t numbers, hipStream_t s) {
   a.numbers = numbers;
   const int64_t groups = (numbers * a.l.k_heads + 7) / 8 * 8 * a.across;
   if (groups * L::kThreads > kMaxGridThreads) return kInvalid;
-  const auto kernel = linear_chunk_kernel<DK, TW, TEAMS, OUT>;
+  const bool plain = a.l.type == LX_BF16 && a.l.wide && (!a.l.gate || a.l.gate_type == LX_BF16) && positive(a.l.scale);
+  const auto kernel = plain ? linear_chunk_kernel<DK, TW, TEAMS, OUT, true> : linear_chunk_kernel<DK, TW, TEAMS, OUT, false>;
   allow_lds(reinterpret_cast<const void*>(kernel), kLds);
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(L::kThreads), kLds, s, a);
   return status_of(hipGetLastError());
@@ -134,6 +136,7 @@ int lx_linear_attention(const void* q, const void* k, const void* v, lx_dtype dt
   const int64_t keys = static_cast<int64_t>(k_heads) * dk, values = static_cast<int64_t>(heads) * dv;
   if (T > 1 && (ld_q < keys || ld_k < keys || ld_v < values || ld_out < values || (gate && ld_gate < values) || (by_token && decay->ld < heads)))
     return fail(kInvalid);
+  if (T > 1 && (ld_q > kMaxStride || ld_k > kMaxStride || ld_v > kMaxStride || ld_out > kMaxStride || (gate && ld_gate > kMaxStride))) return fail(kInvalid);
   LinearArgs p{};
   p.q = q, p.k = k, p.v = v, p.x = by_token ? decay->x : nullptr, p.rate = decay->rate;
   p.bias = decay->kind == LX_DECAY_STEP ? decay->bias : nullptr;

@@ -3,7 +3,7 @@
 // With G_i the sum of the decays' logarithms of a chunk up to token i, b_j the weight of an update and S the state in front of the chunk
 //   out_i = scale (e^{G_i} S^T q_i + sum_{j <= i} (q_i . k_j) e^{G_i - G_j} b_j v_j)
 //   S    <- e^{G_63} S + sum_j k_j (e^{G_63 - G_j} b_j v_j)^T
-// Every exponent is a difference of sums at most 0, formed from sums in 64 bits (as two f32): nothing overflows, and near tokens lose nothing where the sums
+// Every exponent is a difference of sums at most 0, formed from sums in 64 bits (as two f32 each): nothing overflows, and near tokens lose nothing where the sums
 // are large. What is rounded to go into a product (weights, scaled values, the state) goes in as two bf16, a value and what its
 // rounding left: with one, a state would be right to 2^-9 only, and results carry its error on from chunk to chunk.
 //
@@ -22,6 +22,8 @@
 // only), a second one runs through them and leaves the state in front of every part, and this one starts from there.
 #pragma once
 
+#include <type_traits>
+
 #include "linear_attention.h"
 
 namespace dro {
@@ -38,7 +40,7 @@ struct ChunkArgs {
   int64_t numbers;  // of parts that the launch counts to
   int across;       // workgroups of a part and key head
   float* sums;      // [2 (T / size)] states [heads, dk, dv]: parts' sums, then the states in front of them
-  double* logs;     // [2 (T / size), heads] logarithms (base 2) of what the parts leave of what was in front of them
+  double* logs;     // [2 (T / size), heads] logarithms of what the parts leave of what was in front of them
 };
 
 // Where 16-byte unit `unit` of row `row` lies in a tile of rows of `kPitch` bytes (128, 256 or 512): its place in the row is turned by the row's low bits, so
@@ -61,15 +63,18 @@ __device__ __forceinline__ int tile_place(int from, int row, int unit) {
 __device__ __forceinline__ bf16x8 eight_at(const uint8_t* lds, int at) { return *reinterpret_cast<const bf16x8*>(lds + at); }
 
 // The operand of rows across a tile: eight rows 16 s + 8 h .. + 7 of 32 columns, in the order (0-3, 8-11, 4-7, 12-15) of every 16. A lane asks for four
-// neighbouring columns of a row and gets four rows of a column; here is where its four lie, of columns 0 .. 31 and s = 0, for
-// either half of the eight rows.
+// neighbouring columns of a row and gets four rows of a column; here is where its four lie, of columns 0 .. 31 and s = 0, for the first four of
+// the eight rows.
 template <int kPitch>
-__device__ __forceinline__ int across_place(int column, int half) {
+__device__ __forceinline__ int across_place(int column) {
   const int lane = threadIdx.x % kWave, m = lane % 16, h = lane / 32;
   const int from = column + lane / 16 % 2 * 16 + (m % 2 * 8 | m % 4 / 2 * 4);
-  return tile_place<kPitch>(8 * h + 4 * half + m / 4, from / 8) + from % 8 * 2;
+  return tile_place<kPitch>(8 * h + m / 4, from / 8) + from % 8 * 2;
 }
-__device__ __forceinline__ bf16x8 across(const uint8_t* lds, int at0, int at1) {
+// The operand of tile `at` (a whole 256 bytes), from that place, of rows 16 s .. and columns 8 unit .. further.
+template <int kPitch>
+__device__ __forceinline__ bf16x8 across(const uint8_t* lds, int at, int from, int s, int unit) {
+  const int at0 = at + tile_place<kPitch>(from, 16 * s, unit), at1 = at + tile_place<kPitch>(from, 16 * s + 4, unit);
   union {
     s16x4 half[2];
     bf16x8 whole;
@@ -92,41 +97,42 @@ __device__ __forceinline__ void split_eight(const float (&v)[8], bf16x8& high, b
   low = __builtin_bit_cast(bf16x8, b);
 }
 
-// A sum over the wavefront's lanes up to and with each one, in 64 bits.
+// A sum over the wavefront's lanes up to and with each one, of 64-bit integers.
 template <int CTRL, int ROWS>
-__device__ __forceinline__ double scan_step(double v) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROWS, 0xf, true);
-  const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROWS, 0xf, true);
-  return v + __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | low);
+__device__ __forceinline__ int64_t scan_step(int64_t v) {
+  const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, true);
+  const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, true);
+  return v + static_cast<int64_t>(static_cast<uint64_t>(high) << 32 | low);
 }
-__device__ __forceinline__ double wave_scan(double v) {
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {
   v = scan_step<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
   v = scan_step<0x112, 0xf>(v);
   v = scan_step<0x114, 0xf>(v);
   v = scan_step<0x118, 0xf>(v);
-  v = scan_step<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v = scan_step<0x142, 0xa>(v);     // row_bcast:15 into rows 1 and 3
   return scan_step<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
 }
 
-// What of a state is left by a decay: x e^log, or x + x (e^log - 1) where little fades, whose rounding does not go to one side.
+// e^log in two parts: rounded, near 1, it is off to the same side time after time.
 struct Fade {
-  float factor;
-  bool slow;
+  float high, low;
 };
-__device__ __forceinline__ Fade fade_of(double log2_of) {
-  const float log = static_cast<float>(log2_of * 0.69314718055994530942);
-  const bool slow = log > -0.5f;
-  return {slow ? expm1f(log) : expf(log), slow};
+__device__ __forceinline__ Fade fade_of(float log) {
+  const float less = quick_expm1(log), high = 1.0f + less;
+  return log > -0.5f ? Fade{high, less - (high - 1.0f)} : Fade{quick_exp(log), 0.0f};
 }
 
-// The numbers of a chunk's tokens.
+// The numbers of a chunk's tokens. G_i (base 2) is a sum of integers, 2^-40 each, and so exact: `high` its whole 256ths and a rest. Logarithms of
+// -200 at least keep 64 of them within the 24 bits of `high`.
 struct Tokens {
-  float g_high[kChunk], g_low[kChunk];  // G_i, base 2
-  float h_high[kChunk], h_low[kChunk];  // G_j - log2(b_j)
-  float update[kChunk];                 // e^{G_63 - G_j} b_j
-  float seen[kChunk];                   // e^{G_i}
-  double whole, none;                   // G_63; whole 16 bytes
+  float high[kChunk];
+  float row[kChunk];     // the rest of G_i + log(scale)
+  float column[kChunk];  // the rest of G_j - log(b_j)
+  float update[kChunk];  // e^{G_63 - G_j} b_j
+  float seen[kChunk];    // scale e^{G_i}
+  float fade;            // e^{G_63}, and what its rounding left of the chunks before
+  float whole;           // the logarithm of e^{G_63}
+  float none[2];         // whole 16 bytes
 };
 
 template <int DK, int TW, int TEAMS>
@@ -138,24 +144,29 @@ struct ChunkTiles {
   static constexpr int kBlock = 32 * 64;             // a 32 x 32 tile of weights, bf16
   static constexpr int kWeightBytes = 2 * 3 * kBlock;  // of a head: tiles (0, 0), (0, 1), (1, 1) as values, then what their rounding left
   static constexpr int kKeys = 0, kValues = kKeys + kKeyBytes, kTokens = kValues + kValueBytes;
-  static constexpr int kQueries = kTokens + 2 * TEAMS * static_cast<int>(sizeof(Tokens)), kWeights = kQueries + kKeyBytes;
+  // Places in a tile are made by exclusive ors: it begins at a whole 256 bytes.
+  static constexpr int kQueries = kTokens + (2 * TEAMS * static_cast<int>(sizeof(Tokens)) + 255) / 256 * 256, kWeights = kQueries + kKeyBytes;
   static constexpr int kSumBytes = kQueries, kBytes = kWeights + TEAMS * kWeightBytes;
 };
 
-// OUT: outputs and states; otherwise a part's sum of a long sequence only.
-template <int DK, int TW, int TEAMS, bool OUT>
-__global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 ? 1 : 2) linear_chunk_kernel(const ChunkArgs c) {
+// A scale that can be part of an exponent.
+__host__ __device__ __forceinline__ bool positive(float scale) { return scale > 1e-30f && scale < 1e30f; }
+
+// OUT: outputs and states; otherwise a part's sum of a long sequence only. PLAIN: bf16 that can be moved 16 bytes at a time, a positive scale, gates bf16 or
+// none (everything else in its own kernel: its loads and stores, a value at a time perhaps, would cost this one registers).
+template <int DK, int TW, int TEAMS, bool OUT, bool PLAIN>
+__global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 && TW * TEAMS == 2) ? 1 : 2) linear_chunk_kernel(const ChunkArgs c) {
   using L = ChunkTiles<DK, TW, TEAMS>;
   extern __shared__ __attribute__((aligned(256))) uint8_t lds[];
   const LinearArgs& p = c.l;
   // Workgroups that read the same keys follow one another on one die.
-  const int64_t turn = blockIdx.x / 8, unit = turn / c.across * 8 + blockIdx.x % 8;
-  const int beside = static_cast<int>(turn % c.across), k_head = static_cast<int>(unit % p.k_heads);
-  const int64_t number = unit / p.k_heads;
+  const unsigned turn = blockIdx.x / 8, unit = turn / c.across * 8 + blockIdx.x % 8, number = unit / p.k_heads;
+  const int beside = turn % c.across, k_head = unit % p.k_heads;
   if (number >= c.numbers) return;
   int s, j;
   if (OUT ? !mix_find(p.b, MixPieces{c.size, c.single}, number, s, j) : !mix_find_long(p.b, c.size, number, s, j)) return;
   MixSpan span = mix_span(p.b, s);
+  const int slot = __builtin_amdgcn_readfirstlane(mix_slot(p.states, s));
   span.row0 = __builtin_amdgcn_readfirstlane(span.row0), span.first = __builtin_amdgcn_readfirstlane(span.first);
   span.stop = __builtin_amdgcn_readfirstlane(span.stop), span.begins = __builtin_amdgcn_readfirstlane(span.begins);
   const int begin = max(span.first, j * c.size), end = min(span.stop, (j + 1) * c.size);
@@ -173,111 +184,114 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 ? 1 : 2) linear_
   const int head = min(head0 + team, head_end - 1);
   const bool idle = head0 + team >= head_end;
   const int column = column0 + 32 * mate + (n / 16 * 16 + (n % 4 | n / 4 % 2 * 8 | n / 8 % 2 * 4));  // the lane's of the state
-  const int64_t first_row = span.row0 + begin;
+  const int64_t first_row = static_cast<int64_t>(span.row0) + begin;
   const int rows = end - begin, chunks = (rows + kChunk - 1) / kChunk;
-
-  Tokens* const tokens = reinterpret_cast<Tokens*>(lds + L::kTokens) + 2 * team;
-  // Where the lane's first reads lie: row n of the keys (and queries), the columns of the keys and of its values, row n of its values and of the weights.
-  const int key_row = tile_place<L::kKeyPitch>(n, h);
-  const int key_column[2] = {across_place<L::kKeyPitch>(0, 0), across_place<L::kKeyPitch>(0, 1)};
-  const int value_column[2] = {L::kValues + across_place<L::kValuePitch>(32 * wave, 0), L::kValues + across_place<L::kValuePitch>(32 * wave, 1)};
-  const int value_row = tile_place<L::kValuePitch>(n, 4 * wave + h);
-  const int weight_row = team * L::kWeightBytes + 64 * n + 16 * (n >> 2 & 3);
-  auto read_keys = [&](int row, int k) { return eight_at(lds, L::kKeys + tile_place<L::kKeyPitch>(key_row, row, 2 * k)); };
-  auto read_queries = [&](int row, int k) { return eight_at(lds, L::kQueries + tile_place<L::kKeyPitch>(key_row, row, 2 * k)); };
-  auto keys_across = [&](int x, int k) {  // keys' values 32 x .. of tokens 16 k ..
-    return across(lds, L::kKeys + tile_place<L::kKeyPitch>(key_column[0], 16 * k, 4 * x), L::kKeys + tile_place<L::kKeyPitch>(key_column[1], 16 * k, 4 * x));
-  };
-  auto values_across = [&](int k) { return across(lds, value_column[0] + 16 * k * L::kValuePitch, value_column[1] + 16 * k * L::kValuePitch); };
 
   // ---- the next chunk on its way --------------------------------------------------------------------------------------
   constexpr int kKeyLoads = kChunk * DK / 8 / L::kThreads, kValueLoads = kChunk * L::kColumns / 8 / L::kThreads;
   u32x4 next_k[kKeyLoads], next_q[OUT ? kKeyLoads : 1], next_v[kValueLoads];
   const bool whole_tiles = p.dk == DK && head0 + TEAMS <= head_end && column0 + 32 * TW <= p.dv;  // no column is nobody's
-  const bool plain = p.type == LX_BF16 && p.wide && whole_tiles;
   // Where a thread's first loads of a whole chunk lie, from the chunk's first row on; the others follow rows further.
   constexpr int kKeyStep = L::kThreads / (DK / 8), kValueStep = L::kThreads / (L::kColumns / 8);
+  const int my_key_row = threadIdx.x / (DK / 8), my_value_row = threadIdx.x / (L::kColumns / 8);
   const int my_key = threadIdx.x % (DK / 8) * 8, my_value = threadIdx.x % (L::kColumns / 8);
-  const unsigned k_from = static_cast<unsigned>(threadIdx.x / (DK / 8) * p.ld_k + k_head * p.dk + my_key);
-  const unsigned q_from = static_cast<unsigned>(threadIdx.x / (DK / 8) * p.ld_q + k_head * p.dk + my_key);
-  const unsigned v_from = static_cast<unsigned>(threadIdx.x / (L::kColumns / 8) * p.ld_v + (head0 + my_value / (4 * TW)) * p.dv + column0 + my_value % (4 * TW) * 8);
-  auto ask = [&](int chunk) {
+  const int my_head = min(head0 + my_value / (4 * TW), head_end - 1), my_value_at = column0 + my_value % (4 * TW) * 8;
+  const bool my_key_in = my_key < p.dk, my_value_in = my_value_at < p.dv && head0 + my_value / (4 * TW) < head_end;
+  const unsigned k_column = k_head * p.dk + (my_key_in ? my_key : 0), v_column = my_head * p.dv + (my_value_in ? my_value_at : 0);
+  const unsigned k_from = static_cast<unsigned>(my_key_row * p.ld_k) + k_column, q_from = static_cast<unsigned>(my_key_row * p.ld_q) + k_column;
+  const unsigned v_from = static_cast<unsigned>(my_value_row * p.ld_v) + v_column;
+  auto ask = [&](int chunk, bool with_queries, bool with_others) __attribute__((always_inline)) {
     const int64_t row0 = first_row + static_cast<int64_t>(chunk) * kChunk;
     const int last = min(kChunk, rows - chunk * kChunk) - 1;
-    if (plain && last == kChunk - 1) {
-      auto at = [](const void* x, int64_t i, unsigned from) { return *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + i + from); };
+    if (PLAIN && last == kChunk - 1) {
+      const uint16_t* k = static_cast<const uint16_t*>(p.k) + row0 * p.ld_k;
+      const uint16_t* q = static_cast<const uint16_t*>(p.q) + row0 * p.ld_q;
+      const uint16_t* v = static_cast<const uint16_t*>(p.v) + row0 * p.ld_v;
 #pragma unroll
       for (int e = 0; e < kKeyLoads; ++e) {
-        next_k[e] = at(p.k, (row0 + e * kKeyStep) * p.ld_k, k_from);
-        if constexpr (OUT) next_q[e] = at(p.q, (row0 + e * kKeyStep) * p.ld_q, q_from);
-      }
-#pragma unroll
-      for (int e = 0; e < kValueLoads; ++e) next_v[e] = at(p.v, (row0 + e * kValueStep) * p.ld_v, v_from);
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < kKeyLoads; ++e) {
-      const int row = min(static_cast<int>(threadIdx.x) / (DK / 8) + e * kKeyStep, last);
-      const int64_t from = static_cast<int64_t>(k_head) * p.dk + (my_key < p.dk ? my_key : 0);
-      next_k[e] = load_eight_bf16(p.k, p.type, p.wide, (row0 + row) * p.ld_k + from);
-      if constexpr (OUT) next_q[e] = load_eight_bf16(p.q, p.type, p.wide, (row0 + row) * p.ld_q + from);
-    }
-#pragma unroll
-    for (int e = 0; e < kValueLoads; ++e) {
-      const int row = min(static_cast<int>(threadIdx.x) / (L::kColumns / 8) + e * kValueStep, last);
-      const int of = min(head0 + my_value / (4 * TW), head_end - 1), d = column0 + my_value % (4 * TW) * 8;
-      next_v[e] = load_eight_bf16(p.v, p.type, p.wide, (row0 + row) * p.ld_v + static_cast<int64_t>(of) * p.dv + (d < p.dv ? d : 0));
-    }
-  };
-  const int key_place = tile_place<L::kKeyPitch>(threadIdx.x / (DK / 8), my_key / 8);
-  const int value_place = tile_place<L::kValuePitch>(threadIdx.x / (L::kColumns / 8), my_value);
-  auto put = [&](int chunk) {
-    const int m = min(kChunk, rows - chunk * kChunk);
-    auto all = [&](auto in) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < kKeyLoads; ++e) {
-        const bool there = in(static_cast<int>(threadIdx.x) / (DK / 8) + e * kKeyStep < m && my_key < p.dk);
-        const int at = tile_place<L::kKeyPitch>(key_place, e * kKeyStep, 0);
-        *reinterpret_cast<u32x4*>(lds + L::kKeys + at) = there ? next_k[e] : u32x4{};
-        if constexpr (OUT) *reinterpret_cast<u32x4*>(lds + L::kQueries + at) = there ? next_q[e] : u32x4{};
+        if (OUT && with_queries) next_q[e] = *reinterpret_cast<const u32x4*>(q + q_from);
+        if (with_others) next_k[e] = *reinterpret_cast<const u32x4*>(k + k_from);
+        k += kKeyStep * p.ld_k, q += kKeyStep * p.ld_q;
       }
 #pragma unroll
       for (int e = 0; e < kValueLoads; ++e) {
-        const bool there = in(static_cast<int>(threadIdx.x) / (L::kColumns / 8) + e * kValueStep < m && head0 + my_value / (4 * TW) < head_end &&
-                              column0 + my_value % (4 * TW) * 8 < p.dv);
-        *reinterpret_cast<u32x4*>(lds + L::kValues + tile_place<L::kValuePitch>(value_place, e * kValueStep, 0)) = there ? next_v[e] : u32x4{};
+        if (with_others) next_v[e] = *reinterpret_cast<const u32x4*>(v + v_from);
+        v += kValueStep * p.ld_v;
       }
-    };
-    if (m == kChunk && whole_tiles) all([](bool) { return true; });
-    else all([](bool in) { return in; });
+      return;
+    }
+    auto load = [&](const void* x, int64_t i) { return load_eight_bf16(x, PLAIN ? LX_BF16 : p.type, PLAIN || p.wide, i); };
+#pragma unroll
+    for (int e = 0; e < kKeyLoads; ++e) {
+      const int64_t row = row0 + min(my_key_row + e * kKeyStep, last);
+      if (OUT && with_queries) next_q[e] = load(p.q, row * p.ld_q + k_column);
+      if (with_others) next_k[e] = load(p.k, row * p.ld_k + k_column);
+      if (!PLAIN) __builtin_amdgcn_sched_barrier(0);  // one after another: f32 values of all of them do not fit
+    }
+#pragma unroll
+    for (int e = 0; e < kValueLoads; ++e) {
+      if (with_others) next_v[e] = load(p.v, (row0 + min(my_value_row + e * kValueStep, last)) * p.ld_v + v_column);
+      if (!PLAIN) __builtin_amdgcn_sched_barrier(0);
+    }
   };
-  // The decay's numbers, a token a lane: asked for two chunks ahead, made ready one ahead, by the team's last wavefront.
+  // Behind the last chunk: values that nobody reads, so that the registers are known to be free until the next ones are asked for.
+  auto ask_nothing = [&](bool with_queries, bool with_others) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < kKeyLoads; ++e) {
+      if (OUT && with_queries) next_q[e] = u32x4{};
+      if (with_others) next_k[e] = u32x4{};
+    }
+#pragma unroll
+    for (int e = 0; e < kValueLoads; ++e)
+      if (with_others) next_v[e] = u32x4{};
+  };
+  ask(0, true, true);
+
+  // ---- the decays -----------------------------------------------------------------------------------------------------
+  // A token a lane: asked for two chunks ahead, made ready one ahead, by the team's last wavefront.
+  Tokens* const tokens = reinterpret_cast<Tokens*>(lds + L::kTokens) + 2 * team;
+  // A positive scale is part of the rows' exponents, another one multiplied in. The skip is part of a row's weight of its own token.
+  const bool scaled = PLAIN || positive(p.scale);
+  const float log_scale = scaled ? __builtin_amdgcn_logf(p.scale) : 0.0f;
   const bool counts = mate == TW - 1;
-  float next_log = 0.0f, next_weight = 1.0f;
+  const HeadDecay head_numbers = head_decay(p, head);
+  uint32_t next_raw;
+  float carried = 0.0f;
   auto ask_decay = [&](int chunk) {
-    next_log = 0.0f, next_weight = 1.0f;
-    if (chunk * kChunk + lane < rows) decay_of(p, first_row + static_cast<int64_t>(chunk) * kChunk + lane, head, next_log, next_weight);
+    next_raw = decay_raw(p, first_row + min(chunk * kChunk + lane, rows - 1), head);
   };
   auto put_decay = [&](int chunk) {
     Tokens& t = tokens[chunk % 2];
-    const double g = wave_scan(static_cast<double>(next_log) * 1.44269504088896340736);
-    const float b = next_weight == 1.0f ? 0.0f : fminf(fmaxf(__builtin_amdgcn_logf(next_weight), -1e5f), 1e5f);
-    const double more = g - static_cast<double>(next_weight != next_weight ? next_weight : b);
-    const uint64_t u = __builtin_bit_cast(uint64_t, g);
-    const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(u), kWave - 1), high = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), kWave - 1);
-    const double whole = __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | low);
-    t.g_high[lane] = static_cast<float>(g);
-    t.g_low[lane] = static_cast<float>(g - static_cast<double>(static_cast<float>(g)));
-    t.h_high[lane] = static_cast<float>(more);
-    t.h_low[lane] = static_cast<float>(more - static_cast<double>(static_cast<float>(more)));
-    t.update[lane] = __builtin_amdgcn_exp2f(static_cast<float>(whole - more));
-    t.seen[lane] = __builtin_amdgcn_exp2f(static_cast<float>(g));
-    if (lane == 0) t.whole = whole;
+    float log, weight;
+    decay_of(p, head_numbers, next_raw, log, weight);
+    if (chunk * kChunk + lane >= rows) log = 0.0f, weight = 1.0f;
+    const float units = log * (1.44269504f * 256.0f), whole_units = floorf(units);
+    const int64_t g = wave_scan(static_cast<int64_t>(static_cast<int>(whole_units)) << 32 | static_cast<uint32_t>((units - whole_units) * 0x1p32f));
+    const float high = static_cast<float>(static_cast<int>(g >> 32)) * 0x1p-8f, rest = static_cast<float>(static_cast<uint32_t>(g)) * 0x1p-40f;
+    auto last = [](float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), kWave - 1)); };
+    const float last_high = last(high), last_rest = last(rest);
+    // No update at all: an exponent far below; a NaN of a logarithm or a weight is all that is left of a column.
+    const float column = rest - (weight == 1.0f ? 0.0f : fmaxf(__builtin_amdgcn_logf(weight), -1e5f)) + (log - log);
+    if constexpr (OUT) {
+      const float row = rest + log_scale;
+      t.high[lane] = high;
+      t.row[lane] = row;
+      t.column[lane] = column;
+      t.seen[lane] = __builtin_amdgcn_exp2f(high + row) * (scaled ? 1.0f : p.scale);
+    }
+    t.update[lane] = __builtin_amdgcn_exp2f((last_high - high) + (last_rest - column));
+    // What a factor's rounding leaves goes into the next one: a state that lasts many chunks does not drift.
+    const float whole = (last_high + last_rest) * 0.693147181f;
+    const Fade fade = fade_of(whole);
+    const float more = __builtin_fmaf(fade.high, carried, fade.low), factor = fade.high + more;
+    carried = (more - (factor - fade.high)) * __builtin_amdgcn_rcpf(factor);
+    if (!(fabsf(carried) < 1.0f)) carried = 0.0f;
+    if (lane == 0) t.whole = whole, t.fade = factor;
   };
+  if (counts) ask_decay(0);
 
   // ---- the state ------------------------------------------------------------------------------------------------------
   f32x16 state[DK / 32] = {};
-  const int slot = __builtin_amdgcn_readfirstlane(mix_slot(p.states, s));
   const bool mine = column < p.dv && !idle;
   const int64_t state_size = static_cast<int64_t>(p.dk) * p.dv;
   const unsigned state_from = static_cast<unsigned>(8 * h * p.dv + column);
@@ -301,119 +315,165 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 ? 1 : 2) linear_
   const float skip = p.skip ? p.skip[head] : 0.0f;
   double part_log = 0.0;
 
+  // ---- places in LDS --------------------------------------------------------------------------------------------------
+  // `now` of a place: what is made of it is made anew for each chunk (the compiler would keep every address from chunk to chunk, in registers that
+  // then hold none of what is on its way).
+  auto now = [](int place) {
+    asm("" : "+v"(place));
+    return place;
+  };
+  const int key_place = tile_place<L::kKeyPitch>(my_key_row, my_key / 8), value_place = tile_place<L::kValuePitch>(my_value_row, my_value);
+  auto put = [&](int chunk, bool with_queries, bool with_others) __attribute__((always_inline)) {
+    const int m = min(kChunk, rows - chunk * kChunk);
+    auto all = [&](auto in) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < kKeyLoads; ++e) {
+        const bool there = in(my_key_row + e * kKeyStep < m && my_key_in);
+        const int at = tile_place<L::kKeyPitch>(key_place, e * kKeyStep, 0);
+        if (OUT && with_queries) *reinterpret_cast<u32x4*>(lds + L::kQueries + at) = there ? next_q[e] : u32x4{};
+        if (with_others) *reinterpret_cast<u32x4*>(lds + L::kKeys + at) = there ? next_k[e] : u32x4{};
+      }
+#pragma unroll
+      for (int e = 0; e < kValueLoads; ++e) {
+        const bool there = in(my_value_row + e * kValueStep < m && my_value_in);
+        if (with_others) *reinterpret_cast<u32x4*>(lds + L::kValues + tile_place<L::kValuePitch>(value_place, e * kValueStep, 0)) = there ? next_v[e] : u32x4{};
+      }
+    };
+    if (m == kChunk && whole_tiles) all([](bool) { return true; });
+    else all([](bool in) { return in; });
+  };
+  // Where the lane's first reads lie: row n of the keys (and queries), the columns of the keys and of its values, row n of the weights.
+  const int key_row = tile_place<L::kKeyPitch>(n, h);
+  const int key_column = across_place<L::kKeyPitch>(0), value_column = across_place<L::kValuePitch>(32 * wave);
+  const int weight_row = L::kWeights + team * L::kWeightBytes + 64 * n + 16 * (n >> 2 & 3);
+  auto values_across = [&](int k) { return across<L::kValuePitch>(lds, L::kValues, value_column, k, 0); };
+  const int64_t columns = static_cast<int64_t>(head) * p.dv + column0 + 32 * mate;  // the lane's outputs of a row: 16 a + 8 h .. from here on
+  const int my_column = column0 + 32 * mate + 8 * h;
+  const int out_place = static_cast<int>(n * p.ld_out + 8 * h), gate_place = static_cast<int>(n * p.ld_gate + 8 * h);
+
   if (counts) {
-    ask_decay(0);
     put_decay(0);
     ask_decay(1);
   }
-  ask(0);
-  put(0);
+  put(0, true, true);
   __syncthreads();
   for (int chunk = 0; chunk < chunks; ++chunk) {
     const Tokens& t = tokens[chunk % 2];
     const int m = min(kChunk, rows - chunk * kChunk);
     const bool more = chunk + 1 < chunks, two = m > 32;
-    if (more) ask(chunk + 1);
+    const int64_t row0 = first_row + static_cast<int64_t>(chunk) * kChunk;
+    // Queries of the next chunk first, they are put in LDS first; keys and values when the state's products have left their registers.
+    if (more) ask(chunk + 1, true, !OUT);
+    else ask_nothing(true, !OUT);
     __builtin_amdgcn_sched_barrier(0);
     f32x16 out[2] = {};
     if constexpr (OUT) {
-      // Weights: tile `block` has tokens 32 jb .. of rows 32 ib ..
-      auto weigh = [&](int block) {
-        const int jb = block == 2, ib = block > 0;
-        f32x16 w = {};
+      // Weights, in tiles of 32 rows by 32 tokens: (0, 0), (1, 0), (1, 1). Their products here, what is made of them between the products of the
+      // state, which are half as many instructions of the matrix cores as they need of the vector unit.
+      const int from = now(key_row), to = now(weight_row), here = now(n);  // compared anew: kept, the results cost more scalar registers than there are
+      auto raw_weights = [&](int block, f32x16& w) __attribute__((always_inline)) {
+        const int keys_at = L::kKeys + (block == 2) * 32 * L::kKeyPitch, queries_at = L::kQueries + (block > 0) * 32 * L::kKeyPitch;
+        w = f32x16{};
 #pragma unroll
-        for (int k = 0; k < DK / 16; ++k)
-          w = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_keys(32 * jb, k), read_queries(32 * ib, k), w, 0, 0, 0);
-        const float g_high = t.g_high[32 * ib + n], g_low = t.g_low[32 * ib + n];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int token = 8 * g + 4 * h;  // of the tile's, and the three behind it
-          const f32x4 h_high = *reinterpret_cast<const f32x4*>(t.h_high + 32 * jb + token), h_low = *reinterpret_cast<const f32x4*>(t.h_low + 32 * jb + token);
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = w[4 * g + e] * __builtin_amdgcn_exp2f((g_high - h_high[e]) + (g_low - h_low[e]));
-            if (jb == ib) v[e] = token + e <= n ? v[e] : 0.0f;
-          }
-          const uint32_t a = __builtin_bit_cast(uint32_t, pack_bf16(v[0], v[1])), b = __builtin_bit_cast(uint32_t, pack_bf16(v[2], v[3]));
-          const u32x2 left = {__builtin_bit_cast(uint32_t, pack_bf16(v[0] - __uint_as_float(a << 16), v[1] - __uint_as_float(a & 0xffff0000u))),
-                              __builtin_bit_cast(uint32_t, pack_bf16(v[2] - __uint_as_float(b << 16), v[3] - __uint_as_float(b & 0xffff0000u)))};
-          uint8_t* const at = lds + L::kWeights + block * L::kBlock + (weight_row ^ 16 * g) + 8 * h;
-          *reinterpret_cast<u32x2*>(at) = u32x2{a, b};
-          *reinterpret_cast<u32x2*>(at + 3 * L::kBlock) = left;
+        for (int k = 0; k < DK / 16; ++k) {
+          w = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_at(lds, keys_at + (from ^ 32 * k)), eight_at(lds, queries_at + (from ^ 32 * k)), w, 0, 0, 0);
+          if (k % 2) __builtin_amdgcn_sched_barrier(0);  // no more reads ahead than registers
         }
       };
-      if constexpr (TW == 2) {
-        if (mate == 0) {
-          weigh(0);
-          if (two) weigh(1);
-        } else if (two) {
-          weigh(2);
+      // Tokens 8 g + 4 h .. + 3 of the tile's.
+      auto weigh = [&](int block, const f32x16& w, int g) __attribute__((always_inline)) {
+        const int jb = block == 2, ib = block > 0, until = jb == ib ? here : 32, own = jb == ib ? here : -1;
+        const float high = t.high[32 * ib + n], row = t.row[32 * ib + n];
+        const int token = 8 * g + 4 * h;
+        const f32x4 highs = *reinterpret_cast<const f32x4*>(t.high + 32 * jb + token), columns = *reinterpret_cast<const f32x4*>(t.column + 32 * jb + token);
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = w[4 * g + e] * __builtin_amdgcn_exp2f((high - highs[e]) + (row - columns[e]));
+          if (!scaled) v[e] *= p.scale;
+          v[e] = token + e <= until ? v[e] : 0.0f;
+          v[e] += token + e == own ? skip : 0.0f;
         }
-      } else if (mate < 3 && (two || mate == 0)) {
-        weigh(mate);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      // What the rows see of the state: queries read one step ahead.
-      bf16x8 q[2][2];
-      auto read = [&](int k) {
-        q[k % 2][0] = read_queries(0, k);
-        q[k % 2][1] = read_queries(32, k);
+        const uint32_t a = __builtin_bit_cast(uint32_t, pack_bf16(v[0], v[1])), b = __builtin_bit_cast(uint32_t, pack_bf16(v[2], v[3]));
+        const u32x2 left = {__builtin_bit_cast(uint32_t, pack_bf16(v[0] - __uint_as_float(a << 16), v[1] - __uint_as_float(a & 0xffff0000u))),
+                            __builtin_bit_cast(uint32_t, pack_bf16(v[2] - __uint_as_float(b << 16), v[3] - __uint_as_float(b & 0xffff0000u)))};
+        uint8_t* const at = lds + block * L::kBlock + (to ^ 16 * g) + 8 * h;
+        *reinterpret_cast<u32x2*>(at) = u32x2{a, b};
+        *reinterpret_cast<u32x2*>(at + 3 * L::kBlock) = left;
       };
-      read(0);
+      // What the rows see of the state, a step's queries and halves of the state made ready one ahead; `blocks`: tiles of weights that the wavefront
+      // makes meanwhile, the first one tile `block`.
+      auto see = [&](auto blocks, int block) __attribute__((always_inline)) {
+        constexpr int kTiles = decltype(blocks)::value, kSteps = DK / 16;
+        f32x16 w;
+        if constexpr (kTiles > 0) raw_weights(block, w);
+        bf16x8 q[2][2], high[2], low[2];
+        auto ready = [&](int k) __attribute__((always_inline)) {
+          q[k % 2][0] = eight_at(lds, L::kQueries + (from ^ 32 * k));
+          q[k % 2][1] = eight_at(lds, L::kQueries + 32 * L::kKeyPitch + (from ^ 32 * k));
+          float v[8];
 #pragma unroll
-      for (int k = 0; k < DK / 16; ++k) {
-        if (k + 1 < DK / 16) read(k + 1);
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = state[k / 2][k % 2 * 8 + e];
-        bf16x8 high, low;
-        split_eight(v, high, low);
-        out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high, q[k % 2][0], out[0], 0, 0, 0);
-        out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high, q[k % 2][1], out[1], 0, 0, 0);
-        out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low, q[k % 2][0], out[0], 0, 0, 0);
-        out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low, q[k % 2][1], out[1], 0, 0, 0);
+          for (int e = 0; e < 8; ++e) v[e] = state[k / 2][k % 2 * 8 + e];
+          split_eight(v, high[k % 2], low[k % 2]);
+        };
+        ready(0);
         __builtin_amdgcn_sched_barrier(0);
-      }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          if (k + 1 < kSteps) ready(k + 1);
+          out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high[k % 2], q[k % 2][0], out[0], 0, 0, 0);
+          out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high[k % 2], q[k % 2][1], out[1], 0, 0, 0);
+          out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low[k % 2], q[k % 2][0], out[0], 0, 0, 0);
+          out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low[k % 2], q[k % 2][1], out[1], 0, 0, 0);
+#pragma unroll
+          for (int g = 4 * kTiles * k / kSteps; g < 4 * kTiles * (k + 1) / kSteps; ++g) weigh(block + g / 4, w, g % 4);
+          __builtin_amdgcn_sched_barrier(0);
+          if (kTiles > 1 && 2 * (k + 1) == kSteps) raw_weights(block + 1, w);
+        }
+      };
+      if (TW == 2 ? mate == 0 && two : false) see(std::integral_constant<int, TW == 2 ? 2 : 0>(), 0);
+      else if (mate == 0 || (mate < 3 && two)) see(std::integral_constant<int, 1>(), TW == 2 ? 2 * mate : mate);
+      else see(std::integral_constant<int, 0>(), 0);
 #pragma unroll
       for (int i = 0; i < 2; ++i) out[i] *= t.seen[32 * i + n];
     }
+    // Gates are asked for here: earlier, they would take registers from what went before.
+    u32x4 gate[2][2];
+    if (OUT && PLAIN && p.gate) {
+      const unsigned gate_from = now(gate_place);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          gate[i][a] = u32x4{};
+          if (32 * i + n < m && my_column + 16 * a < p.dv)
+            gate[i][a] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.gate) + (row0 + 32 * i) * p.ld_gate + columns + 16 * a + gate_from);
+        }
+    }
+    if (OUT && more) ask(chunk + 1, false, true);
+    else if (OUT) ask_nothing(false, true);
+    __builtin_amdgcn_sched_barrier(0);
     if (counts && more) {
       put_decay(chunk + 1);
       ask_decay(chunk + 2);
     }
     if constexpr (OUT) __syncthreads();
 
-    // Gates of the usual type are asked for here.
-    const bool gates = OUT && p.gate && p.wide && p.gate_type == LX_BF16;
-    u32x4 gate[2][2];
-    if (gates) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const int d = column0 + 32 * mate + 16 * a + 8 * h;
-          const int64_t row = first_row + static_cast<int64_t>(chunk) * kChunk + min(32 * i + n, m - 1);
-          gate[i][a] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.gate) + row * p.ld_gate + static_cast<int64_t>(head) * p.dv + (d < p.dv ? d : 0));
-        }
-    }
     bf16x8 v[kChunk / 16];
 #pragma unroll
     for (int k = 0; k < kChunk / 16; ++k) v[k] = values_across(k);
     if constexpr (OUT) {
-      auto weight_unit = [&](int block, int k, int low) {  // of row n, tokens 16 k + 8 h .. of the tile
-        return eight_at(lds, L::kWeights + (block + 3 * low) * L::kBlock + ((weight_row ^ 16 * h) ^ 32 * k));
-      };
+      if (more) put(chunk + 1, true, false);  // nobody reads this chunk's queries any more
       // A weight of nothing times an infinity or a NaN of a later token is no number: those are taken out of the product, and what rows behind
       // them see of them is added by itself.
-      float odd = 0.0f;
+      float odd[2] = {};
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k) {
         const u32x4 raw = __builtin_bit_cast(u32x4, v[k]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd = __builtin_amdgcn_fdot2_f32_bf16(as_bf16x2(raw[e]), as_bf16x2(0), odd, false);
+        for (int e = 0; e < 4; ++e) odd[e % 2] = __builtin_amdgcn_fdot2_f32_bf16(as_bf16x2(raw[e]), as_bf16x2(0), odd[e % 2], false);
       }
-      const bool some_odd = __any(odd != odd);
+      const bool some_odd = __any(odd[0] + odd[1] != 0.0f);
       if (some_odd) {
 #pragma unroll
         for (int k = 0; k < kChunk / 16; ++k) {
@@ -430,7 +490,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 ? 1 : 2) linear_
           for (int i = 0; i < 2; ++i) {
             if (token > 32 * i + n || 32 * i >= m) continue;
             const int in = token % 32;
-            const uint8_t* const at = lds + L::kWeights + (i + token / 32) * L::kBlock + (weight_row ^ 16 * (in / 8)) + in % 8 * 2;
+            const uint8_t* const at = lds + (i + token / 32) * L::kBlock + (weight_row ^ 16 * (in / 8)) + in % 8 * 2;
             const float weight = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(at)) + bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(at + 3 * L::kBlock));
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
@@ -445,101 +505,99 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 ? 1 : 2) linear_
         }
       }
       __builtin_amdgcn_sched_barrier(0);
+      // The weights' products, the gates' factors meanwhile.
+      const int from = now(weight_row ^ 16 * h);
+      auto weight_unit = [&](int block, int k, int low) {  // of row n, tokens 16 k + 8 h .. of the tile
+        return eight_at(lds, (block + 3 * low) * L::kBlock + (from ^ 32 * k));
+      };
 #pragma unroll
-      for (int k = 0; k < kChunk / 16; ++k) {
+      for (int k = 0; k < kChunk / 16; ++k)
 #pragma unroll
         for (int low = 0; low < 2; ++low) {
           if (k < 2) out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(0, k, low), out[0], 0, 0, 0);
           if (two) out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(1 + k / 2, k % 2, low), out[1], 0, 0, 0);
         }
-      }
       __builtin_amdgcn_sched_barrier(0);
       if (some_odd) {
 #pragma unroll
         for (int k = 0; k < kChunk / 16; ++k) v[k] = values_across(k);
       }
-    }
-    // The state behind the chunk.
-    const double whole = t.whole;
-    const Fade fade = fade_of(whole);
-    if (__builtin_amdgcn_readfirstlane(fade.slow)) {
-#pragma unroll
-      for (int x = 0; x < DK / 32; ++x)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) state[x][r] = __builtin_fmaf(state[x][r], fade.factor, state[x][r]);
-    } else {
-#pragma unroll
-      for (int x = 0; x < DK / 32; ++x) state[x] *= fade.factor;
-    }
-    part_log += whole;
-#pragma unroll
-    for (int k = 0; k < kChunk / 16; ++k) {
-      const u32x4 raw = __builtin_bit_cast(u32x4, v[k]);
-      const f32x4 w0 = *reinterpret_cast<const f32x4*>(t.update + 16 * k + 8 * h), w1 = *reinterpret_cast<const f32x4*>(t.update + 16 * k + 8 * h + 4);
-      float scaled[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t pair = raw[e / 2];
-        scaled[e] = __uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16) * (e < 4 ? w0[e % 4] : w1[e % 4]);
-      }
-      bf16x8 high, low;
-      split_eight(scaled, high, low);
-#pragma unroll
-      for (int x = 0; x < DK / 32; ++x) {
-        const bf16x8 key = keys_across(x, k);
-        state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key, high, state[x], 0, 0, 0);
-        state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key, low, state[x], 0, 0, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (OUT) {
       if (!idle) {
+        const unsigned out_from = now(out_place), gate_from = now(gate_place);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (32 * i + n >= m) continue;
-          const int64_t row = first_row + static_cast<int64_t>(chunk) * kChunk + 32 * i + n;
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
-            const int d = column0 + 32 * mate + 16 * a + 8 * h;
-            if (d >= p.dv) continue;
-            const u32x4 eight = __builtin_bit_cast(u32x4, eight_at(lds, L::kValues + tile_place<L::kValuePitch>(value_row, 32 * i, 2 * a)));
+            if (my_column + 16 * a >= p.dv) continue;
+            const int64_t at = (row0 + 32 * i) * p.ld_out + columns + 16 * a;
             float o[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint32_t pair = eight[e / 2];
-              o[e] = out[i][8 * a + e] * p.scale;
-              if (p.skip) o[e] = __builtin_fmaf(skip, __uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16), o[e]);
-            }
-            const int64_t at = static_cast<int64_t>(head) * p.dv + d;
-            if (gates) {
+            for (int e = 0; e < 8; ++e) o[e] = out[i][8 * a + e];
+            if (PLAIN && p.gate) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const uint32_t pair = gate[i][a][e / 2];
-                o[e] *= quick_silu(__uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16));
+                o[e] *= gate_of(__uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16));
               }
             } else if (p.gate) {
 #pragma unroll
               for (int e = 0; e < 8; e += 4) {
-                const f32x4 z = load_four(p.gate, p.gate_type, p.wide, row * p.ld_gate + at + e);
+                const f32x4 z = load_four(p.gate, p.gate_type, p.wide, (row0 + 32 * i) * p.ld_gate + columns + 16 * a + gate_from + e);
 #pragma unroll
-                for (int f = 0; f < 4; ++f) o[e + f] *= quick_silu(z[f]);
+                for (int f = 0; f < 4; ++f) o[e + f] *= gate_of(z[f]);
               }
             }
-            if (p.wide && p.out_type == LX_BF16) {
+            if ((PLAIN || p.wide) && p.out_type == LX_BF16) {
               const u32x4 packed = {__builtin_bit_cast(uint32_t, pack_bf16(o[0], o[1])), __builtin_bit_cast(uint32_t, pack_bf16(o[2], o[3])),
                                     __builtin_bit_cast(uint32_t, pack_bf16(o[4], o[5])), __builtin_bit_cast(uint32_t, pack_bf16(o[6], o[7]))};
-              *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out) + row * p.ld_out + at) = packed;
+              *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out) + at + out_from) = packed;
             } else {
-              store_four(p.out, p.out_type, p.wide, row * p.ld_out + at, f32x4{o[0], o[1], o[2], o[3]});
-              store_four(p.out, p.out_type, p.wide, row * p.ld_out + at + 4, f32x4{o[4], o[5], o[6], o[7]});
+              store_four(p.out, PLAIN ? LX_F32 : p.out_type, PLAIN || p.wide, at + out_from, f32x4{o[0], o[1], o[2], o[3]});
+              store_four(p.out, PLAIN ? LX_F32 : p.out_type, PLAIN || p.wide, at + out_from + 4, f32x4{o[4], o[5], o[6], o[7]});
             }
           }
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // The state behind the chunk: a step's keys and scaled values made ready one ahead.
+    {
+      const float fade = t.fade;
+      const int from = now(key_column);
+      if constexpr (!OUT) part_log += t.whole;
+      bf16x8 key[2][DK / 32], high[2], low[2];
+      auto ready = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < DK / 32; ++x)
+          key[k % 2][x] = across<L::kKeyPitch>(lds, L::kKeys, from, k, 4 * x);  // columns 32 x .. of tokens 16 k ..
+        const u32x4 raw = __builtin_bit_cast(u32x4, v[k]);
+        const f32x4 w0 = *reinterpret_cast<const f32x4*>(t.update + 16 * k + 8 * h), w1 = *reinterpret_cast<const f32x4*>(t.update + 16 * k + 8 * h + 4);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t pair = raw[e / 2];
+          x[e] = __uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16) * (e < 4 ? w0[e % 4] : w1[e % 4]);
+        }
+        split_eight(x, high[k % 2], low[k % 2]);
+      };
+      ready(0);
+#pragma unroll
+      for (int x = 0; x < DK / 32; ++x) state[x] *= fade;
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < kChunk / 16; ++k) {
+        if (k + 1 < kChunk / 16) ready(k + 1);
+#pragma unroll
+        for (int x = 0; x < DK / 32; ++x) state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key[k % 2][x], high[k % 2], state[x], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < DK / 32; ++x) state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key[k % 2][x], low[k % 2], state[x], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     __syncthreads();
     if (more) {
-      put(chunk + 1);
+      put(chunk + 1, false, true);
       __syncthreads();
     }
   }
@@ -576,9 +634,9 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const ChunkArgs c) {
     const f32x4 before = state;
     if (k + 1 < parts) {
       const f32x4 sum = *at;
-      const Fade fade = fade_of(c.logs[(place + k) * p.heads + head]);
+      const Fade fade = fade_of(static_cast<float>(c.logs[(place + k) * p.heads + head]));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) state[e] = (fade.slow ? __builtin_fmaf(state[e], fade.factor, state[e]) : state[e] * fade.factor) + sum[e];
+      for (int e = 0; e < 4; ++e) state[e] = __builtin_fmaf(state[e], fade.high, __builtin_fmaf(state[e], fade.low, sum[e]));
     }
     *at = before;
   }

@@ -87,9 +87,9 @@ __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 3) linear_step_kernel(co
   float fades, lefts, weights = 1.0f;
   {
     float log = 0.0f;
-    if (lane < rows) decay_of(p, first + lane, head, log, weights);
-    const float less = expm1f(log), slow = 1.0f + less;
-    fades = log > -0.5f ? slow : expf(log), lefts = log > -0.5f ? less - (slow - 1.0f) : 0.0f;
+    if (lane < rows) decay_of(p, head_decay(p, head), decay_raw(p, first + lane, head), log, weights);
+    const float less = quick_expm1(log), slow = 1.0f + less;
+    fades = log > -0.5f ? slow : quick_exp(log), lefts = log > -0.5f ? less - (slow - 1.0f) : 0.0f;
   }
   auto of_token = [&](float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); };
 

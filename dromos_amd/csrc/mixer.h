@@ -53,6 +53,7 @@ inline int64_t mix_piece_count(const MixBatch& b, const MixPieces& p) { return p
 // ascend.
 template <typename Number>
 __device__ __forceinline__ int mix_last(int seqs, int64_t w, Number number) {
+  if (seqs == 1) return number(0) <= w ? 0 : -1;
   const int lane = threadIdx.x % kWave;
   int low = 0, count = seqs;
   while (true) {

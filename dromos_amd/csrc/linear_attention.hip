@@ -6,7 +6,7 @@ namespace dro {
 namespace {
 
 constexpr int kMaxDk = 256, kMaxDv = 512, kMaxHeads = 4096;
-constexpr int kMaxStride = 1 << 24;  // values: rows of a chunk are told apart in 32 bits
+constexpr int kMaxStride = 1 << 22;  // values: rows of a chunk are told apart in 31 bits
 constexpr int kMostSteps = 16;  // rows of a sequence that go token by token
 
 template <int COLS, int ROWS>
@@ -39,8 +39,10 @@ constexpr int kLeastPart = 256;
 Cut cut_of(int T, int max_rows, int heads, int k_heads, int dk, int dv) {
   Cut c;
   const int group = heads / k_heads;
-  c.waves = dv <= 64 ? 2 : 4;
+  // A head of 64 columns or fewer has two wavefronts, and a workgroup two such heads, if there are two that read the same keys; 256 keys' values are too many
+  // loads for two wavefronts.
   c.teams = dv <= 64 && group > 1 ? 2 : 1;
+  c.waves = dv <= 64 && (c.teams == 2 || dk <= 128) ? 2 : 4;
   c.across = c.teams > 1 ? (group + 1) / 2 : group * ((dv + 32 * c.waves - 1) / (32 * c.waves));
   // As many parts as fill the device once: a part costs a second look at its keys and values.
   const int64_t places = static_cast<int64_t>(dk > 128 ? 1 : 2) * compute_units(), columns = static_cast<int64_t>(c.across) * k_heads;
@@ -85,7 +87,10 @@ int chunks_of(const ChunkArgs& a, hipStream_t s) {
 
 template <int DK>
 int chunks_by(const ChunkArgs& a, const Cut& c, hipStream_t s) {
-  return c.waves == 4 ? chunks_of<DK, 4, 1>(a, s) : c.teams == 2 ? chunks_of<DK, 2, 2>(a, s) : chunks_of<DK, 2, 1>(a, s);
+  if (c.waves == 4) return chunks_of<DK, 4, 1>(a, s);
+  if (c.teams == 2) return chunks_of<DK, 2, 2>(a, s);
+  if constexpr (DK <= 128) return chunks_of<DK, 2, 1>(a, s);
+  return kInvalid;
 }
 
 int chunks(const LinearArgs& p, void* workspace, hipStream_t s) {

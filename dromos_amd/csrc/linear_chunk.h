@@ -84,14 +84,29 @@ __device__ __forceinline__ bf16x8 across(const uint8_t* lds, int at, int from, i
   return r.whole;
 }
 
-// Eight f32 as bf16, and what their rounding leaves as bf16.
+// Two f32 as bf16, and what their rounding leaves as bf16. Values that are not used again: taken off by one instruction each, in place (a dot product
+// with minus one and nothing; an infinity or a NaN of one is one of the other's rest too, which is summed with it). KEPT: by two.
+template <bool KEPT>
+__device__ __forceinline__ void split_two(float x, float y, uint32_t& high, uint32_t& low) {
+  const bf16x2 two = pack_bf16(x, y);
+  high = __builtin_bit_cast(uint32_t, two);
+  if constexpr (KEPT) {
+    low = __builtin_bit_cast(uint32_t, pack_bf16(x - __uint_as_float(high << 16), y - __uint_as_float(high & 0xffff0000u)));
+  } else {
+    uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+    asm("" : "+s"(first), "+s"(second));  // as constants of the instruction they are something else
+    low = __builtin_bit_cast(uint32_t, pack_bf16(__builtin_amdgcn_fdot2_f32_bf16(two, as_bf16x2(first), x, false),
+                                                 __builtin_amdgcn_fdot2_f32_bf16(two, as_bf16x2(second), y, false)));
+  }
+}
+template <bool KEPT>
 __device__ __forceinline__ void split_eight(const float (&v)[8], bf16x8& high, bf16x8& low) {
   u32x4 a, b;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t two = __builtin_bit_cast(uint32_t, pack_bf16(v[2 * j], v[2 * j + 1]));
-    a[j] = two;
-    b[j] = __builtin_bit_cast(uint32_t, pack_bf16(v[2 * j] - __uint_as_float(two << 16), v[2 * j + 1] - __uint_as_float(two & 0xffff0000u)));
+    uint32_t x, y;
+    split_two<KEPT>(v[2 * j], v[2 * j + 1], x, y);
+    a[j] = x, b[j] = y;
   }
   high = __builtin_bit_cast(bf16x8, a);
   low = __builtin_bit_cast(bf16x8, b);
@@ -122,17 +137,20 @@ __device__ __forceinline__ Fade fade_of(float log) {
   return log > -0.5f ? Fade{high, less - (high - 1.0f)} : Fade{quick_exp(log), 0.0f};
 }
 
-// The numbers of a chunk's tokens. G_i (base 2) is a sum of integers, 2^-40 each, and so exact: `high` its whole 256ths and a rest. Logarithms of
-// -200 at least keep 64 of them within the 24 bits of `high`.
+// The numbers of a chunk's tokens. G_i (base 2) is a sum of integers, 2^-40 each, and so exact: its whole 256ths and a rest. Logarithms of -200 at
+// least keep 64 of them within the 24 bits of the former.
+// The factor of a row's weight of a token is a product where nothing in it can overflow or is large enough to lose bits: with R the sum up to the row's
+// half of the chunk, e^{G_i - R} times e^{R - G_j} b_j (`quick`: G falls by 24 at most in either half). Otherwise it is made from the difference.
 struct Tokens {
-  float high[kChunk];
-  float row[kChunk];     // the rest of G_i + log(scale)
-  float column[kChunk];  // the rest of G_j - log(b_j)
+  float row[kChunk];     // quick: scale e^{G_i - R}; otherwise the rest of G_i + log(scale)
+  float column[kChunk];  // quick: e^{R - G_j} b_j, R of the token's own half; otherwise the rest of G_j - log(b_j)
+  float other[kChunk];   // quick: the same with R of the second half, of tokens of the first one; otherwise the 256ths of G_i
   float update[kChunk];  // e^{G_63 - G_j} b_j
   float seen[kChunk];    // scale e^{G_i}
   float fade;            // e^{G_63}, and what its rounding left of the chunks before
   float whole;           // the logarithm of e^{G_63}
-  float none[2];         // whole 16 bytes
+  int quick;
+  float none;  // whole 16 bytes
 };
 
 template <int DK, int TW, int TEAMS>
@@ -148,6 +166,17 @@ struct ChunkTiles {
   static constexpr int kQueries = kTokens + (2 * TEAMS * static_cast<int>(sizeof(Tokens)) + 255) / 256 * 256, kWeights = kQueries + kKeyBytes;
   static constexpr int kSumBytes = kQueries, kBytes = kWeights + TEAMS * kWeightBytes;
 };
+
+// A part of a tensor as a buffer: what is read behind its end is zero and what is stored there is dropped, without a branch (behind which the
+// compiler would not know how many loads are on their way, and wait for all).
+constexpr unsigned kOutside = 0x80000000u;  // no buffer here is as long
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4 buffer_load(__amdgpu_buffer_rsrc_t b, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0); }
+__device__ __forceinline__ void buffer_store(__amdgpu_buffer_rsrc_t b, unsigned at, u32x4 v) { __builtin_amdgcn_raw_buffer_store_b128(v, b, at, 0, 0); }
+// Bytes of m rows of `width` values, `ld` apart.
+__device__ __forceinline__ int rows_bytes(int m, int64_t ld, int width, int size) { return m > 0 ? ((m - 1) * static_cast<int>(ld) + width) * size : 0; }
 
 // A scale that can be part of an exponent.
 __host__ __device__ __forceinline__ bool positive(float scale) { return scale > 1e-30f && scale < 1e30f; }
@@ -198,54 +227,51 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
   const int my_head = min(head0 + my_value / (4 * TW), head_end - 1), my_value_at = column0 + my_value % (4 * TW) * 8;
   const bool my_key_in = my_key < p.dk, my_value_in = my_value_at < p.dv && head0 + my_value / (4 * TW) < head_end;
   const unsigned k_column = k_head * p.dk + (my_key_in ? my_key : 0), v_column = my_head * p.dv + (my_value_in ? my_value_at : 0);
-  const unsigned k_from = static_cast<unsigned>(my_key_row * p.ld_k) + k_column, q_from = static_cast<unsigned>(my_key_row * p.ld_q) + k_column;
-  const unsigned v_from = static_cast<unsigned>(my_value_row * p.ld_v) + v_column;
-  auto ask = [&](int chunk, bool with_queries, bool with_others) __attribute__((always_inline)) {
+  const unsigned k_from = my_key_in ? 2 * (static_cast<unsigned>(my_key_row * p.ld_k) + k_column) : kOutside;
+  const unsigned q_from = my_key_in ? 2 * (static_cast<unsigned>(my_key_row * p.ld_q) + k_column) : kOutside;
+  const unsigned v_from = my_value_in ? 2 * (static_cast<unsigned>(my_value_row * p.ld_v) + v_column) : kOutside;
+  auto ask = [&](int chunk) __attribute__((always_inline)) {
     const int64_t row0 = first_row + static_cast<int64_t>(chunk) * kChunk;
-    const int last = min(kChunk, rows - chunk * kChunk) - 1;
-    if (PLAIN && last == kChunk - 1) {
-      const uint16_t* k = static_cast<const uint16_t*>(p.k) + row0 * p.ld_k;
-      const uint16_t* q = static_cast<const uint16_t*>(p.q) + row0 * p.ld_q;
-      const uint16_t* v = static_cast<const uint16_t*>(p.v) + row0 * p.ld_v;
+    if constexpr (PLAIN) {  // behind the last chunk too: of nothing
+      const int m = min(kChunk, rows - chunk * kChunk), keys = p.k_heads * p.dk, all = p.heads * p.dv;
+      const auto k = buffer_of(static_cast<const uint16_t*>(p.k) + row0 * p.ld_k, rows_bytes(m, p.ld_k, keys, 2));
+      const auto q = buffer_of(static_cast<const uint16_t*>(p.q) + row0 * p.ld_q, rows_bytes(m, p.ld_q, keys, 2));
+      const auto v = buffer_of(static_cast<const uint16_t*>(p.v) + row0 * p.ld_v, rows_bytes(m, p.ld_v, all, 2));
 #pragma unroll
       for (int e = 0; e < kKeyLoads; ++e) {
-        if (OUT && with_queries) next_q[e] = *reinterpret_cast<const u32x4*>(q + q_from);
-        if (with_others) next_k[e] = *reinterpret_cast<const u32x4*>(k + k_from);
-        k += kKeyStep * p.ld_k, q += kKeyStep * p.ld_q;
+        next_k[e] = buffer_load(k, k_from + e * static_cast<unsigned>(2 * kKeyStep * p.ld_k));
+        if constexpr (OUT) next_q[e] = buffer_load(q, q_from + e * static_cast<unsigned>(2 * kKeyStep * p.ld_q));
       }
 #pragma unroll
-      for (int e = 0; e < kValueLoads; ++e) {
-        if (with_others) next_v[e] = *reinterpret_cast<const u32x4*>(v + v_from);
-        v += kValueStep * p.ld_v;
-      }
+      for (int e = 0; e < kValueLoads; ++e) next_v[e] = buffer_load(v, v_from + e * static_cast<unsigned>(2 * kValueStep * p.ld_v));
       return;
     }
-    auto load = [&](const void* x, int64_t i) { return load_eight_bf16(x, PLAIN ? LX_BF16 : p.type, PLAIN || p.wide, i); };
+    const int last = min(kChunk, rows - chunk * kChunk) - 1;
+    auto load = [&](const void* x, int64_t i) { return load_eight_bf16(x, p.type, p.wide, i); };
 #pragma unroll
     for (int e = 0; e < kKeyLoads; ++e) {
       const int64_t row = row0 + min(my_key_row + e * kKeyStep, last);
-      if (OUT && with_queries) next_q[e] = load(p.q, row * p.ld_q + k_column);
-      if (with_others) next_k[e] = load(p.k, row * p.ld_k + k_column);
-      if (!PLAIN) __builtin_amdgcn_sched_barrier(0);  // one after another: f32 values of all of them do not fit
+      if constexpr (OUT) next_q[e] = load(p.q, row * p.ld_q + k_column);
+      next_k[e] = load(p.k, row * p.ld_k + k_column);
+      __builtin_amdgcn_sched_barrier(0);  // one after another: f32 values of all of them do not fit
     }
 #pragma unroll
     for (int e = 0; e < kValueLoads; ++e) {
-      if (with_others) next_v[e] = load(p.v, (row0 + min(my_value_row + e * kValueStep, last)) * p.ld_v + v_column);
-      if (!PLAIN) __builtin_amdgcn_sched_barrier(0);
+      next_v[e] = load(p.v, (row0 + min(my_value_row + e * kValueStep, last)) * p.ld_v + v_column);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Behind the last chunk: values that nobody reads, so that the registers are known to be free until the next ones are asked for.
-  auto ask_nothing = [&](bool with_queries, bool with_others) __attribute__((always_inline)) {
+  auto ask_nothing = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < kKeyLoads; ++e) {
-      if (OUT && with_queries) next_q[e] = u32x4{};
-      if (with_others) next_k[e] = u32x4{};
+      if constexpr (OUT) next_q[e] = u32x4{};
+      next_k[e] = u32x4{};
     }
 #pragma unroll
-    for (int e = 0; e < kValueLoads; ++e)
-      if (with_others) next_v[e] = u32x4{};
+    for (int e = 0; e < kValueLoads; ++e) next_v[e] = u32x4{};
   };
-  ask(0, true, true);
+  ask(0);
 
   // ---- the decays -----------------------------------------------------------------------------------------------------
   // A token a lane: asked for two chunks ahead, made ready one ahead, by the team's last wavefront.
@@ -268,15 +294,24 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
     const float units = log * (1.44269504f * 256.0f), whole_units = floorf(units);
     const int64_t g = wave_scan(static_cast<int64_t>(static_cast<int>(whole_units)) << 32 | static_cast<uint32_t>((units - whole_units) * 0x1p32f));
     const float high = static_cast<float>(static_cast<int>(g >> 32)) * 0x1p-8f, rest = static_cast<float>(static_cast<uint32_t>(g)) * 0x1p-40f;
-    auto last = [](float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), kWave - 1)); };
-    const float last_high = last(high), last_rest = last(rest);
+    auto of = [](float x, int token) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), token)); };
+    const float last_high = of(high, kWave - 1), last_rest = of(rest, kWave - 1);
     // No update at all: an exponent far below; a NaN of a logarithm or a weight is all that is left of a column.
     const float column = rest - (weight == 1.0f ? 0.0f : fmaxf(__builtin_amdgcn_logf(weight), -1e5f)) + (log - log);
     if constexpr (OUT) {
-      const float row = rest + log_scale;
-      t.high[lane] = high;
-      t.row[lane] = row;
-      t.column[lane] = column;
+      const float row = rest + log_scale, half_high = of(high, 31), half_rest = of(rest, 31);
+      const float from_high = lane < 32 ? 0.0f : half_high, from_rest = lane < 32 ? 0.0f : half_rest, most = weight == weight ? fmaxf(weight, 1.0f) : 1.0f;
+      const bool quick = half_high > -24.0f && last_high - half_high > -24.0f && __all(most < 0x1p60f);
+      if (quick) {
+        t.row[lane] = __builtin_amdgcn_exp2f((high - from_high) + (row - from_rest)) * (scaled ? 1.0f : p.scale);
+        t.column[lane] = __builtin_amdgcn_exp2f((from_high - high) + (from_rest - column));
+        t.other[lane] = __builtin_amdgcn_exp2f((half_high - high) + (half_rest - column));
+      } else {
+        t.row[lane] = row;
+        t.column[lane] = column;
+        t.other[lane] = high;
+      }
+      if (lane == 0) t.quick = quick;
       t.seen[lane] = __builtin_amdgcn_exp2f(high + row) * (scaled ? 1.0f : p.scale);
     }
     t.update[lane] = __builtin_amdgcn_exp2f((last_high - high) + (last_rest - column));
@@ -323,23 +358,23 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
     return place;
   };
   const int key_place = tile_place<L::kKeyPitch>(my_key_row, my_key / 8), value_place = tile_place<L::kValuePitch>(my_value_row, my_value);
-  auto put = [&](int chunk, bool with_queries, bool with_others) __attribute__((always_inline)) {
+  auto put = [&](int chunk) __attribute__((always_inline)) {
     const int m = min(kChunk, rows - chunk * kChunk);
     auto all = [&](auto in) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < kKeyLoads; ++e) {
         const bool there = in(my_key_row + e * kKeyStep < m && my_key_in);
         const int at = tile_place<L::kKeyPitch>(key_place, e * kKeyStep, 0);
-        if (OUT && with_queries) *reinterpret_cast<u32x4*>(lds + L::kQueries + at) = there ? next_q[e] : u32x4{};
-        if (with_others) *reinterpret_cast<u32x4*>(lds + L::kKeys + at) = there ? next_k[e] : u32x4{};
+        if constexpr (OUT) *reinterpret_cast<u32x4*>(lds + L::kQueries + at) = there ? next_q[e] : u32x4{};
+        *reinterpret_cast<u32x4*>(lds + L::kKeys + at) = there ? next_k[e] : u32x4{};
       }
 #pragma unroll
       for (int e = 0; e < kValueLoads; ++e) {
         const bool there = in(my_value_row + e * kValueStep < m && my_value_in);
-        if (with_others) *reinterpret_cast<u32x4*>(lds + L::kValues + tile_place<L::kValuePitch>(value_place, e * kValueStep, 0)) = there ? next_v[e] : u32x4{};
+        *reinterpret_cast<u32x4*>(lds + L::kValues + tile_place<L::kValuePitch>(value_place, e * kValueStep, 0)) = there ? next_v[e] : u32x4{};
       }
     };
-    if (m == kChunk && whole_tiles) all([](bool) { return true; });
+    if (PLAIN || (m == kChunk && whole_tiles)) all([](bool) { return true; });
     else all([](bool in) { return in; });
   };
   // Where the lane's first reads lie: row n of the keys (and queries), the columns of the keys and of its values, row n of the weights.
@@ -347,123 +382,174 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
   const int key_column = across_place<L::kKeyPitch>(0), value_column = across_place<L::kValuePitch>(32 * wave);
   const int weight_row = L::kWeights + team * L::kWeightBytes + 64 * n + 16 * (n >> 2 & 3);
   auto values_across = [&](int k) { return across<L::kValuePitch>(lds, L::kValues, value_column, k, 0); };
-  const int64_t columns = static_cast<int64_t>(head) * p.dv + column0 + 32 * mate;  // the lane's outputs of a row: 16 a + 8 h .. from here on
-  const int my_column = column0 + 32 * mate + 8 * h;
-  const int out_place = static_cast<int>(n * p.ld_out + 8 * h), gate_place = static_cast<int>(n * p.ld_gate + 8 * h);
+  const int my_column = column0 + 32 * mate + 8 * h;  // the lane's outputs of a row: 16 a .. from here on
+  const int out_place = static_cast<int>(n * p.ld_out) + my_column, gate_place = 2 * (static_cast<int>(n * p.ld_gate) + my_column);
 
   if (counts) {
     put_decay(0);
     ask_decay(1);
   }
-  put(0, true, true);
+  put(0);
   __syncthreads();
   for (int chunk = 0; chunk < chunks; ++chunk) {
     const Tokens& t = tokens[chunk % 2];
     const int m = min(kChunk, rows - chunk * kChunk);
     const bool more = chunk + 1 < chunks, two = m > 32;
     const int64_t row0 = first_row + static_cast<int64_t>(chunk) * kChunk;
-    // Queries of the next chunk first, they are put in LDS first; keys and values when the state's products have left their registers.
-    if (more) ask(chunk + 1, true, !OUT);
-    else ask_nothing(true, !OUT);
-    __builtin_amdgcn_sched_barrier(0);
+    auto ask_next = [&]() __attribute__((always_inline)) {
+      if (PLAIN || more) ask(chunk + 1);
+      else ask_nothing();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (!OUT) ask_next();
     f32x16 out[2] = {};
     if constexpr (OUT) {
-      // Weights, in tiles of 32 rows by 32 tokens: (0, 0), (1, 0), (1, 1). Their products here, what is made of them between the products of the
-      // state, which are half as many instructions of the matrix cores as they need of the vector unit.
+      // Weights, in tiles of 32 rows by 32 tokens: (0, 0), (1, 0), (1, 1).
       const int from = now(key_row), to = now(weight_row), here = now(n);  // compared anew: kept, the results cost more scalar registers than there are
-      auto raw_weights = [&](int block, f32x16& w) __attribute__((always_inline)) {
-        const int keys_at = L::kKeys + (block == 2) * 32 * L::kKeyPitch, queries_at = L::kQueries + (block > 0) * 32 * L::kKeyPitch;
-        w = f32x16{};
-#pragma unroll
-        for (int k = 0; k < DK / 16; ++k) {
-          w = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_at(lds, keys_at + (from ^ 32 * k)), eight_at(lds, queries_at + (from ^ 32 * k)), w, 0, 0, 0);
-          if (k % 2) __builtin_amdgcn_sched_barrier(0);  // no more reads ahead than registers
-        }
+      auto put_weights = [&](int block, int g, const float (&v)[4]) __attribute__((always_inline)) {
+        u32x2 high, low;
+        uint32_t x, y;
+        split_two<false>(v[0], v[1], x, y);
+        high.x = x, low.x = y;
+        split_two<false>(v[2], v[3], x, y);
+        high.y = x, low.y = y;
+        uint8_t* const at = lds + block * L::kBlock + (to ^ 16 * g) + 8 * h;
+        *reinterpret_cast<u32x2*>(at) = high;
+        *reinterpret_cast<u32x2*>(at + 3 * L::kBlock) = low;
       };
-      // Tokens 8 g + 4 h .. + 3 of the tile's.
-      auto weigh = [&](int block, const f32x16& w, int g) __attribute__((always_inline)) {
-        const int jb = block == 2, ib = block > 0, until = jb == ib ? here : 32, own = jb == ib ? here : -1;
-        const float high = t.high[32 * ib + n], row = t.row[32 * ib + n];
-        const int token = 8 * g + 4 * h;
-        const f32x4 highs = *reinterpret_cast<const f32x4*>(t.high + 32 * jb + token), columns = *reinterpret_cast<const f32x4*>(t.column + 32 * jb + token);
+      // Tokens 8 g + 4 h .. + 3 of the tile's. `kind`: the tile is one on the diagonal (1), the one below it (0), or either (2).
+      auto weigh = [&](auto kind, int block, const f32x16& w, int g) __attribute__((always_inline)) {
+        constexpr int kKind = decltype(kind)::value;
+        const int token = 8 * g + 4 * h, jb = block == 2;
+        const float row = t.row[32 * (block > 0) + n];
+        const f32x4 columns = *reinterpret_cast<const f32x4*>((kKind == 1 || (kKind == 2 && block != 1) ? t.column + 32 * jb : t.other) + token);
+        const int until = kKind == 2 && block == 1 ? 32 : here;
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = w[4 * g + e] * __builtin_amdgcn_exp2f((high - highs[e]) + (row - columns[e]));
-          if (!scaled) v[e] *= p.scale;
-          v[e] = token + e <= until ? v[e] : 0.0f;
-          v[e] += token + e == own ? skip : 0.0f;
+          v[e] = w[4 * g + e] * row * columns[e];
+          if (kKind != 0) v[e] = token + e <= until ? v[e] : 0.0f;
         }
-        const uint32_t a = __builtin_bit_cast(uint32_t, pack_bf16(v[0], v[1])), b = __builtin_bit_cast(uint32_t, pack_bf16(v[2], v[3]));
-        const u32x2 left = {__builtin_bit_cast(uint32_t, pack_bf16(v[0] - __uint_as_float(a << 16), v[1] - __uint_as_float(a & 0xffff0000u))),
-                            __builtin_bit_cast(uint32_t, pack_bf16(v[2] - __uint_as_float(b << 16), v[3] - __uint_as_float(b & 0xffff0000u)))};
-        uint8_t* const at = lds + block * L::kBlock + (to ^ 16 * g) + 8 * h;
-        *reinterpret_cast<u32x2*>(at) = u32x2{a, b};
-        *reinterpret_cast<u32x2*>(at + 3 * L::kBlock) = left;
+        put_weights(block, g, v);
       };
-      // What the rows see of the state, a step's queries and halves of the state made ready one ahead; `blocks`: tiles of weights that the wavefront
-      // makes meanwhile, the first one tile `block`.
-      auto see = [&](auto blocks, int block) __attribute__((always_inline)) {
-        constexpr int kTiles = decltype(blocks)::value, kSteps = DK / 16;
-        f32x16 w;
-        if constexpr (kTiles > 0) raw_weights(block, w);
-        bf16x8 q[2][2], high[2], low[2];
-        auto ready = [&](int k) __attribute__((always_inline)) {
-          q[k % 2][0] = eight_at(lds, L::kQueries + (from ^ 32 * k));
-          q[k % 2][1] = eight_at(lds, L::kQueries + 32 * L::kKeyPitch + (from ^ 32 * k));
+      // The same from differences, a tile at a time.
+      auto weigh_far = [&](int block) __attribute__((always_inline)) {
+        const int jb = block == 2, ib = block > 0, until = jb == ib ? here : 32;
+        f32x16 w = {};
+#pragma unroll
+        for (int k = 0; k < DK / 16; ++k) {
+          w = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_at(lds, L::kKeys + jb * 32 * L::kKeyPitch + (from ^ 32 * k)),
+                                                      eight_at(lds, L::kQueries + ib * 32 * L::kKeyPitch + (from ^ 32 * k)), w, 0, 0, 0);
+          if (k % 2) __builtin_amdgcn_sched_barrier(0);  // no more reads ahead than registers
+        }
+        const float high = t.other[32 * ib + n], row = t.row[32 * ib + n];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int token = 8 * g + 4 * h;
+          const f32x4 highs = *reinterpret_cast<const f32x4*>(t.other + 32 * jb + token), columns = *reinterpret_cast<const f32x4*>(t.column + 32 * jb + token);
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = w[4 * g + e] * __builtin_amdgcn_exp2f((high - highs[e]) + (row - columns[e])) * (scaled ? 1.0f : p.scale);
+            v[e] = token + e <= until ? v[e] : 0.0f;
+          }
+          put_weights(block, g, v);
+        }
+      };
+      // The skip, added to the rows' weights of their own tokens.
+      auto add_skip = [&](int block) __attribute__((always_inline)) {
+        if (h != (n >> 2 & 1)) return;
+        asm volatile("" ::: "memory");  // written as other types
+        uint16_t* const at = reinterpret_cast<uint16_t*>(lds + block * L::kBlock + (to ^ 16 * (n >> 3)) + 8 * h + 2 * (n & 3));
+        uint32_t high, low;
+        split_two<false>(bf16_bits_to_f32(at[0]) + bf16_bits_to_f32(at[3 * L::kBlock / 2]) + skip, 0.0f, high, low);
+        at[0] = static_cast<uint16_t>(high);
+        at[3 * L::kBlock / 2] = static_cast<uint16_t>(low);
+      };
+      // What the rows see of the state, and the products of `kTiles` tiles of weights, which read the same queries; a step's operands are made ready one
+      // ahead. `block`: the first tile (two: (0, 0) and (1, 0), of the same keys).
+      auto see = [&](auto tiles, int block) __attribute__((always_inline)) {
+        constexpr int kTiles = decltype(tiles)::value, kSteps = DK / 16;
+        f32x16 w[2] = {};
+        bf16x8 q[2][2], k[2], high[2], low[2];
+        const int keys_at = L::kKeys + (kTiles == 1 && block == 2) * 32 * L::kKeyPitch;
+        auto ready = [&](int step) __attribute__((always_inline)) {
+          const int now = step % 2;
+          q[now][0] = eight_at(lds, L::kQueries + (from ^ 32 * step));
+          q[now][1] = eight_at(lds, L::kQueries + 32 * L::kKeyPitch + (from ^ 32 * step));
+          if constexpr (kTiles > 0) k[now] = eight_at(lds, keys_at + (from ^ 32 * step));
           float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = state[k / 2][k % 2 * 8 + e];
-          split_eight(v, high[k % 2], low[k % 2]);
+          for (int e = 0; e < 8; ++e) v[e] = state[step / 2][step % 2 * 8 + e];
+          split_eight<true>(v, high[now], low[now]);
         };
         ready(0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          if (k + 1 < kSteps) ready(k + 1);
-          out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high[k % 2], q[k % 2][0], out[0], 0, 0, 0);
-          out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high[k % 2], q[k % 2][1], out[1], 0, 0, 0);
-          out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low[k % 2], q[k % 2][0], out[0], 0, 0, 0);
-          out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low[k % 2], q[k % 2][1], out[1], 0, 0, 0);
-#pragma unroll
-          for (int g = 4 * kTiles * k / kSteps; g < 4 * kTiles * (k + 1) / kSteps; ++g) weigh(block + g / 4, w, g % 4);
+        for (int step = 0; step < kSteps; ++step) {
+          const int now = step % 2;
+          if (step + 1 < kSteps) ready(step + 1);
+          out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high[now], q[now][0], out[0], 0, 0, 0);
+          out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high[now], q[now][1], out[1], 0, 0, 0);
+          if constexpr (kTiles == 2) w[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[now], q[now][0], w[0], 0, 0, 0);
+          if constexpr (kTiles == 2) w[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[now], q[now][1], w[1], 0, 0, 0);
+          if constexpr (kTiles == 1) {
+            if (block == 0) w[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[now], q[now][0], w[0], 0, 0, 0);
+            else w[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[now], q[now][1], w[0], 0, 0, 0);
+          }
+          out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low[now], q[now][0], out[0], 0, 0, 0);
+          out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low[now], q[now][1], out[1], 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
-          if (kTiles > 1 && 2 * (k + 1) == kSteps) raw_weights(block + 1, w);
+        }
+        if constexpr (kTiles > 0) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            if (TW == 4) weigh(std::integral_constant<int, 2>(), block, w[0], g);
+            else weigh(std::integral_constant<int, 1>(), block, w[0], g);
+            if constexpr (kTiles > 1) weigh(std::integral_constant<int, 0>(), 1, w[1], g);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
       };
-      if (TW == 2 ? mate == 0 && two : false) see(std::integral_constant<int, TW == 2 ? 2 : 0>(), 0);
-      else if (mate == 0 || (mate < 3 && two)) see(std::integral_constant<int, 1>(), TW == 2 ? 2 * mate : mate);
-      else see(std::integral_constant<int, 0>(), 0);
+      // Of two wavefronts a head the first one makes tiles (0, 0) and (1, 0), the other, which has the decays, (1, 1); of four the first three one each.
+      const int block = TW == 2 ? 2 * mate : mate;
+      const bool makes = mate == 0 || (mate < 3 && two);
+      if (!__builtin_amdgcn_readfirstlane(t.quick)) {
+        if (makes) weigh_far(block);
+        if (TW == 2 && mate == 0 && two) weigh_far(1);
+        see(std::integral_constant<int, 0>(), 0);
+      } else if (TW == 2 && mate == 0 && two) {
+        see(std::integral_constant<int, TW == 2 ? 2 : 0>(), 0);
+      } else if (makes) {
+        see(std::integral_constant<int, 1>(), block);
+      } else {
+        see(std::integral_constant<int, 0>(), 0);
+      }
+      if (p.skip && makes && block != (TW == 2 ? -1 : 1)) add_skip(block);
 #pragma unroll
       for (int i = 0; i < 2; ++i) out[i] *= t.seen[32 * i + n];
     }
-    // Gates are asked for here: earlier, they would take registers from what went before.
-    u32x4 gate[2][2];
-    if (OUT && PLAIN && p.gate) {
-      const unsigned gate_from = now(gate_place);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          gate[i][a] = u32x4{};
-          if (32 * i + n < m && my_column + 16 * a < p.dv)
-            gate[i][a] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.gate) + (row0 + 32 * i) * p.ld_gate + columns + 16 * a + gate_from);
-        }
-    }
-    if (OUT && more) ask(chunk + 1, false, true);
-    else if (OUT) ask_nothing(false, true);
-    __builtin_amdgcn_sched_barrier(0);
     if (counts && more) {
       put_decay(chunk + 1);
       ask_decay(chunk + 2);
     }
+    // Gates are asked for here: earlier, they would take registers from what went before.
+    u32x4 gate[2][2];
+    if (OUT && PLAIN && p.gate) {
+      const unsigned from = now(gate_place);
+      const auto g = buffer_of(static_cast<const uint16_t*>(p.gate) + row0 * p.ld_gate + static_cast<int64_t>(head) * p.dv, rows_bytes(m, p.ld_gate, p.dv, 2));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) gate[i][a] = buffer_load(g, from + i * static_cast<unsigned>(64 * p.ld_gate) + 32 * a);
+    }
+    if constexpr (OUT) ask_next();  // not before the products of the state have left their registers
     if constexpr (OUT) __syncthreads();
 
     bf16x8 v[kChunk / 16];
 #pragma unroll
     for (int k = 0; k < kChunk / 16; ++k) v[k] = values_across(k);
     if constexpr (OUT) {
-      if (more) put(chunk + 1, true, false);  // nobody reads this chunk's queries any more
       // A weight of nothing times an infinity or a NaN of a later token is no number: those are taken out of the product, and what rows behind
       // them see of them is added by itself.
       float odd[2] = {};
@@ -522,40 +608,55 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
 #pragma unroll
         for (int k = 0; k < kChunk / 16; ++k) v[k] = values_across(k);
       }
-      if (!idle) {
-        const unsigned out_from = now(out_place), gate_from = now(gate_place);
+      if constexpr (PLAIN) {
+        const bool half = p.out_type == LX_BF16;
+        const int size = half ? 2 : 4;
+        const auto to = buffer_of(static_cast<char*>(p.out) + (row0 * p.ld_out + static_cast<int64_t>(head) * p.dv) * size, idle ? 0 : rows_bytes(m, p.ld_out, p.dv, size));
+        const unsigned from = now(out_place);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = out[i][8 * a + e];
+            if (p.gate) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t pair = gate[i][a][e / 2];
+                o[e] *= gate_of(__uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16));
+              }
+            }
+            const unsigned at = my_column + 16 * a < p.dv ? (from + i * static_cast<unsigned>(32 * p.ld_out) + 16 * a) * size : kOutside;
+            if (half) {
+              buffer_store(to, at, u32x4{__builtin_bit_cast(uint32_t, pack_bf16(o[0], o[1])), __builtin_bit_cast(uint32_t, pack_bf16(o[2], o[3])),
+                                         __builtin_bit_cast(uint32_t, pack_bf16(o[4], o[5])), __builtin_bit_cast(uint32_t, pack_bf16(o[6], o[7]))});
+            } else {
+              buffer_store(to, at, u32x4{__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3])});
+              buffer_store(to, at + 16, u32x4{__float_as_uint(o[4]), __float_as_uint(o[5]), __float_as_uint(o[6]), __float_as_uint(o[7])});
+            }
+          }
+      } else if (!idle) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (32 * i + n >= m) continue;
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
             if (my_column + 16 * a >= p.dv) continue;
-            const int64_t at = (row0 + 32 * i) * p.ld_out + columns + 16 * a;
+            const int64_t column_at = static_cast<int64_t>(head) * p.dv + my_column + 16 * a, row = row0 + 32 * i + n;
             float o[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = out[i][8 * a + e];
-            if (PLAIN && p.gate) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const uint32_t pair = gate[i][a][e / 2];
-                o[e] *= gate_of(__uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16));
-              }
-            } else if (p.gate) {
+            if (p.gate) {
 #pragma unroll
               for (int e = 0; e < 8; e += 4) {
-                const f32x4 z = load_four(p.gate, p.gate_type, p.wide, (row0 + 32 * i) * p.ld_gate + columns + 16 * a + gate_from + e);
+                const f32x4 z = load_four(p.gate, p.gate_type, p.wide, row * p.ld_gate + column_at + e);
 #pragma unroll
                 for (int f = 0; f < 4; ++f) o[e + f] *= gate_of(z[f]);
               }
             }
-            if ((PLAIN || p.wide) && p.out_type == LX_BF16) {
-              const u32x4 packed = {__builtin_bit_cast(uint32_t, pack_bf16(o[0], o[1])), __builtin_bit_cast(uint32_t, pack_bf16(o[2], o[3])),
-                                    __builtin_bit_cast(uint32_t, pack_bf16(o[4], o[5])), __builtin_bit_cast(uint32_t, pack_bf16(o[6], o[7]))};
-              *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out) + at + out_from) = packed;
-            } else {
-              store_four(p.out, PLAIN ? LX_F32 : p.out_type, PLAIN || p.wide, at + out_from, f32x4{o[0], o[1], o[2], o[3]});
-              store_four(p.out, PLAIN ? LX_F32 : p.out_type, PLAIN || p.wide, at + out_from + 4, f32x4{o[4], o[5], o[6], o[7]});
-            }
+            store_four(p.out, p.out_type, p.wide, row * p.ld_out + column_at, f32x4{o[0], o[1], o[2], o[3]});
+            store_four(p.out, p.out_type, p.wide, row * p.ld_out + column_at + 4, f32x4{o[4], o[5], o[6], o[7]});
           }
         }
       }
@@ -579,7 +680,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
           const uint32_t pair = raw[e / 2];
           x[e] = __uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16) * (e < 4 ? w0[e % 4] : w1[e % 4]);
         }
-        split_eight(x, high[k % 2], low[k % 2]);
+        split_eight<false>(x, high[k % 2], low[k % 2]);
       };
       ready(0);
 #pragma unroll
@@ -597,7 +698,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
     }
     __syncthreads();
     if (more) {
-      put(chunk + 1, false, true);
+      put(chunk + 1);
       __syncthreads();
     }
   }

@@ -360,7 +360,7 @@ typedef struct {
  *   LX_DECAY_HEAD  g = rate[h], b = 1
  *   LX_DECAY_LOG   g = x[t, h] * rate[h] (rate null: 1), b = 1
  *   LX_DECAY_STEP  d = log(1 + exp(x[t, h] + bias[h])) (bias null: 0), g = d * rate[h] (rate null: -1), b = d
- * q, k and v all bf16 or all f32 (rounded to bf16, as lx_gemm_w's BF16 math does), out f32 or bf16, row strides in elements, up to 2^24; states f32
+ * q, k and v all bf16 or all f32 (rounded to bf16, as lx_gemm_w's BF16 math does), out f32 or bf16, row strides in elements, up to 2^22; states f32
  * [count, heads, dk, dv], 16-byte aligned, or null. Calls of few rows a sequence go token by token in f32, longer ones by
  * chunks of 64 tokens on the matrix cores: there f32 factors (weights of tokens, values times their decay, the state) enter products as two
  * bf16 (16 bits are kept) and sums are f32. Neither form's bits depend on the other sequences of the call; which form a call takes depends on max_rows, and where

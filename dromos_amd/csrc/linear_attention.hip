@@ -55,7 +55,7 @@ Cut cut_of(int T, int max_rows, int heads, int k_heads, int dk, int dv) {
   return c;
 }
 
-int64_t sum_bytes(const Cut& c, int heads, int dk, int dv) { return 4 * static_cast<int64_t>(c.places) * heads * dk * dv; }
+int64_t sum_bytes(const Cut& c, int heads, int dk, int dv) { return 4 * static_cast<int64_t>(c.places) * heads * part_values(dk, dv); }
 
 template <int DK, int TW, int TEAMS, bool OUT>
 int launch_chunks(ChunkArgs a, int64_t numbers, hipStream_t s) {
@@ -77,7 +77,7 @@ int chunks_of(const ChunkArgs& a, hipStream_t s) {
   if (!a.single) {
     const int64_t places = 2 * static_cast<int64_t>(b.T / a.size);
     if (int st = launch_chunks<DK, TW, TEAMS, false>(a, places, s)) return st;
-    const int64_t fours = static_cast<int64_t>(a.l.heads) * a.l.dk * a.l.dv / 4, groups = (fours + 255) / 256 * (places / 2);
+    const int64_t fours = a.l.heads * part_values(a.l.dk, a.l.dv) / 4, groups = (fours + 255) / 256 * (places / 2);
     if (groups * 256 > kMaxGridThreads) return kInvalid;
     hipLaunchKernelGGL(linear_parts_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, a);
     if (int st = status_of(hipGetLastError())) return st;

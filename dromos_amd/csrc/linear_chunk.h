@@ -39,9 +39,15 @@ struct ChunkArgs {
   int single;       // no sequence has more than one part
   int64_t numbers;  // of parts that the launch counts to
   int across;       // workgroups of a part and key head
-  float* sums;      // [2 (T / size)] states [heads, dk, dv]: parts' sums, then the states in front of them
+  float* sums;      // [2 (T / size), heads] states as wavefronts hold them: parts' sums, then the states in front of them
   double* logs;     // [2 (T / size), heads] logarithms of what the parts leave of what was in front of them
 };
+
+// A state as the wavefronts' registers hold it, for the parts of long sequences: columns by 32s, rows by 32s, then four registers by four of all
+// lanes (as rows and columns, a lane's values would be 64 loads of four bytes: 4 us of a part's 45).
+__host__ __device__ __forceinline__ int64_t part_values(int dk, int dv) { return static_cast<int64_t>(dk <= 64 ? 64 : dk <= 128 ? 128 : 256) * ((dv + 31) / 32 * 32); }
+// Lane n's column of 32.
+__device__ __forceinline__ int lane_column(int n) { return n / 16 * 16 + (n % 4 | n / 4 % 2 * 8 | n / 8 % 2 * 4); }
 
 // Where 16-byte unit `unit` of row `row` lies in a tile of rows of `kPitch` bytes (128, 256 or 512): its place in the row is turned by the row's low bits, so
 // that sixteen rows' units of one place fall on all banks, and so do four neighbouring rows' of four neighbouring places.
@@ -212,7 +218,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
   const int column0 = TEAMS > 1 ? 0 : beside % blocks * 32 * TW;
   const int head = min(head0 + team, head_end - 1);
   const bool idle = head0 + team >= head_end;
-  const int column = column0 + 32 * mate + (n / 16 * 16 + (n % 4 | n / 4 % 2 * 8 | n / 8 % 2 * 4));  // the lane's of the state
+  const int column = column0 + 32 * mate + lane_column(n);  // the lane's of the state
   const int64_t first_row = static_cast<int64_t>(span.row0) + begin;
   const int rows = end - begin, chunks = (rows + kChunk - 1) / kChunk;
 
@@ -341,11 +347,17 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
         for (int r = 0; r < 8; ++r) use((row + static_cast<int64_t>(r) * p.dv)[state_from], t, 8 * a + r);
       }
   };
-  if constexpr (OUT) {
-    float* from = nullptr;
-    if (split) from = c.sums + (place * p.heads + head) * state_size;
-    else if (p.states.in && slot >= 0 && !span.begins) from = const_cast<float*>(static_cast<const float*>(p.states.in)) + (static_cast<int64_t>(slot) * p.heads + head) * state_size;
-    if (from) each_state(from, [&](float& x, int t, int r) { state[t][r] = x; });
+  f32x4* const part = reinterpret_cast<f32x4*>(c.sums + (place * p.heads + head) * part_values(p.dk, p.dv)) + (column0 / 32 + mate) * (DK / 32 * 4 * kWave);
+  if (OUT && split && column0 + 32 * mate < p.dv) {
+#pragma unroll
+    for (int i = 0; i < DK / 8; ++i) {
+      const f32x4 four = part[i * kWave + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) state[i / 4][i % 4 * 4 + e] = four[e];
+    }
+  } else if (OUT && !split && p.states.in && slot >= 0 && !span.begins) {
+    float* const from = const_cast<float*>(static_cast<const float*>(p.states.in)) + (static_cast<int64_t>(slot) * p.heads + head) * state_size;
+    each_state(from, [&](float& x, int t, int r) { state[t][r] = x; });
   }
   const float skip = p.skip ? p.skip[head] : 0.0f;
   double part_log = 0.0;
@@ -703,35 +715,43 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
     }
   }
 
-  float* to = nullptr;
   if constexpr (OUT) {
-    if (p.states.out && slot >= 0 && end == span.stop) to = static_cast<float*>(p.states.out) + (static_cast<int64_t>(slot) * p.heads + head) * state_size;
-  } else {
-    to = c.sums + (place * p.heads + head) * state_size;
-    if (!idle && mate == 0 && lane == 0 && column0 == 0) c.logs[place * p.heads + head] = part_log;
+    if (p.states.out && slot >= 0 && end == span.stop)
+      each_state(static_cast<float*>(p.states.out) + (static_cast<int64_t>(slot) * p.heads + head) * state_size, [&](float& x, int t, int r) { x = state[t][r]; });
+  } else if (!idle && column0 + 32 * mate < p.dv) {
+#pragma unroll
+    for (int i = 0; i < DK / 8; ++i) part[i * kWave + lane] = f32x4{state[i / 4][i % 4 * 4], state[i / 4][i % 4 * 4 + 1], state[i / 4][i % 4 * 4 + 2], state[i / 4][i % 4 * 4 + 3]};
+    if (mate == 0 && lane == 0 && column0 == 0) c.logs[place * p.heads + head] = part_log;
   }
-  if (to) each_state(to, [&](float& x, int t, int r) { x = state[t][r]; });
 }
 
 // The states in front of a long sequence's parts, where their sums were: four values a thread, all parts in order.
 __global__ void __launch_bounds__(256) linear_parts_kernel(const ChunkArgs c) {
   const LinearArgs& p = c.l;
-  const int64_t state_size = static_cast<int64_t>(p.dk) * p.dv, fours = p.heads * state_size / 4;
-  const int64_t groups = (fours + 255) / 256;
+  const int64_t part_size = part_values(p.dk, p.dv), fours = p.heads * part_size / 4;
+  const unsigned groups = static_cast<unsigned>((fours + 255) / 256);
   int s, j;
   if (!mix_find_long(p.b, c.size, 2 * (blockIdx.x / groups), s, j) || j != 0) return;
   const MixSpan span = mix_span(p.b, s);
   if (span.stop <= c.size) return;
-  const int64_t i = blockIdx.x % groups * 256 + threadIdx.x;
+  const int64_t i = static_cast<int64_t>(blockIdx.x % groups) * 256 + threadIdx.x;
   if (i >= fours) return;
-  const int head = static_cast<int>(4 * i / state_size), parts = (span.stop + c.size - 1) / c.size;
+  const int head = static_cast<int>(4 * i / part_size), of_head = static_cast<int>(i - head * (part_size / 4)), parts = (span.stop + c.size - 1) / c.size;
   const int64_t place = 2 * static_cast<int64_t>(span.row0 / c.size);
   const int slot = mix_slot(p.states, s);
   f32x4 state = {};
-  if (p.states.in && slot >= 0 && !span.begins) state = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p.states.in) + static_cast<int64_t>(slot) * p.heads * state_size + 4 * i);
-  const int skipped = min(span.first / c.size, parts);  // parts in front of position 0 have left no sum
-  for (int k = skipped; k < parts; ++k) {
-    f32x4* const at = reinterpret_cast<f32x4*>(c.sums + (place + k) * p.heads * state_size + 4 * i);
+  if (p.states.in && slot >= 0 && !span.begins) {
+    // Four neighbouring rows of a column.
+    const int lane = of_head % kWave, quad = of_head / kWave % 4, tiles = p.dk <= 64 ? 2 : p.dk <= 128 ? 4 : 8, t = of_head / kWave / 4 % tiles;
+    const int row = 32 * t + quad / 2 * 16 + lane / 32 * 8 + quad % 2 * 4, column = of_head / kWave / 4 / tiles * 32 + lane_column(lane % 32);
+    const float* const from = static_cast<const float*>(p.states.in) + ((static_cast<int64_t>(slot) * p.heads + head) * p.dk + row) * p.dv + column;
+    if (row < p.dk && column < p.dv) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) state[e] = from[e * p.dv];
+    }
+  }
+  for (int k = span.first / c.size; k < parts; ++k) {  // parts in front of position 0 have left no sum
+    f32x4* const at = reinterpret_cast<f32x4*>(c.sums + (place + k) * p.heads * part_size) + i;
     const f32x4 before = state;
     if (k + 1 < parts) {
       const f32x4 sum = *at;

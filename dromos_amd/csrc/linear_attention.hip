@@ -34,7 +34,7 @@ struct Cut {
   int size, places;  // rows of a part; parts of long sequences there may be
 };
 
-constexpr int kLeastPart = 256;
+constexpr int kLeastPart = 128;
 
 Cut cut_of(int T, int max_rows, int heads, int k_heads, int dk, int dv) {
   Cut c;

@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
   span.row0 = __builtin_amdgcn_readfirstlane(span.row0), span.first = __builtin_amdgcn_readfirstlane(span.first);
   span.stop = __builtin_amdgcn_readfirstlane(span.stop), span.begins = __builtin_amdgcn_readfirstlane(span.begins);
   const int begin = max(span.first, j * c.size), end = min(span.stop, (j + 1) * c.size);
-  const bool split = span.stop > c.size;
+  // A sequence whose parts have not all been found (its rows do not ascend) has left no states between them.
+  const bool split = span.stop > c.size && (!OUT || mix_all_found(p.b, c.size, s, span));
   if (begin >= end || (!OUT && (!split || end == span.stop))) return;
   // A sequence's part has a place of its own: those of more than one part are more than `size` rows each.
   const int64_t place = 2 * static_cast<int64_t>(span.row0 / c.size) + j;
@@ -733,7 +734,7 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const ChunkArgs c) {
   int s, j;
   if (!mix_find_long(p.b, c.size, 2 * (blockIdx.x / groups), s, j) || j != 0) return;
   const MixSpan span = mix_span(p.b, s);
-  if (span.stop <= c.size) return;
+  if (span.stop <= c.size || !mix_all_found(p.b, c.size, s, span)) return;
   const int64_t i = static_cast<int64_t>(blockIdx.x % groups) * 256 + threadIdx.x;
   if (i >= fours) return;
   const int head = static_cast<int>(4 * i / part_size), of_head = static_cast<int>(i - head * (part_size / 4)), parts = (span.stop + c.size - 1) / c.size;

@@ -92,6 +92,15 @@ __device__ __forceinline__ bool mix_find_long(const MixBatch& b, int size, int64
   return s >= 0 && of <= b.T / size;
 }
 
+// Whether those numbers find all pieces of sequence s, as they do wherever rows ascend: if its first and last ones, then those between them, since a search
+// for a later number never ends in front of one for an earlier one.
+__device__ __forceinline__ bool mix_all_found(const MixBatch& b, int size, int s, const MixSpan& span) {
+  if (b.seqs == 1) return true;
+  auto number = [&](int i) { return 2 * static_cast<int64_t>(mix_clamp(b.rows[i], 0, b.T) / size); };
+  const int64_t first = 2 * static_cast<int64_t>(span.row0 / size);
+  return mix_last(b.seqs, first, number) == s && mix_last(b.seqs, first + (span.stop - 1) / size, number) == s;
+}
+
 struct MixStates {
   const void* in;
   void* out;

@@ -3,8 +3,8 @@
 // Bytes decide: x is read once and y written once. A row's angles are the same for all its heads, so a workgroup makes them
 // once for a few rows (a thread an angle, in 64 bits), leaves cosines and sines in LDS and goes over the rows' heads, PAIRS pairs a lane, the
 // next ones on their way meanwhile. A call of few rows has several workgroups a row, each with some of the heads. Rows of 36 heads of 128
-// values bf16, half of each turned, 125 MB read and written together: 32.8 us (3.8 TB/s; 40.3 us with a unit's place divided out anew each time and
-// nothing on its way); 1 row of 40 heads: 3.5 to 4.6 us, a launch and one chain of loads.
+// values bf16, half of each turned, 125 MB read and written together: 28.4 us (4.4 TB/s; 40.3 us with a unit's place divided out anew each time and
+// nothing on its way; two units on their way 29.7); 1 row of 40 heads: 3.4 to 4.2 us, a launch and one chain of loads.
 #include <cmath>
 
 #include "mixer.h"
@@ -121,21 +121,6 @@ __global__ void __launch_bounds__(256) rotate_kernel(const RotateArgs p) {
   const int64_t first = static_cast<int64_t>(blockIdx.x / p.parts) * p.rows;
   const int part = blockIdx.x % p.parts, half = p.rot / 2;
   const int rows = static_cast<int>(p.T - first < p.rows ? p.T - first : p.rows);
-  for (int r = threadIdx.x / kWave; r < rows; r += 256 / kWave) {  // every lane of a wavefront alike
-    int position = 0;
-    const bool in = position_of(p, static_cast<int>(first) + r, position);
-    if (threadIdx.x % kWave == 0) found[r] = in, place[r] = position;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * half; i += 256) {
-    const int r = i / half, n = i % half;
-    const double quarters[1] = {static_cast<double>(p.freq[n]) * 0.63661977236758134308};
-    float c[1], s[1];
-    angles(quarters, place[r], c, s);
-    cosines[i] = c[0] * p.amplitude;
-    sines[i] = s[0] * p.amplitude;
-  }
-  __syncthreads();
   // Unit u of head `head` of row r, 256 units further at each turn; the next one's values on their way meanwhile.
   const int units = (p.dim + 2 * PAIRS - 1) / (2 * PAIRS), turned = half / PAIRS, low = part * p.per, high = min(p.heads, low + p.per);
   const int heads = high - low, all = rows * heads * units;
@@ -156,6 +141,21 @@ __global__ void __launch_bounds__(256) rotate_kernel(const RotateArgs p) {
     b = both ? load_raw<PAIRS>(p.x, p.x_type, row + b_at) : a;
   };
   if (static_cast<int>(threadIdx.x) < all) ask();
+  for (int r = threadIdx.x / kWave; r < rows; r += 256 / kWave) {  // every lane of a wavefront alike
+    int position = 0;
+    const bool in = position_of(p, static_cast<int>(first) + r, position);
+    if (threadIdx.x % kWave == 0) found[r] = in, place[r] = position;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * half; i += 256) {
+    const int r = i / half, n = i % half;
+    const double quarters[1] = {static_cast<double>(p.freq[n]) * 0.63661977236758134308};
+    float c[1], s[1];
+    angles(quarters, place[r], c, s);
+    cosines[i] = c[0] * p.amplitude;
+    sines[i] = s[0] * p.amplitude;
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < all; i += 256) {
     int a_at, b_at;
     const bool both = places(a_at, b_at), turns = u < turned;
@@ -199,10 +199,11 @@ __global__ void __launch_bounds__(256) rotate_kernel(const RotateArgs p) {
 template <int PAIRS>
 int launch(RotateArgs p, hipStream_t s) {
   const int half = p.rot / 2, units = (p.dim + 2 * PAIRS - 1) / (2 * PAIRS);
-  // As many rows a workgroup as have an angle a thread, fewer where that leaves the device short of wavefronts.
+  // As many rows a workgroup as have an angle a thread, fewer where that makes fewer than four workgroups a unit of the device: all of them are there at
+  // once then (6820 rows: 28.4 us; eight workgroups a unit, seven of them at work on average, 31.7 us).
   int rows = half ? 256 / half : kMostRows;
   rows = rows < 1 ? 1 : rows > kMostRows ? kMostRows : rows;
-  const int spread = (p.T + 8 * compute_units() - 1) / (8 * compute_units());
+  const int spread = (p.T + 4 * compute_units() - 1) / (4 * compute_units());
   p.rows = rows < spread ? rows : spread;
   const int64_t groups = (static_cast<int64_t>(p.T) + p.rows - 1) / p.rows;
   // Several workgroups a row where rows are few, a unit a thread at least.

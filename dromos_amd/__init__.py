@@ -7,7 +7,12 @@ calls the library the way the reference's kernel tests call any backend library
 """
 
 from .abi import (  # noqa: F401
+    ACT_NONE,
+    ACT_SILU,
     BF16,
+    DECAY_HEAD,
+    DECAY_LOG,
+    DECAY_STEP,
     DTYPE,
     F32,
     MATH_BF16,
@@ -17,13 +22,20 @@ from .abi import (  # noqa: F401
     NORM_LAYER,
     NORM_RMS,
     NOT_SUPPORTED,
+    ROPE_BASE,
+    ROPE_LINEAR,
+    ROPE_PARTS,
+    ROPE_PLAIN,
+    ROPE_WAVES,
     W_BF16,
     W_FP8,
     W_INT8,
     W_NVFP4,
     Kernels,
+    LxDecay,
     LxKv8,
     LxKv8Batch,
+    LxStates,
     LxWeight,
     hip_library_path,
     load_hip,

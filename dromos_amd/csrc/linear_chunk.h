@@ -751,16 +751,26 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const ChunkArgs c) {
       for (int e = 0; e < 4; ++e) state[e] = from[e * p.dv];
     }
   }
-  for (int k = span.first / c.size; k < parts; ++k) {  // parts in front of position 0 have left no sum
-    f32x4* const at = reinterpret_cast<f32x4*>(c.sums + (place + k) * p.heads * part_size) + i;
-    const f32x4 before = state;
-    if (k + 1 < parts) {
-      const f32x4 sum = *at;
-      const Fade fade = fade_of(static_cast<float>(c.logs[(place + k) * p.heads + head]));
+  // Parts in front of position 0 have left no sum. Several at a time: one by one, each would wait for a load behind the last one's store.
+  constexpr int kTogether = 8;
+  for (int k0 = span.first / c.size; k0 < parts; k0 += kTogether) {
+    const int last = parts - 1;
+    f32x4 sum[kTogether];
+    double log[kTogether];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) state[e] = __builtin_fmaf(state[e], fade.high, __builtin_fmaf(state[e], fade.low, sum[e]));
+    for (int e = 0; e < kTogether; ++e) {  // of the last part nothing is used, and it may have left nothing
+      const int64_t at = place + max(min(k0 + e, last - 1), 0);
+      sum[e] = reinterpret_cast<const f32x4*>(c.sums + at * p.heads * part_size)[i];
+      log[e] = c.logs[at * p.heads + head];
     }
-    *at = before;
+#pragma unroll
+    for (int e = 0; e < kTogether; ++e) {
+      if (k0 + e > last) break;
+      reinterpret_cast<f32x4*>(c.sums + (place + k0 + e) * p.heads * part_size)[i] = state;
+      const Fade fade = fade_of(static_cast<float>(log[e]));
+#pragma unroll
+      for (int x = 0; x < 4; ++x) state[x] = __builtin_fmaf(state[x], fade.high, __builtin_fmaf(state[x], fade.low, sum[e][x]));
+    }
   }
 }
 

@@ -59,13 +59,14 @@ int64_t sum_bytes(const Cut& c, int heads, int dk, int dv) { return 4 * static_c
 
 template <int DK, int TW, int TEAMS, bool OUT>
 int launch_chunks(ChunkArgs a, int64_t numbers, hipStream_t s) {
-  using L = ChunkTiles<DK, TW, TEAMS>;
+  constexpr int kHalves = DK > 128 ? 2 : 1;
+  using L = ChunkTiles<DK, TW, TEAMS, kHalves>;
   constexpr int kLds = OUT ? L::kBytes : L::kSumBytes;
   a.numbers = numbers;
   const int64_t groups = (numbers * a.l.k_heads + 7) / 8 * 8 * a.across;
   if (groups * L::kThreads > kMaxGridThreads) return kInvalid;
   const bool plain = a.l.type == LX_BF16 && a.l.wide && (!a.l.gate || a.l.gate_type == LX_BF16) && positive(a.l.scale);
-  const auto kernel = plain ? linear_chunk_kernel<DK, TW, TEAMS, OUT, true> : linear_chunk_kernel<DK, TW, TEAMS, OUT, false>;
+  const auto kernel = plain ? linear_chunk_kernel<DK, TW, TEAMS, kHalves, OUT, true> : linear_chunk_kernel<DK, TW, TEAMS, kHalves, OUT, false>;
   allow_lds(reinterpret_cast<const void*>(kernel), kLds);
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(L::kThreads), kLds, s, a);
   return status_of(hipGetLastError());

@@ -159,9 +159,9 @@ struct Tokens {
   float none;  // whole 16 bytes
 };
 
-template <int DK, int TW, int TEAMS>
+template <int DK, int TW, int TEAMS, int HALVES>
 struct ChunkTiles {
-  static constexpr int kWaves = TW * TEAMS, kThreads = kWave * kWaves;
+  static constexpr int kWaves = TW * TEAMS, kThreads = kWave * kWaves * HALVES;
   static constexpr int kColumns = 32 * kWaves;
   static constexpr int kKeyPitch = 2 * DK, kValuePitch = 2 * kColumns;
   static constexpr int kKeyBytes = kChunk * kKeyPitch, kValueBytes = kChunk * kValuePitch;
@@ -170,7 +170,9 @@ struct ChunkTiles {
   static constexpr int kKeys = 0, kValues = kKeys + kKeyBytes, kTokens = kValues + kValueBytes;
   // Places in a tile are made by exclusive ors: it begins at a whole 256 bytes.
   static constexpr int kQueries = kTokens + (2 * TEAMS * static_cast<int>(sizeof(Tokens)) + 255) / 256 * 256, kWeights = kQueries + kKeyBytes;
-  static constexpr int kSumBytes = kQueries, kBytes = kWeights + TEAMS * kWeightBytes;
+  // What a wavefront of one half of the rows has for the other half's, one 32 x 32 tile each.
+  static constexpr int kExchange = kWeights + TEAMS * kWeightBytes, kTileBytes = 4 * 32 * 32;
+  static constexpr int kSumBytes = kQueries, kBytes = kExchange + (HALVES > 1 ? kWaves * HALVES * kTileBytes : 0);
 };
 
 // A part of a tensor as a buffer: what is read behind its end is zero and what is stored there is dropped, without a branch (behind which the
@@ -189,9 +191,10 @@ __host__ __device__ __forceinline__ bool positive(float scale) { return scale > 
 
 // OUT: outputs and states; otherwise a part's sum of a long sequence only. PLAIN: bf16 that can be moved 16 bytes at a time, a positive scale, gates bf16 or
 // none (everything else in its own kernel: its loads and stores, a value at a time perhaps, would cost this one registers).
-template <int DK, int TW, int TEAMS, bool OUT, bool PLAIN>
-__global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 && TW * TEAMS == 2) ? 1 : 2) linear_chunk_kernel(const ChunkArgs c) {
-  using L = ChunkTiles<DK, TW, TEAMS>;
+template <int DK, int TW, int TEAMS, int HALVES, bool OUT, bool PLAIN>
+__global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW * TEAMS * HALVES == 2 ? 1 : 2) linear_chunk_kernel(const ChunkArgs c) {
+  using L = ChunkTiles<DK, TW, TEAMS, HALVES>;
+  constexpr int kRows = DK / HALVES;  // of the state, a wavefront's
   extern __shared__ __attribute__((aligned(256))) uint8_t lds[];
   const LinearArgs& p = c.l;
   // Workgroups that read the same keys follow one another on one die.
@@ -212,7 +215,8 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
   const int64_t place = 2 * static_cast<int64_t>(span.row0 / c.size) + j;
 
   const int lane = threadIdx.x % kWave, h = lane / 32, n = lane % 32;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), team = wave / TW, mate = wave % TW;
+  const int number_of_wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = HALVES > 1 ? number_of_wave / L::kWaves : 0;
+  const int wave = number_of_wave - half * L::kWaves, team = wave / TW, mate = wave % TW;  // by columns
   const int blocks = (p.dv + 32 * TW - 1) / (32 * TW);  // TEAMS > 1: one
   const int head0 = k_head * p.group + (TEAMS > 1 ? beside * TEAMS : beside / blocks);
   const int head_end = (k_head + 1) * p.group;
@@ -279,6 +283,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
     for (int e = 0; e < kValueLoads; ++e) next_v[e] = u32x4{};
   };
   ask(0);
+  constexpr bool kEach = TW * HALVES >= 4;  // a head's wavefronts make one tile of weights each
 
   // ---- the decays -----------------------------------------------------------------------------------------------------
   // A token a lane: asked for two chunks ahead, made ready one ahead, by the team's last wavefront.
@@ -286,7 +291,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
   // A positive scale is part of the rows' exponents, another one multiplied in. The skip is part of a row's weight of its own token.
   const bool scaled = PLAIN || positive(p.scale);
   const float log_scale = scaled ? __builtin_amdgcn_logf(p.scale) : 0.0f;
-  const bool counts = mate == TW - 1;
+  const bool counts = mate == TW - 1 && half == HALVES - 1;
   const HeadDecay head_numbers = head_decay(p, head);
   uint32_t next_raw;
   float carried = 0.0f;
@@ -333,25 +338,25 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
   if (counts) ask_decay(0);
 
   // ---- the state ------------------------------------------------------------------------------------------------------
-  f32x16 state[DK / 32] = {};
+  f32x16 state[kRows / 32] = {};
   const bool mine = column < p.dv && !idle;
   const int64_t state_size = static_cast<int64_t>(p.dk) * p.dv;
-  const unsigned state_from = static_cast<unsigned>(8 * h * p.dv + column);
+  const unsigned state_from = static_cast<unsigned>((half * kRows + 8 * h) * p.dv + column);
   auto each_state = [&](float* base, auto use) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < DK / 32; ++t)
+    for (int t = 0; t < kRows / 32; ++t)
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        if (!mine || 32 * t + 16 * a + 8 * h >= p.dk) continue;
+        if (!mine || half * kRows + 32 * t + 16 * a + 8 * h >= p.dk) continue;
         float* const row = base + static_cast<int64_t>(32 * t + 16 * a) * p.dv;
 #pragma unroll
         for (int r = 0; r < 8; ++r) use((row + static_cast<int64_t>(r) * p.dv)[state_from], t, 8 * a + r);
       }
   };
-  f32x4* const part = reinterpret_cast<f32x4*>(c.sums + (place * p.heads + head) * part_values(p.dk, p.dv)) + (column0 / 32 + mate) * (DK / 32 * 4 * kWave);
+  f32x4* const part = reinterpret_cast<f32x4*>(c.sums + (place * p.heads + head) * part_values(p.dk, p.dv)) + (column0 / 32 + mate) * (DK / 32 * 4 * kWave) + half * (kRows / 32 * 4 * kWave);
   if (OUT && split && column0 + 32 * mate < p.dv) {
 #pragma unroll
-    for (int i = 0; i < DK / 8; ++i) {
+    for (int i = 0; i < kRows / 8; ++i) {
       const f32x4 four = part[i * kWave + lane];
 #pragma unroll
       for (int e = 0; e < 4; ++e) state[i / 4][i % 4 * 4 + e] = four[e];
@@ -392,7 +397,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
   };
   // Where the lane's first reads lie: row n of the keys (and queries), the columns of the keys and of its values, row n of the weights.
   const int key_row = tile_place<L::kKeyPitch>(n, h);
-  const int key_column = across_place<L::kKeyPitch>(0), value_column = across_place<L::kValuePitch>(32 * wave);
+  const int key_column = across_place<L::kKeyPitch>(half * kRows), value_column = across_place<L::kValuePitch>(32 * wave);
   const int weight_row = L::kWeights + team * L::kWeightBytes + 64 * n + 16 * (n >> 2 & 3);
   auto values_across = [&](int k) { return across<L::kValuePitch>(lds, L::kValues, value_column, k, 0); };
   const int my_column = column0 + 32 * mate + 8 * h;  // the lane's outputs of a row: 16 a .. from here on
@@ -482,15 +487,16 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
       // What the rows see of the state, and the products of `kTiles` tiles of weights, which read the same queries; a step's operands are made ready one
       // ahead. `block`: the first tile (two: (0, 0) and (1, 0), of the same keys).
       auto see = [&](auto tiles, int block) __attribute__((always_inline)) {
-        constexpr int kTiles = decltype(tiles)::value, kSteps = DK / 16;
+        constexpr int kTiles = decltype(tiles)::value, kSteps = kRows / 16;
+        const int from_half = HALVES > 1 ? from ^ 32 * kSteps * half : from;
         f32x16 w[2] = {};
         bf16x8 q[2][2], k[2], high[2], low[2];
         const int keys_at = L::kKeys + (kTiles == 1 && block == 2) * 32 * L::kKeyPitch;
         auto ready = [&](int step) __attribute__((always_inline)) {
           const int now = step % 2;
-          q[now][0] = eight_at(lds, L::kQueries + (from ^ 32 * step));
-          q[now][1] = eight_at(lds, L::kQueries + 32 * L::kKeyPitch + (from ^ 32 * step));
-          if constexpr (kTiles > 0) k[now] = eight_at(lds, keys_at + (from ^ 32 * step));
+          q[now][0] = eight_at(lds, L::kQueries + (from_half ^ 32 * step));
+          q[now][1] = eight_at(lds, L::kQueries + 32 * L::kKeyPitch + (from_half ^ 32 * step));
+          if constexpr (kTiles > 0) k[now] = eight_at(lds, keys_at + (from_half ^ 32 * step));
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = state[step / 2][step % 2 * 8 + e];
@@ -514,50 +520,75 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
           out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low[now], q[now][1], out[1], 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (kTiles > 0 && HALVES > 1) {  // the tile's products of the other half's keys
+          const int from_other = from_half ^ 32 * kSteps, queries_at = L::kQueries + (block > 0) * 32 * L::kKeyPitch;
+#pragma unroll
+          for (int step = 0; step < kSteps; ++step) {
+            w[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_at(lds, keys_at + (from_other ^ 32 * step)), eight_at(lds, queries_at + (from_other ^ 32 * step)), w[0], 0, 0, 0);
+            if (step % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          }
+        }
         if constexpr (kTiles > 0) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            if (TW == 4) weigh(std::integral_constant<int, 2>(), block, w[0], g);
+            if (kEach) weigh(std::integral_constant<int, 2>(), block, w[0], g);
             else weigh(std::integral_constant<int, 1>(), block, w[0], g);
             if constexpr (kTiles > 1) weigh(std::integral_constant<int, 0>(), 1, w[1], g);
             __builtin_amdgcn_sched_barrier(0);
           }
         }
       };
-      // Of two wavefronts a head the first one makes tiles (0, 0) and (1, 0), the other, which has the decays, (1, 1); of four the first three one each.
-      const int block = TW == 2 ? 2 * mate : mate;
-      const bool makes = mate == 0 || (mate < 3 && two);
+      // Of two wavefronts a head the first one makes tiles (0, 0) and (1, 0), the other, which has the decays, (1, 1); of more the first three one each.
+      const int maker = half * TW + mate, block = kEach ? maker : 2 * maker;
+      const bool makes = maker == 0 || (maker < 3 && two);
       if (!__builtin_amdgcn_readfirstlane(t.quick)) {
         if (makes) weigh_far(block);
-        if (TW == 2 && mate == 0 && two) weigh_far(1);
+        if (!kEach && mate == 0 && two) weigh_far(1);
         see(std::integral_constant<int, 0>(), 0);
-      } else if (TW == 2 && mate == 0 && two) {
-        see(std::integral_constant<int, TW == 2 ? 2 : 0>(), 0);
+      } else if (!kEach && mate == 0 && two) {
+        see(std::integral_constant<int, kEach ? 0 : 2>(), 0);
       } else if (makes) {
         see(std::integral_constant<int, 1>(), block);
       } else {
         see(std::integral_constant<int, 0>(), 0);
       }
-      if (p.skip && makes && block != (TW == 2 ? -1 : 1)) add_skip(block);
+      if (p.skip && makes && block != (kEach ? 1 : -1)) add_skip(block);
 #pragma unroll
       for (int i = 0; i < 2; ++i) out[i] *= t.seen[32 * i + n];
+      if constexpr (HALVES > 1) {  // a half keeps the rows of its own number
+        const f32x16 give = half ? out[0] : out[1];
+        if (half) out[0] = out[1];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          *reinterpret_cast<f32x4*>(lds + L::kExchange + number_of_wave * L::kTileBytes + 16 * (r * kWave + lane)) = f32x4{give[4 * r], give[4 * r + 1], give[4 * r + 2], give[4 * r + 3]};
+      }
     }
     if (counts && more) {
       put_decay(chunk + 1);
       ask_decay(chunk + 2);
     }
     // Gates are asked for here: earlier, they would take registers from what went before.
-    u32x4 gate[2][2];
+    constexpr int kOutTiles = 2 / HALVES;  // of 32 rows, a wavefront's; tile i has the rows from 32 (i + half) on
+    u32x4 gate[kOutTiles][2];
     if (OUT && PLAIN && p.gate) {
       const unsigned from = now(gate_place);
       const auto g = buffer_of(static_cast<const uint16_t*>(p.gate) + row0 * p.ld_gate + static_cast<int64_t>(head) * p.dv, rows_bytes(m, p.ld_gate, p.dv, 2));
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < kOutTiles; ++i)
 #pragma unroll
-        for (int a = 0; a < 2; ++a) gate[i][a] = buffer_load(g, from + i * static_cast<unsigned>(64 * p.ld_gate) + 32 * a);
+        for (int a = 0; a < 2; ++a) gate[i][a] = buffer_load(g, from + (i + half) * static_cast<unsigned>(64 * p.ld_gate) + 32 * a);
     }
     if constexpr (OUT) ask_next();  // not before the products of the state have left their registers
     if constexpr (OUT) __syncthreads();
+    if constexpr (OUT && HALVES > 1) {
+      const int other = number_of_wave + (half ? -L::kWaves : L::kWaves);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 four = *reinterpret_cast<const f32x4*>(lds + L::kExchange + other * L::kTileBytes + 16 * (r * kWave + lane));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[0][4 * r + e] += four[e];
+      }
+    }
 
     bf16x8 v[kChunk / 16];
 #pragma unroll
@@ -586,10 +617,10 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
         }
         for (int token = 0; token < m; ++token) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (token > 32 * i + n || 32 * i >= m) continue;
+          for (int i = 0; i < kOutTiles; ++i) {
+            if (token > 32 * (i + half) + n || 32 * (i + half) >= m) continue;
             const int in = token % 32;
-            const uint8_t* const at = lds + (i + token / 32) * L::kBlock + (weight_row ^ 16 * (in / 8)) + in % 8 * 2;
+            const uint8_t* const at = lds + (i + half + token / 32) * L::kBlock + (weight_row ^ 16 * (in / 8)) + in % 8 * 2;
             const float weight = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(at)) + bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(at + 3 * L::kBlock));
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
@@ -613,8 +644,9 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
       for (int k = 0; k < kChunk / 16; ++k)
 #pragma unroll
         for (int low = 0; low < 2; ++low) {
-          if (k < 2) out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(0, k, low), out[0], 0, 0, 0);
-          if (two) out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(1 + k / 2, k % 2, low), out[1], 0, 0, 0);
+          if (k < 2 && half == 0) out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(0, k, low), out[0], 0, 0, 0);
+          if (two && HALVES == 1) out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(1 + k / 2, k % 2, low), out[1], 0, 0, 0);
+          if (two && half) out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(1 + k / 2, k % 2, low), out[0], 0, 0, 0);
         }
       __builtin_amdgcn_sched_barrier(0);
       if (some_odd) {
@@ -622,12 +654,12 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
         for (int k = 0; k < kChunk / 16; ++k) v[k] = values_across(k);
       }
       if constexpr (PLAIN) {
-        const bool half = p.out_type == LX_BF16;
-        const int size = half ? 2 : 4;
+        const bool short_out = p.out_type == LX_BF16;
+        const int size = short_out ? 2 : 4;
         const auto to = buffer_of(static_cast<char*>(p.out) + (row0 * p.ld_out + static_cast<int64_t>(head) * p.dv) * size, idle ? 0 : rows_bytes(m, p.ld_out, p.dv, size));
         const unsigned from = now(out_place);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kOutTiles; ++i)
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
             float o[8];
@@ -640,8 +672,8 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
                 o[e] *= gate_of(__uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16));
               }
             }
-            const unsigned at = my_column + 16 * a < p.dv ? (from + i * static_cast<unsigned>(32 * p.ld_out) + 16 * a) * size : kOutside;
-            if (half) {
+            const unsigned at = my_column + 16 * a < p.dv ? (from + (i + half) * static_cast<unsigned>(32 * p.ld_out) + 16 * a) * size : kOutside;
+            if (short_out) {
               buffer_store(to, at, u32x4{__builtin_bit_cast(uint32_t, pack_bf16(o[0], o[1])), __builtin_bit_cast(uint32_t, pack_bf16(o[2], o[3])),
                                          __builtin_bit_cast(uint32_t, pack_bf16(o[4], o[5])), __builtin_bit_cast(uint32_t, pack_bf16(o[6], o[7]))});
             } else {
@@ -651,12 +683,12 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
           }
       } else if (!idle) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (32 * i + n >= m) continue;
+        for (int i = 0; i < kOutTiles; ++i) {
+          if (32 * (i + half) + n >= m) continue;
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
             if (my_column + 16 * a >= p.dv) continue;
-            const int64_t column_at = static_cast<int64_t>(head) * p.dv + my_column + 16 * a, row = row0 + 32 * i + n;
+            const int64_t column_at = static_cast<int64_t>(head) * p.dv + my_column + 16 * a, row = row0 + 32 * (i + half) + n;
             float o[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = out[i][8 * a + e];
@@ -680,10 +712,10 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
       const float fade = t.fade;
       const int from = now(key_column);
       if constexpr (!OUT) part_log += t.whole;
-      bf16x8 key[2][DK / 32], high[2], low[2];
+      bf16x8 key[2][kRows / 32], high[2], low[2];
       auto ready = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-        for (int x = 0; x < DK / 32; ++x)
+        for (int x = 0; x < kRows / 32; ++x)
           key[k % 2][x] = across<L::kKeyPitch>(lds, L::kKeys, from, k, 4 * x);  // columns 32 x .. of tokens 16 k ..
         const u32x4 raw = __builtin_bit_cast(u32x4, v[k]);
         const f32x4 w0 = *reinterpret_cast<const f32x4*>(t.update + 16 * k + 8 * h), w1 = *reinterpret_cast<const f32x4*>(t.update + 16 * k + 8 * h + 4);
@@ -697,15 +729,15 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
       };
       ready(0);
 #pragma unroll
-      for (int x = 0; x < DK / 32; ++x) state[x] *= fade;
+      for (int x = 0; x < kRows / 32; ++x) state[x] *= fade;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k) {
         if (k + 1 < kChunk / 16) ready(k + 1);
 #pragma unroll
-        for (int x = 0; x < DK / 32; ++x) state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key[k % 2][x], high[k % 2], state[x], 0, 0, 0);
+        for (int x = 0; x < kRows / 32; ++x) state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key[k % 2][x], high[k % 2], state[x], 0, 0, 0);
 #pragma unroll
-        for (int x = 0; x < DK / 32; ++x) state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key[k % 2][x], low[k % 2], state[x], 0, 0, 0);
+        for (int x = 0; x < kRows / 32; ++x) state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key[k % 2][x], low[k % 2], state[x], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -721,8 +753,8 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS, DK == 256 || (DK == 128 &&
       each_state(static_cast<float*>(p.states.out) + (static_cast<int64_t>(slot) * p.heads + head) * state_size, [&](float& x, int t, int r) { x = state[t][r]; });
   } else if (!idle && column0 + 32 * mate < p.dv) {
 #pragma unroll
-    for (int i = 0; i < DK / 8; ++i) part[i * kWave + lane] = f32x4{state[i / 4][i % 4 * 4], state[i / 4][i % 4 * 4 + 1], state[i / 4][i % 4 * 4 + 2], state[i / 4][i % 4 * 4 + 3]};
-    if (mate == 0 && lane == 0 && column0 == 0) c.logs[place * p.heads + head] = part_log;
+    for (int i = 0; i < kRows / 8; ++i) part[i * kWave + lane] = f32x4{state[i / 4][i % 4 * 4], state[i / 4][i % 4 * 4 + 1], state[i / 4][i % 4 * 4 + 2], state[i / 4][i % 4 * 4 + 3]};
+    if (mate == 0 && half == 0 && lane == 0 && column0 == 0) c.logs[place * p.heads + head] = part_log;
   }
 }
 

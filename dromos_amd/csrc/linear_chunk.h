@@ -766,12 +766,12 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const ChunkArgs c) {
   int s, j;
   if (!mix_find_long(p.b, c.size, 2 * (blockIdx.x / groups), s, j) || j != 0) return;
   const MixSpan span = mix_span(p.b, s);
+  const int slot = mix_slot(p.states, s);
   if (span.stop <= c.size || !mix_all_found(p.b, c.size, s, span)) return;
   const int64_t i = static_cast<int64_t>(blockIdx.x % groups) * 256 + threadIdx.x;
   if (i >= fours) return;
   const int head = static_cast<int>(4 * i / part_size), of_head = static_cast<int>(i - head * (part_size / 4)), parts = (span.stop + c.size - 1) / c.size;
   const int64_t place = 2 * static_cast<int64_t>(span.row0 / c.size);
-  const int slot = mix_slot(p.states, s);
   f32x4 state = {};
   if (p.states.in && slot >= 0 && !span.begins) {
     // Four neighbouring rows of a column.
@@ -790,8 +790,9 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const ChunkArgs c) {
     f32x4 sum[kTogether];
     double log[kTogether];
 #pragma unroll
-    for (int e = 0; e < kTogether; ++e) {  // of the last part nothing is used, and it may have left nothing
-      const int64_t at = place + max(min(k0 + e, last - 1), 0);
+    for (int e = 0; e < kTogether; ++e) {
+      if (k0 + e >= last) break;  // the last part leaves no sum
+      const int64_t at = place + k0 + e;
       sum[e] = reinterpret_cast<const f32x4*>(c.sums + at * p.heads * part_size)[i];
       log[e] = c.logs[at * p.heads + head];
     }
@@ -799,6 +800,7 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const ChunkArgs c) {
     for (int e = 0; e < kTogether; ++e) {
       if (k0 + e > last) break;
       reinterpret_cast<f32x4*>(c.sums + (place + k0 + e) * p.heads * part_size)[i] = state;
+      if (k0 + e == last) break;
       const Fade fade = fade_of(static_cast<float>(log[e]));
 #pragma unroll
       for (int x = 0; x < 4; ++x) state[x] = __builtin_fmaf(state[x], fade.high, __builtin_fmaf(state[x], fade.low, sum[e][x]));

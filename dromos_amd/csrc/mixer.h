@@ -92,13 +92,23 @@ __device__ __forceinline__ bool mix_find_long(const MixBatch& b, int size, int64
   return s >= 0 && of <= b.T / size;
 }
 
-// Whether those numbers find all pieces of sequence s, as they do wherever rows ascend: if its first and last ones, then those between them, since a search
-// for a later number never ends in front of one for an earlier one.
+// Whether those numbers find all pieces of sequence s, as they do wherever rows ascend: if they find its first and last ones, then those between them, since a
+// search for a later number never ends in front of one for an earlier one. Both searches in one.
 __device__ __forceinline__ bool mix_all_found(const MixBatch& b, int size, int s, const MixSpan& span) {
   if (b.seqs == 1) return true;
-  auto number = [&](int i) { return 2 * static_cast<int64_t>(mix_clamp(b.rows[i], 0, b.T) / size); };
-  const int64_t first = 2 * static_cast<int64_t>(span.row0 / size);
-  return mix_last(b.seqs, first, number) == s && mix_last(b.seqs, first + (span.stop - 1) / size, number) == s;
+  const int lane = threadIdx.x % kWave, first = 2 * (span.row0 / size), last = first + (span.stop - 1) / size;  // at most 2 T / size
+  int low = 0, count = b.seqs;
+  while (true) {
+    const int step = (count + kWave - 1) / kWave, at = lane * step;
+    const int number = 2 * (mix_clamp(b.rows[low + (at < count ? at : 0)], 0, b.T) / size);
+    const uint64_t before_first = __ballot(at < count && number <= first), before_last = __ballot(at < count && number <= last);
+    if (!before_first) return false;
+    const int pick = kWave - 1 - __builtin_clzll(before_last);
+    if (pick != kWave - 1 - __builtin_clzll(before_first)) return false;
+    low += pick * step;
+    count = count - pick * step < step ? count - pick * step : step;
+    if (count <= 1) return __builtin_amdgcn_readfirstlane(low) == s;
+  }
 }
 
 struct MixStates {

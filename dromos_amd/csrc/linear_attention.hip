@@ -35,6 +35,9 @@ struct Cut {
 };
 
 constexpr int kLeastPart = 128;
+// Of sequences of so many parts the outputs' kernel adds up what is in front of a part by itself; of more, where that would be most of what it reads, a kernel in between
+// runs through them once. 4096 tokens of 128 heads, 8 parts: 114 us and 128; eight sequences of up to 4 parts of 8 heads of 256 by 256: 123 and 150.
+constexpr int kFewParts = 8;
 
 Cut cut_of(int T, int max_rows, int heads, int k_heads, int dk, int dv) {
   Cut c;
@@ -78,10 +81,12 @@ int chunks_of(const ChunkArgs& a, hipStream_t s) {
   if (!a.single) {
     const int64_t places = 2 * static_cast<int64_t>(b.T / a.size);
     if (int st = launch_chunks<DK, TW, TEAMS, false>(a, places, s)) return st;
-    const int64_t fours = a.l.heads * part_values(a.l.dk, a.l.dv) / 4, groups = (fours + 255) / 256 * (places / 2);
-    if (groups * 256 > kMaxGridThreads) return kInvalid;
-    hipLaunchKernelGGL(linear_parts_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, a);
-    if (int st = status_of(hipGetLastError())) return st;
+    if (!a.sums_only) {
+      const int64_t fours = a.l.heads * part_values(a.l.dk, a.l.dv) / 4, groups = (fours + 255) / 256 * (places / 2);
+      if (groups * 256 > kMaxGridThreads) return kInvalid;
+      hipLaunchKernelGGL(linear_parts_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, a);
+      if (int st = status_of(hipGetLastError())) return st;
+    }
   }
   return launch_chunks<DK, TW, TEAMS, true>(a, mix_piece_count(b, MixPieces{a.size, a.single}), s);
 }
@@ -98,6 +103,7 @@ int chunks(const LinearArgs& p, void* workspace, hipStream_t s) {
   const Cut c = cut_of(p.b.T, p.b.max_rows, p.heads, p.k_heads, p.dk, p.dv);
   ChunkArgs a{};
   a.l = p, a.size = c.size, a.single = mix_pieces(p.b, c.size).single, a.across = c.across;
+  a.sums_only = p.b.max_rows <= kFewParts * c.size;
   if (!a.single) {
     if (!workspace) return kInvalid;
     a.sums = static_cast<float*>(workspace);

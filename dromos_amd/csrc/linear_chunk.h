@@ -19,7 +19,8 @@
 // registers meanwhile.
 //
 // Long sequences are cut into parts where there are too few workgroups: a first kernel leaves each part's own sum (keys and values
-// only), a second one runs through them and leaves the state in front of every part, and this one starts from there.
+// only), and this one starts from the sums in front of its part; where there are many, a kernel in between runs through them and leaves the state in front of every
+// part.
 #pragma once
 
 #include <type_traits>
@@ -39,6 +40,7 @@ struct ChunkArgs {
   int single;       // no sequence has more than one part
   int64_t numbers;  // of parts that the launch counts to
   int across;       // workgroups of a part and key head
+  int sums_only;    // sequences have few parts at most: nothing runs through them in between
   float* sums;      // [2 (T / size), heads] states as wavefronts hold them: parts' sums, then the states in front of them
   double* logs;     // [2 (T / size), heads] logarithms of what the parts leave of what was in front of them
 };
@@ -210,7 +212,10 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
   const int begin = max(span.first, j * c.size), end = min(span.stop, (j + 1) * c.size);
   // A sequence whose parts have not all been found (its rows do not ascend) has left no states between them.
   const bool split = span.stop > c.size && (!OUT || mix_all_found(p.b, c.size, s, span));
-  if (begin >= end || (!OUT && (!split || end == span.stop))) return;
+  // The last part leaves no sum; where nothing runs through the sums afterwards, its place takes the state that the sequence goes on from: read in the
+  // outputs' kernel, it may have been replaced already.
+  const bool last = end == span.stop, keeps = !OUT && last && c.sums_only && p.states.in && slot >= 0 && !span.begins;
+  if (begin >= end || (!OUT && (!split || (last && !keeps)))) return;
   // A sequence's part has a place of its own: those of more than one part are more than `size` rows each.
   const int64_t place = 2 * static_cast<int64_t>(span.row0 / c.size) + j;
 
@@ -225,7 +230,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
   const bool idle = head0 + team >= head_end;
   const int column = column0 + 32 * mate + lane_column(n);  // the lane's of the state
   const int64_t first_row = static_cast<int64_t>(span.row0) + begin;
-  const int rows = end - begin, chunks = (rows + kChunk - 1) / kChunk;
+  const int rows = end - begin, chunks = keeps ? 0 : (rows + kChunk - 1) / kChunk;
 
   // ---- the next chunk on its way --------------------------------------------------------------------------------------
   constexpr int kKeyLoads = kChunk * DK / 8 / L::kThreads, kValueLoads = kChunk * L::kColumns / 8 / L::kThreads;
@@ -353,17 +358,28 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
         for (int r = 0; r < 8; ++r) use((row + static_cast<int64_t>(r) * p.dv)[state_from], t, 8 * a + r);
       }
   };
-  f32x4* const part = reinterpret_cast<f32x4*>(c.sums + (place * p.heads + head) * part_values(p.dk, p.dv)) + (column0 / 32 + mate) * (DK / 32 * 4 * kWave) + half * (kRows / 32 * 4 * kWave);
-  if (OUT && split && column0 + 32 * mate < p.dv) {
-#pragma unroll
-    for (int i = 0; i < kRows / 8; ++i) {
-      const f32x4 four = part[i * kWave + lane];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) state[i / 4][i % 4 * 4 + e] = four[e];
-    }
-  } else if (OUT && !split && p.states.in && slot >= 0 && !span.begins) {
+  const int64_t part_size = part_values(p.dk, p.dv);
+  f32x4* const part = reinterpret_cast<f32x4*>(c.sums + (place * p.heads + head) * part_size) + (column0 / 32 + mate) * (DK / 32 * 4 * kWave) + half * (kRows / 32 * 4 * kWave);
+  const bool goes_on = p.states.in && slot >= 0 && !span.begins;
+  if (OUT ? !split && goes_on : keeps) {
     float* const from = const_cast<float*>(static_cast<const float*>(p.states.in)) + (static_cast<int64_t>(slot) * p.heads + head) * state_size;
     each_state(from, [&](float& x, int t, int r) { state[t][r] = x; });
+  }
+  if (OUT && split && column0 + 32 * mate < p.dv) {
+    auto take = [&](int k, Fade fade) {
+      const f32x4* const from = part + (k - j) * p.heads * (part_size / 4);
+      f32x4 four[kRows / 8];
+#pragma unroll
+      for (int i = 0; i < kRows / 8; ++i) four[i] = from[i * kWave + lane];
+#pragma unroll
+      for (int i = 0; i < kRows / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          state[i / 4][i % 4 * 4 + e] = __builtin_fmaf(state[i / 4][i % 4 * 4 + e], fade.high, __builtin_fmaf(state[i / 4][i % 4 * 4 + e], fade.low, four[i][e]));
+    };
+    if (!c.sums_only) take(j, Fade{0.0f, 0.0f});
+    else if (goes_on) take((span.stop - 1) / c.size, Fade{0.0f, 0.0f});
+    for (int k = c.sums_only ? span.first / c.size : j; k < j; ++k) take(k, fade_of(static_cast<float>(c.logs[(place + k - j) * p.heads + head])));
   }
   const float skip = p.skip ? p.skip[head] : 0.0f;
   double part_log = 0.0;
@@ -749,7 +765,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
   }
 
   if constexpr (OUT) {
-    if (p.states.out && slot >= 0 && end == span.stop)
+    if (p.states.out && slot >= 0 && last)
       each_state(static_cast<float*>(p.states.out) + (static_cast<int64_t>(slot) * p.heads + head) * state_size, [&](float& x, int t, int r) { x = state[t][r]; });
   } else if (!idle && column0 + 32 * mate < p.dv) {
 #pragma unroll

@@ -60,19 +60,29 @@ Cut cut_of(int T, int max_rows, int heads, int k_heads, int dk, int dv) {
 
 int64_t sum_bytes(const Cut& c, int heads, int dk, int dv) { return 4 * static_cast<int64_t>(c.places) * heads * part_values(dk, dv); }
 
-template <int DK, int TW, int TEAMS, bool OUT>
-int launch_chunks(ChunkArgs a, int64_t numbers, hipStream_t s) {
+template <int DK, int TW, int TEAMS, bool OUT, bool PLAIN, int TERMS>
+int launch_kernel(const ChunkArgs& a, int64_t groups, hipStream_t s) {
   constexpr int kHalves = DK > 128 ? 2 : 1;
-  using L = ChunkTiles<DK, TW, TEAMS, kHalves>;
+  using L = ChunkTiles<DK, TW, TEAMS, kHalves, TERMS>;
   constexpr int kLds = OUT ? L::kBytes : L::kSumBytes;
-  a.numbers = numbers;
-  const int64_t groups = (numbers * a.l.k_heads + 7) / 8 * 8 * a.across;
   if (groups * L::kThreads > kMaxGridThreads) return kInvalid;
-  const bool plain = a.l.type == LX_BF16 && a.l.wide && (!a.l.gate || a.l.gate_type == LX_BF16) && positive(a.l.scale);
-  const auto kernel = plain ? linear_chunk_kernel<DK, TW, TEAMS, kHalves, OUT, true> : linear_chunk_kernel<DK, TW, TEAMS, kHalves, OUT, false>;
+  const auto kernel = linear_chunk_kernel<DK, TW, TEAMS, kHalves, OUT, PLAIN, TERMS>;
   allow_lds(reinterpret_cast<const void*>(kernel), kLds);
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(L::kThreads), kLds, s, a);
   return status_of(hipGetLastError());
+}
+
+template <int DK, int TW, int TEAMS, bool OUT>
+int launch_chunks(ChunkArgs a, int64_t numbers, hipStream_t s) {
+  a.numbers = numbers;
+  const int64_t groups = (numbers * a.l.k_heads + 7) / 8 * 8 * a.across;
+  const bool plain = a.l.type == LX_BF16 && a.l.wide && (!a.l.gate || a.l.gate_type == LX_BF16) && positive(a.l.scale);
+  if constexpr (OUT) {
+    if (plain && a.l.out_type == LX_BF16) return launch_kernel<DK, TW, TEAMS, true, true, 2>(a, groups, s);
+    return plain ? launch_kernel<DK, TW, TEAMS, true, true, 3>(a, groups, s) : launch_kernel<DK, TW, TEAMS, true, false, 3>(a, groups, s);
+  } else {
+    return plain ? launch_kernel<DK, TW, TEAMS, false, true, 2>(a, groups, s) : launch_kernel<DK, TW, TEAMS, false, false, 2>(a, groups, s);
+  }
 }
 
 template <int DK, int TW, int TEAMS>

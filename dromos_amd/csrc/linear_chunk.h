@@ -92,32 +92,37 @@ __device__ __forceinline__ bf16x8 across(const uint8_t* lds, int at, int from, i
   return r.whole;
 }
 
-// Two f32 as bf16, and what their rounding leaves as bf16. Values that are not used again: taken off by one instruction each, in place (a dot product
-// with minus one and nothing; an infinity or a NaN of one is one of the other's rest too, which is summed with it). KEPT: by two.
-template <bool KEPT>
-__device__ __forceinline__ void split_two(float x, float y, uint32_t& high, uint32_t& low) {
-  const bf16x2 two = pack_bf16(x, y);
-  high = __builtin_bit_cast(uint32_t, two);
-  if constexpr (KEPT) {
-    low = __builtin_bit_cast(uint32_t, pack_bf16(x - __uint_as_float(high << 16), y - __uint_as_float(high & 0xffff0000u)));
-  } else {
-    uint32_t first = 0x0000bf80u, second = 0xbf800000u;
-    asm("" : "+s"(first), "+s"(second));  // as constants of the instruction they are something else
-    low = __builtin_bit_cast(uint32_t, pack_bf16(__builtin_amdgcn_fdot2_f32_bf16(two, as_bf16x2(first), x, false),
-                                                 __builtin_amdgcn_fdot2_f32_bf16(two, as_bf16x2(second), y, false)));
+// Two f32 as bf16, what their rounding leaves as bf16, and so on, TERMS of them. Values that are not used again: taken off by one instruction each, in
+// place (a dot product with minus one and nothing; an infinity or a NaN of one is one of the other's rest too, which is summed with it). KEPT: by two at first.
+template <bool KEPT, int TERMS>
+__device__ __forceinline__ void split_two(float x, float y, uint32_t (&term)[TERMS]) {
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    const bf16x2 two = pack_bf16(x, y);
+    term[t] = __builtin_bit_cast(uint32_t, two);
+    if (t + 1 == TERMS) break;
+    if (KEPT && t == 0) {
+      x -= __uint_as_float(term[t] << 16), y -= __uint_as_float(term[t] & 0xffff0000u);
+    } else {
+      uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+      asm("" : "+s"(first), "+s"(second));  // as constants of the instruction they are something else
+      x = __builtin_amdgcn_fdot2_f32_bf16(two, as_bf16x2(first), x, false);
+      y = __builtin_amdgcn_fdot2_f32_bf16(two, as_bf16x2(second), y, false);
+    }
   }
 }
-template <bool KEPT>
-__device__ __forceinline__ void split_eight(const float (&v)[8], bf16x8& high, bf16x8& low) {
-  u32x4 a, b;
+template <bool KEPT, int TERMS>
+__device__ __forceinline__ void split_eight(const float (&v)[8], bf16x8 (&term)[TERMS]) {
+  u32x4 all[TERMS];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t x, y;
-    split_two<KEPT>(v[2 * j], v[2 * j + 1], x, y);
-    a[j] = x, b[j] = y;
+    uint32_t two[TERMS];
+    split_two<KEPT>(v[2 * j], v[2 * j + 1], two);
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) all[t][j] = two[t];
   }
-  high = __builtin_bit_cast(bf16x8, a);
-  low = __builtin_bit_cast(bf16x8, b);
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) term[t] = __builtin_bit_cast(bf16x8, all[t]);
 }
 
 // A sum over the wavefront's lanes up to and with each one, of 64-bit integers.
@@ -161,14 +166,14 @@ struct Tokens {
   float none;  // whole 16 bytes
 };
 
-template <int DK, int TW, int TEAMS, int HALVES>
+template <int DK, int TW, int TEAMS, int HALVES, int TERMS>
 struct ChunkTiles {
   static constexpr int kWaves = TW * TEAMS, kThreads = kWave * kWaves * HALVES;
   static constexpr int kColumns = 32 * kWaves;
   static constexpr int kKeyPitch = 2 * DK, kValuePitch = 2 * kColumns;
   static constexpr int kKeyBytes = kChunk * kKeyPitch, kValueBytes = kChunk * kValuePitch;
   static constexpr int kBlock = 32 * 64;             // a 32 x 32 tile of weights, bf16
-  static constexpr int kWeightBytes = 2 * 3 * kBlock;  // of a head: tiles (0, 0), (0, 1), (1, 1) as values, then what their rounding left
+  static constexpr int kWeightBytes = TERMS * 3 * kBlock;  // of a head: tiles (0, 0), (0, 1), (1, 1) as values, then what their rounding left
   static constexpr int kKeys = 0, kValues = kKeys + kKeyBytes, kTokens = kValues + kValueBytes;
   // Places in a tile are made by exclusive ors: it begins at a whole 256 bytes.
   static constexpr int kQueries = kTokens + (2 * TEAMS * static_cast<int>(sizeof(Tokens)) + 255) / 256 * 256, kWeights = kQueries + kKeyBytes;
@@ -193,9 +198,9 @@ __host__ __device__ __forceinline__ bool positive(float scale) { return scale > 
 
 // OUT: outputs and states; otherwise a part's sum of a long sequence only. PLAIN: bf16 that can be moved 16 bytes at a time, a positive scale, gates bf16 or
 // none (everything else in its own kernel: its loads and stores, a value at a time perhaps, would cost this one registers).
-template <int DK, int TW, int TEAMS, int HALVES, bool OUT, bool PLAIN>
+template <int DK, int TW, int TEAMS, int HALVES, bool OUT, bool PLAIN, int TERMS>
 __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW * TEAMS * HALVES == 2 ? 1 : 2) linear_chunk_kernel(const ChunkArgs c) {
-  using L = ChunkTiles<DK, TW, TEAMS, HALVES>;
+  using L = ChunkTiles<DK, TW, TEAMS, HALVES, TERMS>;
   constexpr int kRows = DK / HALVES;  // of the state, a wavefront's
   extern __shared__ __attribute__((aligned(256))) uint8_t lds[];
   const LinearArgs& p = c.l;
@@ -441,15 +446,12 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
       // Weights, in tiles of 32 rows by 32 tokens: (0, 0), (1, 0), (1, 1).
       const int from = now(key_row), to = now(weight_row), here = now(n);  // compared anew: kept, the results cost more scalar registers than there are
       auto put_weights = [&](int block, int g, const float (&v)[4]) __attribute__((always_inline)) {
-        u32x2 high, low;
-        uint32_t x, y;
-        split_two<false>(v[0], v[1], x, y);
-        high.x = x, low.x = y;
-        split_two<false>(v[2], v[3], x, y);
-        high.y = x, low.y = y;
+        uint32_t x[TERMS], y[TERMS];
+        split_two<false>(v[0], v[1], x);
+        split_two<false>(v[2], v[3], y);
         uint8_t* const at = lds + block * L::kBlock + (to ^ 16 * g) + 8 * h;
-        *reinterpret_cast<u32x2*>(at) = high;
-        *reinterpret_cast<u32x2*>(at + 3 * L::kBlock) = low;
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) *reinterpret_cast<u32x2*>(at + 3 * L::kBlock * term) = u32x2{x[term], y[term]};
       };
       // Tokens 8 g + 4 h .. + 3 of the tile's. `kind`: the tile is one on the diagonal (1), the one below it (0), or either (2).
       auto weigh = [&](auto kind, int block, const f32x16& w, int g) __attribute__((always_inline)) {
@@ -495,10 +497,13 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
         if (h != (n >> 2 & 1)) return;
         asm volatile("" ::: "memory");  // written as other types
         uint16_t* const at = reinterpret_cast<uint16_t*>(lds + block * L::kBlock + (to ^ 16 * (n >> 3)) + 8 * h + 2 * (n & 3));
-        uint32_t high, low;
-        split_two<false>(bf16_bits_to_f32(at[0]) + bf16_bits_to_f32(at[3 * L::kBlock / 2]) + skip, 0.0f, high, low);
-        at[0] = static_cast<uint16_t>(high);
-        at[3 * L::kBlock / 2] = static_cast<uint16_t>(low);
+        float whole = 0.0f;
+#pragma unroll
+        for (int term = TERMS - 1; term >= 0; --term) whole += bf16_bits_to_f32(at[3 * L::kBlock / 2 * term]);
+        uint32_t parts[TERMS];
+        split_two<false>(whole + skip, 0.0f, parts);
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) at[3 * L::kBlock / 2 * term] = static_cast<uint16_t>(parts[term]);
       };
       // What the rows see of the state, and the products of `kTiles` tiles of weights, which read the same queries; a step's operands are made ready one
       // ahead. `block`: the first tile (two: (0, 0) and (1, 0), of the same keys).
@@ -506,7 +511,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
         constexpr int kTiles = decltype(tiles)::value, kSteps = kRows / 16;
         const int from_half = HALVES > 1 ? from ^ 32 * kSteps * half : from;
         f32x16 w[2] = {};
-        bf16x8 q[2][2], k[2], high[2], low[2];
+        bf16x8 q[2][2], k[2], held[2][TERMS];
         const int keys_at = L::kKeys + (kTiles == 1 && block == 2) * 32 * L::kKeyPitch;
         auto ready = [&](int step) __attribute__((always_inline)) {
           const int now = step % 2;
@@ -516,7 +521,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = state[step / 2][step % 2 * 8 + e];
-          split_eight<true>(v, high[now], low[now]);
+          split_eight<true>(v, held[now]);
         };
         ready(0);
         __builtin_amdgcn_sched_barrier(0);
@@ -524,16 +529,19 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
         for (int step = 0; step < kSteps; ++step) {
           const int now = step % 2;
           if (step + 1 < kSteps) ready(step + 1);
-          out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high[now], q[now][0], out[0], 0, 0, 0);
-          out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(high[now], q[now][1], out[1], 0, 0, 0);
+          out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(held[now][0], q[now][0], out[0], 0, 0, 0);
+          out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(held[now][0], q[now][1], out[1], 0, 0, 0);
           if constexpr (kTiles == 2) w[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[now], q[now][0], w[0], 0, 0, 0);
           if constexpr (kTiles == 2) w[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[now], q[now][1], w[1], 0, 0, 0);
           if constexpr (kTiles == 1) {
             if (block == 0) w[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[now], q[now][0], w[0], 0, 0, 0);
             else w[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[now], q[now][1], w[0], 0, 0, 0);
           }
-          out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low[now], q[now][0], out[0], 0, 0, 0);
-          out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(low[now], q[now][1], out[1], 0, 0, 0);
+#pragma unroll
+          for (int term = 1; term < TERMS; ++term) {
+            out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(held[now][term], q[now][0], out[0], 0, 0, 0);
+            out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(held[now][term], q[now][1], out[1], 0, 0, 0);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (kTiles > 0 && HALVES > 1) {  // the tile's products of the other half's keys
@@ -637,7 +645,9 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
             if (token > 32 * (i + half) + n || 32 * (i + half) >= m) continue;
             const int in = token % 32;
             const uint8_t* const at = lds + (i + half + token / 32) * L::kBlock + (weight_row ^ 16 * (in / 8)) + in % 8 * 2;
-            const float weight = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(at)) + bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(at + 3 * L::kBlock));
+            float weight = 0.0f;
+#pragma unroll
+            for (int term = TERMS - 1; term >= 0; --term) weight += bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(at + 3 * L::kBlock * term));
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
               const u32x4 eight = __builtin_bit_cast(u32x4, eight_at(lds, L::kValues + tile_place<L::kValuePitch>(token, 4 * wave + 2 * a + h)));
@@ -653,16 +663,16 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
       __builtin_amdgcn_sched_barrier(0);
       // The weights' products, the gates' factors meanwhile.
       const int from = now(weight_row ^ 16 * h);
-      auto weight_unit = [&](int block, int k, int low) {  // of row n, tokens 16 k + 8 h .. of the tile
-        return eight_at(lds, (block + 3 * low) * L::kBlock + (from ^ 32 * k));
+      auto weight_unit = [&](int block, int k, int term) {  // of row n, tokens 16 k + 8 h .. of the tile
+        return eight_at(lds, (block + 3 * term) * L::kBlock + (from ^ 32 * k));
       };
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k)
 #pragma unroll
-        for (int low = 0; low < 2; ++low) {
-          if (k < 2 && half == 0) out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(0, k, low), out[0], 0, 0, 0);
-          if (two && HALVES == 1) out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(1 + k / 2, k % 2, low), out[1], 0, 0, 0);
-          if (two && half) out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(1 + k / 2, k % 2, low), out[0], 0, 0, 0);
+        for (int term = 0; term < TERMS; ++term) {
+          if (k < 2 && half == 0) out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(0, k, term), out[0], 0, 0, 0);
+          if (two && HALVES == 1) out[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(1 + k / 2, k % 2, term), out[1], 0, 0, 0);
+          if (two && half) out[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[k], weight_unit(1 + k / 2, k % 2, term), out[0], 0, 0, 0);
         }
       __builtin_amdgcn_sched_barrier(0);
       if (some_odd) {
@@ -728,7 +738,8 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
       const float fade = t.fade;
       const int from = now(key_column);
       if constexpr (!OUT) part_log += t.whole;
-      bf16x8 key[2][kRows / 32], high[2], low[2];
+      constexpr int kTerms = 3;
+      bf16x8 key[2][kRows / 32], scaled_v[2][kTerms];
       auto ready = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < kRows / 32; ++x)
@@ -741,7 +752,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
           const uint32_t pair = raw[e / 2];
           x[e] = __uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16) * (e < 4 ? w0[e % 4] : w1[e % 4]);
         }
-        split_eight<false>(x, high[k % 2], low[k % 2]);
+        split_eight<false>(x, scaled_v[k % 2]);
       };
       ready(0);
 #pragma unroll
@@ -751,9 +762,9 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
       for (int k = 0; k < kChunk / 16; ++k) {
         if (k + 1 < kChunk / 16) ready(k + 1);
 #pragma unroll
-        for (int x = 0; x < kRows / 32; ++x) state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key[k % 2][x], high[k % 2], state[x], 0, 0, 0);
+        for (int term = 0; term < kTerms; ++term)
 #pragma unroll
-        for (int x = 0; x < kRows / 32; ++x) state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key[k % 2][x], low[k % 2], state[x], 0, 0, 0);
+          for (int x = 0; x < kRows / 32; ++x) state[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key[k % 2][x], scaled_v[k % 2][term], state[x], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
     }

@@ -4,7 +4,7 @@
 // eight channels of a piece of a sequence's rows and slides over them with the last rows in registers, four rows ahead on their way. The first
 // piece of a sequence reads the rows it kept, and leaves the new ones (no other piece looks at either), so `in` and `out` may
 // be the same. A single token is a chain of loads: the sequence's bounds and slot, its kept rows; filters are asked for before the first of them.
-// 4096 rows of 10240 channels, bf16, four taps: 34.4 us (4.9 TB/s; 61.0 us a row at a time with pieces of 16 rows), 64 sequences of one row of them
+// 4096 rows of 10240 channels, bf16, four taps: 33.4 us (5.0 TB/s; 61.0 us a row at a time), 64 sequences of one row of them
 // 5.6 us (12.9 us with filters read a value at a time). Five sequences of 611 rows of 2050 channels f32, which only two at a time are aligned: 9.5 us
 // (15.0 us one at a time).
 #include "mixer.h"
@@ -243,9 +243,10 @@ __global__ void __launch_bounds__(256) conv_kernel(const ConvArgs p) {
 template <int V, int W>
 int launch(ConvArgs p, hipStream_t s) {
   p.blocks = (p.C + 256 * V - 1) / (256 * V);
-  // Rows of a piece: a filter is read for each, so many, as long as the device has work for every place.
+  // Rows of a piece: a filter is read for each and so are the rows in front of it, so many of them as long as eight wavefronts a unit of the device remain. 4096 rows of
+  // 10240 channels: 33.4 us by 32 rows, 34.4 by 16; 2400 rows of 2050 f32 channels, half as many threads: 12.3 us and 9.5.
   const int64_t threads = static_cast<int64_t>(p.b.T) * p.blocks * 256;
-  const int size = threads / 32 >= 1536 * static_cast<int64_t>(compute_units()) ? 32 : 16;
+  const int size = threads / 32 >= 512 * static_cast<int64_t>(compute_units()) ? 32 : 16;
   p.pieces = mix_pieces(p.b, size);
   const int64_t groups = mix_piece_count(p.b, p.pieces) * p.blocks;
   if (groups * 256 > kMaxGridThreads) return kInvalid;

@@ -7,7 +7,10 @@ namespace {
 
 constexpr int kMaxDk = 256, kMaxDv = 512, kMaxHeads = 4096;
 constexpr int kMaxStride = 1 << 22;  // values: rows of a chunk are told apart in 31 bits
-constexpr int kMostSteps = 16;  // rows of a sequence that go token by token
+// Rows of a sequence that go token by token; from there on by chunks, whose products cost the same for one row and 64. 128 heads of 128 by 64, by tokens and by a chunk: 8
+// sequences of 4 rows 17.2 us and 18.8, of 8 24.5 and 19.2, of 16 37.6 and 20.7; 64 sequences of 4 105 and 132, of 8 139 and 136; one sequence of 32 heads of 128 by
+// 128, 4 rows 7.0 and 11.3, 8 rows 10.0 and 11.3, 12 rows 13.0 and 11.3.
+constexpr int kMostSteps = 6;
 
 template <int COLS, int ROWS>
 int launch_step(const LinearArgs& p, hipStream_t s) {
@@ -21,7 +24,8 @@ int launch_step(const LinearArgs& p, hipStream_t s) {
 
 int steps(const LinearArgs& p, hipStream_t s) {
   if (p.dk <= 64) return launch_step<8, 8>(p, s);
-  // 16 columns a wavefront where 32 leave the device short of wavefronts.
+  // 16 columns a wavefront where 32 leave the device short of wavefronts: one sequence of 32 heads of 128 by 128 4.4 us, 4.9 by 32; eight of 128 heads of 128 by 64,
+  // 2048 wavefronts of 32 columns, 17.6 us and 18.1 by 16.
   const bool few = static_cast<int64_t>(p.b.seqs) * p.heads * ((p.dv + 31) / 32) < 4 * compute_units();
   if (p.dk <= 128) return few ? launch_step<4, 8>(p, s) : launch_step<8, 16>(p, s);
   return few ? launch_step<4, 16>(p, s) : launch_step<8, 32>(p, s);
@@ -34,7 +38,7 @@ struct Cut {
   int size, places;  // rows of a part; parts of long sequences there may be
 };
 
-constexpr int kLeastPart = 128;
+constexpr int kLeastPart = 128;  // rows; five sequences of up to 611 rows of 12 heads 32.7 us, 43.2 by 256
 // Of sequences of so many parts the outputs' kernel adds up what is in front of a part by itself; of more, where that would be most of what it reads, a kernel in between
 // runs through them once. 4096 tokens of 128 heads, 8 parts: 114 us and 128; eight sequences of up to 4 parts of 8 heads of 256 by 256: 123 and 150.
 constexpr int kFewParts = 8;
@@ -42,13 +46,15 @@ constexpr int kFewParts = 8;
 Cut cut_of(int T, int max_rows, int heads, int k_heads, int dk, int dv) {
   Cut c;
   const int group = heads / k_heads;
-  // A head of 64 columns or fewer has two wavefronts, and a workgroup two such heads, if there are two that read the same keys; 256 keys' values are too many
-  // loads for two wavefronts.
+  // A head of 64 columns or fewer has two wavefronts, and a workgroup two such heads, if there are two that read the same keys (4096 tokens of 128 heads, 16 of
+  // them to a key head: 125 us, 167 by one head a workgroup); 256 keys' values are too many loads for two wavefronts.
   c.teams = dv <= 64 && group > 1 ? 2 : 1;
   c.waves = dv <= 64 && (c.teams == 2 || dk <= 128) ? 2 : 4;
   c.across = c.teams > 1 ? (group + 1) / 2 : group * ((dv + 32 * c.waves - 1) / (32 * c.waves));
-  // As many parts as fill the device once: a part costs a second look at its keys and values.
-  const int64_t places = static_cast<int64_t>(dk > 128 ? 1 : 2) * compute_units(), columns = static_cast<int64_t>(c.across) * k_heads;
+  // As many parts as two workgroups a unit of the device: a part costs a second look at its keys and values, but few of them end together. By one, two and four
+  // workgroups a unit: 4096 tokens of 128 heads 156, 131 and 169 us, 16384 of 16 heads 141, 136 and 155 us; eight prompts of up to 2048 of 8 heads of 256 by 256, of which
+  // a unit has one at a time, by one 134 us, by two 124.
+  const int64_t places = 2 * static_cast<int64_t>(compute_units()), columns = static_cast<int64_t>(c.across) * k_heads;
   const int64_t even = (T * columns + places - 1) / places, size = (even + kChunk - 1) / kChunk * kChunk;
   c.size = static_cast<int>(size < kLeastPart ? kLeastPart : size);
   // No call of T rows or fewer has more: a part is no shorter than T columns / places.

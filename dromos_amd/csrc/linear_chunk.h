@@ -4,14 +4,17 @@
 //   out_i = scale (e^{G_i} S^T q_i + sum_{j <= i} (q_i . k_j) e^{G_i - G_j} b_j v_j)
 //   S    <- e^{G_63} S + sum_j k_j (e^{G_63 - G_j} b_j v_j)^T
 // Every exponent is a difference of sums at most 0, formed from sums in 64 bits (as two f32 each): nothing overflows, and near tokens lose nothing where the sums
-// are large. What is rounded to go into a product (weights, scaled values, the state) goes in as two bf16, a value and what its
-// rounding left: with one, a state would be right to 2^-9 only, and results carry its error on from chunk to chunk.
+// are large. What is rounded to go into a product goes in as bf16 terms, a value, what its rounding left, and so on: three of the values that a state is made of
+// (24 bits; with two, states were right to 2.6e-6, with one to 2^-9, and what a state has lost goes on from chunk to chunk), and of the state and the weights where results
+// are f32; two of those where results are rounded to bf16, 2^-8 of them, in any case.
 //
-// A wavefront owns 32 columns of a head's state, all its rows, in registers, for the whole of a sequence's part. Its layout is what
+// A wavefront owns 32 columns of a head's state in registers, all rows or (of more than 128 keys) one half of them, for the whole of a sequence's part. Its layout is what
 // makes that work: v_mfma_f32_32x32x16 leaves a lane with four neighbouring rows, and four others 8 further, of its column. Rows and columns are given to
 // the instruction in the order (0-3, 8-11, 4-7, 12-15) of every 16 (the transposing reads of LDS take any four neighbours from anywhere), and
 // so a lane's eight values are neighbours: the state is the next product's operand as it lies, an output's eight values are one
 // store. Products are transposed, out^T = S^T Q^T + V^T P^T, so that a row's factors are a lane's own.
+// Halves give each other what they have for the other's 32 tokens through LDS (a wavefront with all 256 rows leaves a SIMD to itself: eight prompts of up to 2048
+// of 8 heads of 256 by 256 168 us, 150 by halves).
 //
 // Queries, keys and values of a chunk stand in LDS, read along rows (16 bytes a lane) and across (ds_read_tr16), units of 16 bytes swizzled so that both
 // fall on all banks. The weights P of a head are made once by its wavefronts, 32 x 32 tiles on and below the diagonal, and shared through
@@ -41,7 +44,7 @@ struct ChunkArgs {
   int64_t numbers;  // of parts that the launch counts to
   int across;       // workgroups of a part and key head
   int sums_only;    // sequences have few parts at most: nothing runs through them in between
-  float* sums;      // [2 (T / size), heads] states as wavefronts hold them: parts' sums, then the states in front of them
+  float* sums;      // [2 (T / size), heads] states as wavefronts hold them: parts' sums, and what a sequence goes on from or the states in front of the parts
   double* logs;     // [2 (T / size), heads] logarithms of what the parts leave of what was in front of them
 };
 

@@ -145,3 +145,62 @@ def test_workspace_to_the_byte(hip, dk, dv, counts):
     out, kept = m.run(hip, workspace=space)
     m.check(out, kept, m.want(), SHARE)
     assert bool((space[need:] == 0xFF).all())
+
+
+@pytest.mark.parametrize("decay", ["log", "step"])
+@pytest.mark.parametrize("rows,dk,dv", [(7, 128, 64), (64, 64, 64), (200, 128, 128), (200, 256, 72), (700, 128, 64)])
+def test_states_and_f32_results_keep_their_precision(hip, rows, dk, dv, decay):
+    """As a whole, by 2-norms. A token's factors are off by 2^-22 each (an exponent up to 4 rounded, its exponential), 2^-23 on average and on their own, terms
+    and products by 2^-24, and twelve sums a chunk by 2^-24 each, 2^-22 together where they come as they like: under 2^-20."""
+    for out in (F, BF):
+        m = Mixer(Rows([rows], [rows + 9], [0]), 4, 2, dk, dv, decay, out=out, seed=rows + dk)
+        want = m.want()
+        got, kept = m.run(hip)
+        assert (kept[0].double().cpu() - want["states"][0]).norm() <= 2.0**-20 * want["states"][0].norm()
+        if out == F:
+            assert (got.double().cpu() - want["out"]).norm() <= 2.0**-20 * want["out"].norm()
+
+
+@pytest.mark.parametrize("counts", [[70, 3], [300, 0, 0, 400], [0, 0, 513, 0]])
+def test_no_lengths(hip, counts):
+    """No sequence begins with such a call."""
+    m = Mixer(Rows(counts, None, list(range(len(counts)))), 2, 1, 64, 64, "step", seed=1)
+    out, kept = m.run(hip)
+    m.check(out, kept, m.want(), SHARE)
+
+
+@pytest.mark.parametrize("most", [2, 8])
+def test_thousands_of_sequences(hip, most):
+    """More than the 64 x 64 that two turns of the search for a row's sequence tell apart; some are empty."""
+    g = torch.Generator().manual_seed(most)
+    counts = torch.randint(0, most + 1, (4200,), generator=g).tolist()
+    slots = torch.randperm(4200, generator=g).tolist()
+    rows = Rows(counts, [n + i % 3 for i, n in enumerate(counts)], slots)
+    m = Mixer(rows, 1, 1, 8, 8, "log", seed=most)
+    out, kept = m.run(hip)
+    m.check(out, kept, m.want(), SHARE)
+    x, weight, front = torch.randn(rows.T, 8, generator=g).to(BF), torch.randn(8, 4, generator=g), torch.randn(4200, 3, 8, generator=g).to(BF)
+    device = Rows(counts, rows.lengths, slots, device="cuda")
+    held, w, y = front.cuda(), weight.cuda(), torch.full((rows.T, 8), UNTOUCHED, dtype=BF, device="cuda")
+    # Bounds far above the real rows: pieces, and a search among them.
+    device.max_rows = 100
+    states = device.states(held, held, 4200)
+    hip("causal_conv", x.cuda(), BF16, 8, w, None, F32, 4, ACT_NONE, pointer(device.lx()), pointer(states), y, BF16, 8, rows.T, 8)
+    want, size, after = convolved(x, weight, None, False, rows, front, 4200)
+    share = 1.1 * 5 * 2.0**-24 * size
+    assert bool(((y.double().cpu() - want).abs() <= share + 2.0**-8 * 1.01 * (want.abs() + share)).all())
+    whole = front.double()
+    for slot, values in after.items():
+        whole[slot] = values
+    assert torch.equal(held.double().cpu(), whole)
+
+
+def test_bounds_above_the_real_rows(hip):
+    """One captured size for anything up to it: the same results whatever max_rows says, as long as the same form is taken."""
+    outs = []
+    for most in (160, 700, 100000):
+        m = Mixer(Rows([160, 5], [160, 30], [0, 1], T=700, max_rows=most), 4, 2, 128, 64, "step", True, BF, seed=3)
+        out, kept = m.run(hip)
+        m.check(out, kept, m.want(), SHARE)
+        outs.append((out, kept))
+    assert all(torch.equal(outs[0][i], o[i]) for o in outs[1:] for i in range(2))

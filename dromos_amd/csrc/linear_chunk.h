@@ -526,6 +526,8 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
           for (int e = 0; e < 8; ++e) v[e] = state[step / 2][step % 2 * 8 + e];
           split_eight<true>(v, held[now]);
         };
+        // A wavefront with products goes in front of one with vector arithmetic (here and below: 126.6 -> 124.3 us for the 4096 tokens).
+        __builtin_amdgcn_s_setprio(1);
         ready(0);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -547,6 +549,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
           }
           __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         if constexpr (kTiles > 0 && HALVES > 1) {  // the tile's products of the other half's keys
           const int from_other = from_half ^ 32 * kSteps, queries_at = L::kQueries + (block > 0) * 32 * L::kKeyPitch;
 #pragma unroll
@@ -757,6 +760,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
         }
         split_eight<false>(x, scaled_v[k % 2]);
       };
+      __builtin_amdgcn_s_setprio(1);
       ready(0);
 #pragma unroll
       for (int x = 0; x < kRows / 32; ++x) state[x] *= fade;
@@ -771,6 +775,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     __syncthreads();
     if (more) {
       put(chunk + 1);

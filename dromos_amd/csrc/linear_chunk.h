@@ -24,6 +24,10 @@
 // Long sequences are cut into parts where there are too few workgroups: a first kernel leaves each part's own sum (keys and values
 // only), and this one starts from the sums in front of its part; where there are many, a kernel in between runs through them and leaves the state in front of every
 // part.
+//
+// What bounds it: a wavefront's vector arithmetic (terms, exponentials, gates: 1200 instructions a chunk) and its products (104, 3300 cycles), one after
+// another in each of the two wavefronts that a SIMD has registers for. 4096 tokens of 128 heads of 128 by 64, 16 to a key head: 124 - 132 us (devices differ; sums 38,
+// outputs 100), 16384 of 16 heads of 128 by 128 131 - 136 us (42, 15 in between, 80), eight prompts of up to 2048 of 8 heads of 256 by 256 122 us (44, 91).
 #pragma once
 
 #include <type_traits>

@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 3) linear_step_kernel(co
   };
   ask(0);
 
-  // The decays, a token a lane. e^g in two parts: rounded, near 1, it is off to the same side token after token (after 4096 tokens of a
-  // memory as long, 3e-4 were missing).
+  // The decays, a token a lane. e^g in two parts: rounded, near 1, it is off to the same side token after token: up to 2^-25 of
+  // the state for each of as many tokens as it remembers.
   const float skip = p.skip ? p.skip[head] : 0.0f;
   float fades, lefts, weights = 1.0f;
   {

@@ -157,8 +157,9 @@ __device__ __forceinline__ Fade fade_of(float log) {
   return log > -0.5f ? Fade{high, less - (high - 1.0f)} : Fade{quick_exp(log), 0.0f};
 }
 
-// The numbers of a chunk's tokens. G_i (base 2) is a sum of integers, 2^-40 each, and so exact: its whole 256ths and a rest. Logarithms of -200 at
-// least keep 64 of them within the 24 bits of the former.
+// The numbers of a chunk's tokens. G_i (base 2) is a sum of integers of 2^-47, to which a logarithm is rounded in 64 bits, and exact beyond that (131072 tokens are off by
+// less than 2^-30 of a state however slow their decay; from f32's `x - floor(x)`, 1 - 2^-24 at most, they were by 1e-5): its nearest 256th and a rest of either sign, as exact as
+// f32 is near nothing. Logarithms of 200 at most keep the sum of 64 below 2^62 and its 256ths within 24 bits.
 // The factor of a row's weight of a token is a product where nothing in it can overflow or is large enough to lose bits: with R the sum up to the row's
 // half of the chunk, e^{G_i - R} times e^{R - G_j} b_j (`quick`: G falls by 24 at most in either half). Otherwise it is made from the difference.
 struct Tokens {
@@ -320,9 +321,9 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
     float log, weight;
     decay_of(p, head_numbers, next_raw, log, weight);
     if (chunk * kChunk + lane >= rows) log = 0.0f, weight = 1.0f;
-    const float units = log * (1.44269504f * 256.0f), whole_units = floorf(units);
-    const int64_t g = wave_scan(static_cast<int64_t>(static_cast<int>(whole_units)) << 32 | static_cast<uint32_t>((units - whole_units) * 0x1p32f));
-    const float high = static_cast<float>(static_cast<int>(g >> 32)) * 0x1p-8f, rest = static_cast<float>(static_cast<uint32_t>(g)) * 0x1p-40f;
+    const double units = static_cast<double>(log) * (1.4426950408889634 * 0x1p47);
+    const int64_t g = wave_scan(log == log ? static_cast<int64_t>(rint(units)) : 0), nearest = (g + (int64_t{1} << 38)) >> 39;
+    const float high = static_cast<float>(static_cast<int>(nearest)) * 0x1p-8f, rest = static_cast<float>(g - (nearest << 39)) * 0x1p-47f;
     auto of = [](float x, int token) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), token)); };
     const float last_high = of(high, kWave - 1), last_rest = of(rest, kWave - 1);
     // No update at all: an exponent far below; a NaN of a logarithm or a weight is all that is left of a column.

@@ -169,9 +169,9 @@ struct Tokens {
   float update[kChunk];  // e^{G_63 - G_j} b_j
   float seen[kChunk];    // scale e^{G_i}
   float fade;            // e^{G_63}, and what its rounding left of the chunks before
+  float left;            // what its own rounding leaves, for a state that no further chunk of the call follows
   float whole;           // the logarithm of e^{G_63}
   int quick;
-  float none;  // whole 16 bytes
 };
 
 template <int DK, int TW, int TEAMS, int HALVES, int TERMS>
@@ -345,13 +345,14 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
       t.seen[lane] = __builtin_amdgcn_exp2f(high + row) * (scaled ? 1.0f : p.scale);
     }
     t.update[lane] = __builtin_amdgcn_exp2f((last_high - high) + (last_rest - column));
-    // What a factor's rounding leaves goes into the next one: a state that lasts many chunks does not drift.
+    // What a factor's rounding leaves goes into the next one, and behind the last one into the state itself: one that lasts many chunks, or many calls of one, does not drift.
     const float whole = (last_high + last_rest) * 0.693147181f;
     const Fade fade = fade_of(whole);
     const float more = __builtin_fmaf(fade.high, carried, fade.low), factor = fade.high + more;
-    carried = (more - (factor - fade.high)) * __builtin_amdgcn_rcpf(factor);
+    const float left = more - (factor - fade.high);
+    carried = left * __builtin_amdgcn_rcpf(factor);
     if (!(fabsf(carried) < 1.0f)) carried = 0.0f;
-    if (lane == 0) t.whole = whole, t.fade = factor;
+    if (lane == 0) t.whole = whole, t.fade = factor, t.left = left;
   };
   if (counts) ask_decay(0);
 
@@ -765,10 +766,20 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
         }
         split_eight<false>(x, scaled_v[k % 2]);
       };
+      // In front of the products' first operands: behind them, the branch costs registers that are not there (45 spilled, 184 us for the 4096 tokens).
+      if (OUT && !more) {
+        const float left = t.left;
+#pragma unroll
+        for (int x = 0; x < kRows / 32; ++x)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) state[x][e] = __builtin_fmaf(state[x][e], fade, state[x][e] * left);
+      } else {
+#pragma unroll
+        for (int x = 0; x < kRows / 32; ++x) state[x] *= fade;
+      }
+      __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
       ready(0);
-#pragma unroll
-      for (int x = 0; x < kRows / 32; ++x) state[x] *= fade;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k) {

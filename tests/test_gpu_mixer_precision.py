@@ -1,5 +1,7 @@
 """What lx_linear_attention keeps of f32 where little things add up."""
 
+import math
+
 import pytest
 import torch
 
@@ -45,3 +47,21 @@ def test_slow_decays_of_a_prompt(hip, rows, rate):
     errors = f.errors(rows)
     assert abs(errors.mean().item()) <= 2.0**-22 * abs(rows * rate) + 2.0**-23
     assert errors.abs().max().item() <= 2.0**-22 * abs(rows * rate) + 2.0**-18
+
+
+@pytest.mark.parametrize("rows,pieces", [(1, [1]), (6, [1] * 6), (7, [7]), (8, [8]), (64, [64]), (130, [128, 2])])
+def test_slow_decays_of_many_short_calls(hip, rows, pieces):
+    """8192 calls; a state is rounded once a piece. That is nothing random where a state falls by few steps at a time (6 rows: 4e-6 of a value, to one side), so what is
+    compared with is the same in 64 bits rounded as often. Beside that the logarithms' errors, 2^-22 of them as in a prompt, and their last places, 2^-21 of all tokens."""
+    calls, whole = 8192, -0.57
+    f = Fading(hip, rows, whole / (calls * rows), 2)
+    for _ in range(calls):
+        f.call()
+    rate, state = f.rate.double().item(), f.before.clone()
+    fades = [math.exp(rate * n) for n in pieces]
+    for _ in range(calls):
+        for fade in fades:
+            state = (state.double() * fade).float()
+    apart = f.state[0, 0].double().cpu() / state.double() - 1
+    assert abs(apart.mean().item()) <= 2.0**-22 * -whole + 2.0**-21
+    assert apart.abs().max().item() <= 2.0**-22 * -whole + 2.0**-19

@@ -82,7 +82,7 @@ template <int DK, int TW, int TEAMS, bool OUT>
 int launch_chunks(ChunkArgs a, int64_t numbers, hipStream_t s) {
   a.numbers = numbers;
   const int64_t groups = (numbers * a.l.k_heads + 7) / 8 * 8 * a.across;
-  const bool plain = a.l.type == LX_BF16 && a.l.wide && (!a.l.gate || a.l.gate_type == LX_BF16) && positive(a.l.scale);
+  const bool plain = a.l.type == LX_BF16 && a.l.wide && (!a.l.gate || a.l.gate_type == LX_BF16);
   if constexpr (OUT) {
     if (plain && a.l.out_type == LX_BF16) return launch_kernel<DK, TW, TEAMS, true, true, 2>(a, groups, s);
     return plain ? launch_kernel<DK, TW, TEAMS, true, true, 3>(a, groups, s) : launch_kernel<DK, TW, TEAMS, true, false, 3>(a, groups, s);

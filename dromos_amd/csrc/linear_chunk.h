@@ -161,10 +161,11 @@ __device__ __forceinline__ Fade fade_of(float log) {
 // less than 2^-30 of a state however slow their decay; from f32's `x - floor(x)`, 1 - 2^-24 at most, they were by 1e-5): its nearest 256th and a rest of either sign, as exact as
 // f32 is near nothing. Logarithms of 200 at most keep the sum of 64 below 2^62 and its 256ths within 24 bits.
 // The factor of a row's weight of a token is a product where nothing in it can overflow or is large enough to lose bits: with R the sum up to the row's
-// half of the chunk, e^{G_i - R} times e^{R - G_j} b_j (`quick`: G falls by 24 at most in either half). Otherwise it is made from the difference.
+// half of the chunk, e^{G_i - R} times e^{R - G_j} b_j (`quick`: G falls by 24 at most in either half, and the scale is no extreme). Otherwise it is made from the difference.
+// b and the scale are factors throughout: as parts of an exponent, their logarithms' roundings were 2^-21 of an update of 1000.
 struct Tokens {
-  float row[kChunk];     // quick: scale e^{G_i - R}; otherwise the rest of G_i + log(scale)
-  float column[kChunk];  // quick: e^{R - G_j} b_j, R of the token's own half; otherwise the rest of G_j - log(b_j)
+  float row[kChunk];     // quick: scale e^{G_i - R}; otherwise b_i
+  float column[kChunk];  // quick: e^{R - G_j} b_j, R of the token's own half; otherwise the rest of G_j
   float other[kChunk];   // quick: the same with R of the second half, of tokens of the first one; otherwise the 256ths of G_i
   float update[kChunk];  // e^{G_63 - G_j} b_j
   float seen[kChunk];    // scale e^{G_i}
@@ -201,10 +202,7 @@ __device__ __forceinline__ void buffer_store(__amdgpu_buffer_rsrc_t b, unsigned 
 // Bytes of m rows of `width` values, `ld` apart.
 __device__ __forceinline__ int rows_bytes(int m, int64_t ld, int width, int size) { return m > 0 ? ((m - 1) * static_cast<int>(ld) + width) * size : 0; }
 
-// A scale that can be part of an exponent.
-__host__ __device__ __forceinline__ bool positive(float scale) { return scale > 1e-30f && scale < 1e30f; }
-
-// OUT: outputs and states; otherwise a part's sum of a long sequence only. PLAIN: bf16 that can be moved 16 bytes at a time, a positive scale, gates bf16 or
+// OUT: outputs and states; otherwise a part's sum of a long sequence only. PLAIN: bf16 that can be moved 16 bytes at a time, gates bf16 or
 // none (everything else in its own kernel: its loads and stores, a value at a time perhaps, would cost this one registers).
 template <int DK, int TW, int TEAMS, int HALVES, bool OUT, bool PLAIN, int TERMS>
 __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW * TEAMS * HALVES == 2 ? 1 : 2) linear_chunk_kernel(const ChunkArgs c) {
@@ -306,9 +304,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
   // ---- the decays -----------------------------------------------------------------------------------------------------
   // A token a lane: asked for two chunks ahead, made ready one ahead, by the team's last wavefront.
   Tokens* const tokens = reinterpret_cast<Tokens*>(lds + L::kTokens) + 2 * team;
-  // A positive scale is part of the rows' exponents, another one multiplied in. The skip is part of a row's weight of its own token.
-  const bool scaled = PLAIN || positive(p.scale);
-  const float log_scale = scaled ? __builtin_amdgcn_logf(p.scale) : 0.0f;
+  // The scale is part of the rows' factors, the skip of a row's weight of its own token.
   const bool counts = mate == TW - 1 && half == HALVES - 1;
   const HeadDecay head_numbers = head_decay(p, head);
   uint32_t next_raw;
@@ -326,25 +322,25 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
     const float high = static_cast<float>(static_cast<int>(nearest)) * 0x1p-8f, rest = static_cast<float>(g - (nearest << 39)) * 0x1p-47f;
     auto of = [](float x, int token) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), token)); };
     const float last_high = of(high, kWave - 1), last_rest = of(rest, kWave - 1);
-    // No update at all: an exponent far below; a NaN of a logarithm or a weight is all that is left of a column.
-    const float column = rest - (weight == 1.0f ? 0.0f : fmaxf(__builtin_amdgcn_logf(weight), -1e5f)) + (log - log);
+    // A NaN of a logarithm is one of its token's weight.
+    const float by = weight + (log - log);
     if constexpr (OUT) {
-      const float row = rest + log_scale, half_high = of(high, 31), half_rest = of(rest, 31);
+      const float half_high = of(high, 31), half_rest = of(rest, 31);
       const float from_high = lane < 32 ? 0.0f : half_high, from_rest = lane < 32 ? 0.0f : half_rest, most = weight == weight ? fmaxf(weight, 1.0f) : 1.0f;
-      const bool quick = half_high > -24.0f && last_high - half_high > -24.0f && __all(most < 0x1p60f);
+      const bool quick = half_high > -24.0f && last_high - half_high > -24.0f && __all(most < 0x1p60f) && fabsf(p.scale) > 0x1p-100f && fabsf(p.scale) < 0x1p100f;
       if (quick) {
-        t.row[lane] = __builtin_amdgcn_exp2f((high - from_high) + (row - from_rest)) * (scaled ? 1.0f : p.scale);
-        t.column[lane] = __builtin_amdgcn_exp2f((from_high - high) + (from_rest - column));
-        t.other[lane] = __builtin_amdgcn_exp2f((half_high - high) + (half_rest - column));
+        t.row[lane] = __builtin_amdgcn_exp2f((high - from_high) + (rest - from_rest)) * p.scale;
+        t.column[lane] = __builtin_amdgcn_exp2f((from_high - high) + (from_rest - rest)) * by;
+        t.other[lane] = __builtin_amdgcn_exp2f((half_high - high) + (half_rest - rest)) * by;
       } else {
-        t.row[lane] = row;
-        t.column[lane] = column;
+        t.row[lane] = by;
+        t.column[lane] = rest;
         t.other[lane] = high;
       }
       if (lane == 0) t.quick = quick;
-      t.seen[lane] = __builtin_amdgcn_exp2f(high + row) * (scaled ? 1.0f : p.scale);
+      t.seen[lane] = __builtin_amdgcn_exp2f(high + rest) * p.scale;
     }
-    t.update[lane] = __builtin_amdgcn_exp2f((last_high - high) + (last_rest - column));
+    t.update[lane] = __builtin_amdgcn_exp2f((last_high - high) + (last_rest - rest)) * by;
     // What a factor's rounding leaves goes into the next one, and behind the last one into the state itself: one that lasts many chunks, or many calls of one, does not drift.
     const float whole = (last_high + last_rest) * 0.693147181f;
     const Fade fade = fade_of(whole);
@@ -487,15 +483,16 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
                                                       eight_at(lds, L::kQueries + ib * 32 * L::kKeyPitch + (from ^ 32 * k)), w, 0, 0, 0);
           if (k % 2) __builtin_amdgcn_sched_barrier(0);  // no more reads ahead than registers
         }
-        const float high = t.other[32 * ib + n], row = t.row[32 * ib + n];
+        const float high = t.other[32 * ib + n], rest = t.column[32 * ib + n];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int token = 8 * g + 4 * h;
-          const f32x4 highs = *reinterpret_cast<const f32x4*>(t.other + 32 * jb + token), columns = *reinterpret_cast<const f32x4*>(t.column + 32 * jb + token);
+          const f32x4 highs = *reinterpret_cast<const f32x4*>(t.other + 32 * jb + token), rests = *reinterpret_cast<const f32x4*>(t.column + 32 * jb + token);
+          const f32x4 by = *reinterpret_cast<const f32x4*>(t.row + 32 * jb + token);
           float v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[e] = w[4 * g + e] * __builtin_amdgcn_exp2f((high - highs[e]) + (row - columns[e])) * (scaled ? 1.0f : p.scale);
+            v[e] = w[4 * g + e] * __builtin_amdgcn_exp2f((high - highs[e]) + (rest - rests[e])) * by[e] * p.scale;
             v[e] = token + e <= until ? v[e] : 0.0f;
           }
           put_weights(block, g, v);

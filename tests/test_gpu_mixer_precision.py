@@ -1,4 +1,4 @@
-"""What lx_linear_attention keeps of f32 where little things add up."""
+"""What lx_linear_attention keeps of f32 where little things add up or sizes are extreme."""
 
 import math
 
@@ -6,10 +6,10 @@ import pytest
 import torch
 
 from dromos_amd.abi import BF16, DECAY_HEAD, F32, LxDecay, LxKv8Batch, LxStates
-from mixer import pointer
+from mixer import Mixer, Rows, pointer
 
 pytestmark = pytest.mark.gpu
-BF = torch.bfloat16
+BF, F = torch.bfloat16, torch.float32
 
 
 class Fading:
@@ -65,3 +65,42 @@ def test_slow_decays_of_many_short_calls(hip, rows, pieces):
     apart = f.state[0, 0].double().cpu() / state.double() - 1
     assert abs(apart.mean().item()) <= 2.0**-22 * -whole + 2.0**-21
     assert apart.abs().max().item() <= 2.0**-22 * -whole + 2.0**-19
+
+
+def relative(got, want):
+    errors = got.double().cpu() / want - 1
+    return errors.square().mean().sqrt().item(), errors.abs().max().item()
+
+
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (256, 64)])
+def test_updates_weights(hip, far, dk, dv):
+    """A row of the state for each token, and a column of the values: states and results are single weights, e^{G - G_j} b_j. Steps that are their x as they stand
+    (100 and more), decays of hardly anything. An exponential is right to 2^-23, a product to 2^-24: of a state one and one, and 2^-24 for terms and sums, 2^-22
+    together, 2^-23.6 on average (each anywhere within its bound); of a result's weight two and five, 2^-20.8 and 2^-23. `far`: a token that all before it is forgotten at."""
+    rows, heads = 64, 4
+    m = Mixer(Rows([rows], [rows], [0]), heads, 1, dk, dv, "step", out=F, seed=dk, spare=0)
+    g = torch.Generator().manual_seed(9)
+    m.x = torch.rand(rows, heads, generator=g) * 1900 + 100
+    m.bias, m.rate = None, -torch.rand(heads, generator=g) * 1e-5
+    if far:
+        m.x[0], m.rate[:] = 1e7, -1e-5
+    m.k, m.q, m.v = torch.zeros(rows, dk, dtype=BF), torch.zeros(rows, dk, dtype=BF), torch.zeros(rows, heads, dv, dtype=BF)
+    for t in range(rows):
+        m.k[t, t % dk], m.v[t, :, t % dv] = 1.0, 1.0
+    m.q[:] = 1.0
+    m.v = m.v.view(rows, heads * dv)
+    m.scale = 0.5
+    b = m.x.double()
+    sums = (b * m.rate.double()).cumsum(0)
+    out, kept = m.run(hip)
+    at = torch.arange(rows)
+    state = kept[0].cpu()[:, at % dk, at % dv].t()  # [rows, heads]
+    mean, worst = relative(state[1:], (torch.exp(sums[-1] - sums) * b)[1:])
+    assert mean <= 2.0**-23.3 and worst <= 2.0**-22
+    seen = out.cpu().view(rows, heads, dv)[:, :, at % dv]  # [row, head, token]
+    want = 0.5 * torch.exp(sums[:, :, None] - sums.t()[None]) * b.t()[None]
+    some = (at[:, None] >= at)[:, None].expand(-1, heads, -1) & (at > 0)
+    mean, worst = relative(seen[some], want[some])
+    assert mean <= 2.0**-22.9 and worst <= 2.0**-20.8
+    assert bool((seen[(at[:, None] < at)[:, None].expand(-1, heads, -1)] == 0).all())

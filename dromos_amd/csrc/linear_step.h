@@ -14,7 +14,8 @@
 
 namespace dro {
 
-// COLS lanes side by side in a row of the state; ROWS rows of it a lane. PLAIN: queries, keys, values and gates bf16 that can be moved 16 bytes at
+// COLS lanes side by side in a row of the state; ROWS rows of it a lane. Sums over the rows are made in the same order by four lanes of up to 16 rows and by eight of up to
+// 32, whose two halves are summed apart: which of them a call takes goes by the number of its sequences, and no sequence's bits may. PLAIN: queries, keys, values and gates bf16 that can be moved 16 bytes at
 // a time (everything else in its own kernel: the registers of its loads would be missing here).
 template <int COLS, int ROWS, bool PLAIN>
 __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 3) linear_step_kernel(const LinearArgs p) {
@@ -102,9 +103,11 @@ __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 3) linear_step_kernel(co
     const float fade = of_token(fades, i), left = of_token(lefts, i), weight = of_token(weights, i);
     const f32x4 raw = four_of(value), z = four_of(gate), v = raw * weight;
     if (i + 1 < rows) ask(i + 1);
-    f32x4 o = {};
+    constexpr int kSums = COLS == 8 && ROWS > 8 ? 2 : 1;
+    f32x4 sums[kSums] = {};
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
+      f32x4& o = sums[r * kSums / ROWS];
       const uint32_t two_k = ks[r / 8][r % 8 / 2], two_q = qs[r / 8][r % 8 / 2];
       const float k = __uint_as_float(r % 2 ? two_k & 0xffff0000u : two_k << 16), q = __uint_as_float(r % 2 ? two_q & 0xffff0000u : two_q << 16);
 #pragma unroll
@@ -118,10 +121,12 @@ __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 3) linear_step_kernel(co
       }
       if (r % 2) __builtin_amdgcn_sched_barrier(0);  // left alone, products of all rows are made before the first sum, in registers that are not there
     }
+    f32x4 o = sums[0];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (COLS == 4) o[j] += dpp_move<0x124>(o[j]);  // row_ror:4
-      o[j] += dpp_move<0x128>(o[j]);                 // row_ror:8
+      if (COLS == 4) o[j] += dpp_move<0x124>(o[j]);                // row_ror:4
+      if (kSums > 1) o[j] += dpp_move<0x128>(sums[kSums - 1][j]);  // as that adds them: the first rows' half and the last ones', then those between
+      o[j] += dpp_move<0x128>(o[j]);                               // row_ror:8
       float a, b;
       swap_halves<true>(o[j], a, b);
       const float half = a + b;

@@ -1,4 +1,4 @@
-"""What lx_linear_attention keeps of f32 where little things add up or sizes are extreme."""
+"""What lx_linear_attention keeps of f32 where little things add up or sizes are extreme, and that a sequence's bits do not depend on how many others a call has."""
 
 import math
 
@@ -104,3 +104,19 @@ def test_updates_weights(hip, far, dk, dv):
     mean, worst = relative(seen[some], want[some])
     assert mean <= 2.0**-22.9 and worst <= 2.0**-20.8
     assert bool((seen[(at[:, None] < at)[:, None].expand(-1, heads, -1)] == 0).all())
+
+
+@pytest.mark.parametrize("heads,k_heads,dk,dv", [(32, 32, 128, 128), (32, 8, 256, 64), (64, 4, 72, 40), (32, 32, 64, 64)])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_bits_do_not_depend_on_how_many_sequences(hip, rows, heads, k_heads, dk, dv):
+    """f32 results and states, bit for bit, of the first sequence by itself, with one more, with 40 more."""
+    alone = Mixer(Rows([rows], [rows + 2], [1], max_rows=rows), heads, k_heads, dk, dv, "step", True, BF, out=F, seed=4)
+    first, state = alone.run(hip)
+    for others in (1, 40):
+        counts, slots = [rows] * (1 + others), [1, 0] + list(range(2, others + 1))
+        more = Mixer(Rows(counts, [rows + 2] + [9] * others, slots, max_rows=rows), heads, k_heads, dk, dv, "step", True, BF, out=F, seed=5)
+        for name in ("q", "k", "v", "x", "gate"):
+            getattr(more, name)[:rows] = getattr(alone, name)
+        more.rate, more.bias, more.skip, more.state[1] = alone.rate, alone.bias, alone.skip, alone.state[1]
+        out, kept = more.run(hip)
+        assert torch.equal(out[:rows], first) and torch.equal(kept[1], state[1]), others

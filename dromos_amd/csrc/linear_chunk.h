@@ -148,15 +148,6 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
   return scan_step<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
 }
 
-// e^log in two parts: rounded, near 1, it is off to the same side time after time.
-struct Fade {
-  float high, low;
-};
-__device__ __forceinline__ Fade fade_of(float log) {
-  const float less = quick_expm1(log), high = 1.0f + less;
-  return log > -0.5f ? Fade{high, less - (high - 1.0f)} : Fade{quick_exp(log), 0.0f};
-}
-
 // The numbers of a chunk's tokens. G_i (base 2) is a sum of integers of 2^-47, to which a logarithm is rounded in 64 bits, and exact beyond that (131072 tokens are off by
 // less than 2^-30 of a state however slow their decay; from f32's `x - floor(x)`, 1 - 2^-24 at most, they were by 1e-5): its nearest 256th and a rest of either sign, as exact as
 // f32 is near nothing. Logarithms of 200 at most keep the sum of 64 below 2^62 and its 256ths within 24 bits.
@@ -346,9 +337,10 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
     const Fade fade = fade_of(whole);
     const float more = __builtin_fmaf(fade.high, carried, fade.low), factor = fade.high + more;
     const float left = more - (factor - fade.high);
+    const Fade last = fade_from(factor, left);
     carried = left * __builtin_amdgcn_rcpf(factor);
     if (!(fabsf(carried) < 1.0f)) carried = 0.0f;
-    if (lane == 0) t.whole = whole, t.fade = factor, t.left = left;
+    if (lane == 0) t.whole = whole, t.fade = (chunk + 1) * kChunk < rows ? factor : last.high, t.left = last.low;
   };
   if (counts) ask_decay(0);
 

@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 3) linear_step_kernel(co
   {
     float log = 0.0f;
     if (lane < rows) decay_of(p, head_decay(p, head), decay_raw(p, first + lane, head), log, weights);
-    const float less = quick_expm1(log), slow = 1.0f + less;
-    fades = log > -0.5f ? slow : quick_exp(log), lefts = log > -0.5f ? less - (slow - 1.0f) : 0.0f;
+    const Fade fade = fade_of(log);
+    fades = fade.high, lefts = fade.low;
   }
   auto of_token = [&](float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); };
 

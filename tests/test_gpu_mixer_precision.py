@@ -120,3 +120,30 @@ def test_bits_do_not_depend_on_how_many_sequences(hip, rows, heads, k_heads, dk,
         more.rate, more.bias, more.skip, more.state[1] = alone.rate, alone.bias, alone.skip, alone.state[1]
         out, kept = more.run(hip)
         assert torch.equal(out[:rows], first) and torch.equal(kept[1], state[1]), others
+
+
+@pytest.mark.parametrize("rate", [0.0, -1e-4, -0.3, -3.0])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 64), (256, 32)])
+@pytest.mark.parametrize("rows", [1, 5, 70, 400])
+def test_infinities_of_a_state(hip, rows, dk, dv, rate):
+    """An infinity of a state stays one and where it is, unless all that a chunk leaves of a state is nothing in f32 (e^-192 < 2^-149), whose product with it is a NaN. Token by
+    token its column's results are the sum's; by chunks they are no numbers (an infinity or a NaN). All others are as they are without it."""
+    m = Mixer(Rows([rows], [rows + 7], [0]), 2, 1, dk, dv, "head", out=F, seed=rows + dk)
+    m.rate[:] = rate
+    clean, kept = m.run(hip)
+    m.state[0, 0, 3, 5], m.state[0, 1, dk - 1, dv - 1] = float("inf"), float("-inf")
+    out, after = m.run(hip)
+    kept[0, 0, 3, 5], kept[0, 1, dk - 1, dv - 1] = float("inf"), float("-inf")
+    if rows > 6 and 64 * rate < -150:
+        for at in ((0, 0, 3, 5), (0, 1, dk - 1, dv - 1)):
+            assert not math.isfinite(after[at].item())
+            after[at] = kept[at]
+    assert torch.equal(after, kept)
+    clean, out = clean.view(rows, 2, dv), out.view(rows, 2, dv)
+    for head, column, row, sign in ((0, 5, 3, 1.0), (1, dv - 1, dk - 1, -1.0)):
+        seen = out[:, head, column].clone()
+        assert not bool(torch.isfinite(seen).any())
+        if rows <= 6:
+            assert torch.equal(seen, sign * m.q[:, row].float().cuda().sign() * float("inf"))
+        out[:, head, column] = clean[:, head, column]
+    assert torch.equal(out, clean)

@@ -124,13 +124,14 @@ __device__ __forceinline__ int mix_slot(const MixStates& t, int s) {
   return slot >= 0 && slot < t.count ? slot : -1;
 }
 
-// v / (1 + exp(-v)), right to 2^-21: the exponent's product in two parts, one reciprocal in place of a division.
+// v / (1 + exp(-v)), right to 2^-21, of any v: the exponent's product in two parts, one reciprocal in place of a division. Below -87, where that would be
+// no normal number, nothing (the value is less than 2e-36).
 __device__ __forceinline__ float quick_silu(float v) {
-  const float x = -fmaxf(v, -87.0f), t = x * 1.44269502f;
+  const float x = fminf(fmaxf(-v, -87.0f), 87.0f), t = x * 1.44269502f;
   const float rest = __builtin_fmaf(x, 1.44269502f, -t);  // what t's rounding left, exactly
   float e = __builtin_amdgcn_exp2f(t);
   e = __builtin_fmaf(e, __builtin_fmaf(x, 1.334976e-8f, rest * 0.693147181f), e);  // log2(e) - 1.44269502 is 1.92596e-8
-  return v * __builtin_amdgcn_rcpf(1.0f + e);
+  return v * (v < -87.0f ? 0.0f : __builtin_amdgcn_rcpf(1.0f + e));
 }
 
 inline bool mix_type(lx_dtype t) { return t == LX_F32 || t == LX_BF16; }

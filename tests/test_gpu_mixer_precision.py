@@ -1,12 +1,13 @@
-"""What lx_linear_attention keeps of f32 where little things add up or sizes are extreme, and that a sequence's bits do not depend on how many others a call has."""
+"""What lx_causal_conv and lx_linear_attention keep of f32 where little things add up or sizes are extreme, and that a sequence's bits do not depend on how many others
+a call has."""
 
 import math
 
 import pytest
 import torch
 
-from dromos_amd.abi import BF16, DECAY_HEAD, F32, LxDecay, LxKv8Batch, LxStates
-from mixer import Mixer, Rows, pointer
+from dromos_amd.abi import ACT_SILU, BF16, DECAY_HEAD, DTYPE, F32, LxDecay, LxKv8Batch, LxStates
+from mixer import UNTOUCHED, Mixer, Rows, pointer
 
 pytestmark = pytest.mark.gpu
 BF, F = torch.bfloat16, torch.float32
@@ -147,3 +148,36 @@ def test_infinities_of_a_state(hip, rows, dk, dv, rate):
             assert torch.equal(seen, sign * m.q[:, row].float().cuda().sign() * float("inf"))
         out[:, head, column] = clean[:, head, column]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("gate", [BF, F])
+@pytest.mark.parametrize("rows", [3])
+def test_gates_of_f32_results(hip, rows, gate):
+    """silu right to 2^-21 at any size, and to 2e-36 where it is less; keys and queries of zero, so that a result is its gate's factor (of two products, 2^-23)."""
+    heads, dv = 2, 64
+    m = Mixer(Rows([rows], [rows], [0]), heads, 1, 64, dv, "head", True, gate, out=F, seed=rows)
+    m.k.zero_(), m.q.zero_(), m.v.fill_(1.0), m.skip.fill_(1.0)
+    m.gate = ((torch.rand(rows, heads * dv, generator=torch.Generator().manual_seed(3)) - 0.5) * 176).to(gate)
+    m.gate[0, :8] = torch.tensor([0.0, 1e30, -1e30, 3e38, -3e38, float("inf"), -90.0, -104.0]).to(gate)
+    out, _ = m.run(hip)
+    z = m.gate.double()
+    want = z / (1 + torch.exp(-z))
+    out = out.double().cpu()
+    assert out[0, 5].item() == float("inf")
+    out[0, 5] = want[0, 5] = 0.0
+    assert bool(((out - want).abs() <= (2.0**-21 + 2.0**-23) * want.abs() + 2e-36).all())
+
+
+@pytest.mark.parametrize("out", [F, BF])
+def test_silu_of_a_convolution(hip, out):
+    """As the gates', sums of f32 that are their last row as it stands; bf16 results' own rounding beside 2^-17."""
+    C, z = 64, torch.cat([torch.linspace(-88, 88, 52), torch.tensor([1e30, -1e30, 3e38, -3e38, -90.0, -104.0, -1e5, 1e5, 0.0, -0.5, 300.0, float("inf")])])
+    x = torch.zeros(2, C)
+    x[1] = z
+    weight, y = torch.tensor([[0.0, 1.0]] * C).cuda(), torch.full((2, C), UNTOUCHED, dtype=out, device="cuda")
+    rows = Rows([2], [2], device="cuda")
+    hip("causal_conv", x.cuda(), F32, C, weight, None, F32, 2, ACT_SILU, pointer(rows.lx()), None, y, DTYPE[out], C, 2, C)
+    got, want = y[1].double().cpu(), z.double() / (1 + torch.exp(-z.double()))
+    assert got[-1].item() == float("inf")
+    share = 2.0**-21 if out == F else 2.0**-17 + 2.0**-8 * 1.01
+    assert bool(((got - want).abs()[:-1] <= share * want.abs()[:-1] + 2e-36).all())

@@ -28,7 +28,7 @@ struct LinearArgs {
 // numbers (and exact) where a state is forgotten altogether.
 constexpr float kForgotten = -200.0f;
 
-// z / (1 + exp(-z)) as a gate: right to 2^-21 near zero, 2^-24 |z| beyond.
+// z / (1 + exp(-z)) as a gate of bf16 results, whose rounding is 2^-8: right to 2^-21 near zero, 2^-24 |z| beyond.
 __device__ __forceinline__ float gate_of(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
 
 // The functions of a decay without the library's care for every argument: a wavefront makes a chunk's while the others wait for it. log(1 + u), u in 0 .. 1, and

@@ -696,7 +696,8 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const uint32_t pair = gate[i][a][e / 2];
-                o[e] *= gate_of(__uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16));
+                const float z = __uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16);
+                o[e] *= TERMS > 2 ? quick_silu(z) : gate_of(z);
               }
             }
             const unsigned at = my_column + 16 * a < p.dv ? (from + (i + half) * static_cast<unsigned>(32 * p.ld_out) + 16 * a) * size : kOutside;
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
               for (int e = 0; e < 8; e += 4) {
                 const f32x4 z = load_four(p.gate, p.gate_type, p.wide, row * p.ld_gate + column_at + e);
 #pragma unroll
-                for (int f = 0; f < 4; ++f) o[e + f] *= gate_of(z[f]);
+                for (int f = 0; f < 4; ++f) o[e + f] *= quick_silu(z[f]);
               }
             }
             store_four(p.out, p.out_type, p.wide, row * p.ld_out + column_at, f32x4{o[0], o[1], o[2], o[3]});

@@ -151,7 +151,7 @@ def test_infinities_of_a_state(hip, rows, dk, dv, rate):
 
 
 @pytest.mark.parametrize("gate", [BF, F])
-@pytest.mark.parametrize("rows", [3])
+@pytest.mark.parametrize("rows", [3, 70, 300])
 def test_gates_of_f32_results(hip, rows, gate):
     """silu right to 2^-21 at any size, and to 2e-36 where it is less; keys and queries of zero, so that a result is its gate's factor (of two products, 2^-23)."""
     heads, dv = 2, 64

@@ -178,6 +178,8 @@ int lx_linear_attention(const void* q, const void* k, const void* v, lx_dtype dt
   p.b = mix_batch(*batch, T);
   p.states = mix_states(states);
   if (p.b.max_rows == 0 || p.b.seqs == 0) return kOk;
+  // Other columns' workgroups still read what a result would replace.
+  if (out == q || out == k || out == v || out == gate || out == p.x) return fail(kInvalid);
   const int st = p.b.max_rows <= kMostSteps ? steps(p, as_stream(stream)) : chunks(p, workspace, as_stream(stream));
   return st ? fail(st) : kOk;
 }

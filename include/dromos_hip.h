@@ -360,7 +360,7 @@ typedef struct {
  *   LX_DECAY_HEAD  g = rate[h], b = 1
  *   LX_DECAY_LOG   g = x[t, h] * rate[h] (rate null: 1), b = 1
  *   LX_DECAY_STEP  d = log(1 + exp(x[t, h] + bias[h])) (bias null: 0), g = d * rate[h] (rate null: -1), b = d
- * q, k and v all bf16 or all f32 (rounded to bf16, as lx_gemm_w's BF16 math does), out f32 or bf16, apart from what is read, row strides in elements, up to
+ * q, k and v all bf16 or all f32 (rounded to bf16, as lx_gemm_w's BF16 math does), out f32 or bf16, apart from what is read (out that is q, k, v, gate or x is refused), row strides in elements, up to
  * 2^22; states f32 [count, heads, dk, dv], 16-byte aligned, or null. Calls of few rows a sequence go token by token in f32, longer ones by chunks of 64 tokens
  * on the matrix cores: f32 factors (weights of tokens, values times their decay, the state) enter products there as bf16 terms, three of them for
  * states and for f32 results (24 bits are kept), two for bf16 results (16 bits), and sums are f32. An infinity of a state stays one where keys and values are finite;

@@ -26,3 +26,13 @@ def test_strides_refused(lx, changes):  # noqa: F811
 def test_a_workspace_is_asked_for(lx):  # noqa: F811
     """Rows enough for parts, and no workspace: refused before anything is launched."""
     assert linear(lx, T=4096, batch=ctypes.pointer(abi.LxKv8Batch(2, HERE, HERE, None, 0, 4096, 0)), decay=decay(abi.DECAY_STEP, HERE, F32, 4)) == 1
+
+
+@pytest.mark.parametrize("over", ["q", "k", "v", "gate", "x"])
+def test_results_over_an_input_refused(lx, over):  # noqa: F811
+    """One row of a sequence, every tensor at a place of its own but for one."""
+    places = {"q": HERE, "k": HERE + 256, "v": HERE + 512, "gate": HERE + 1024, "x": HERE + 1536}
+    at = dict(places)
+    x = at.pop("x")
+    one = ctypes.pointer(abi.LxKv8Batch(1, HERE, HERE, None, 0, 1, 0))
+    assert linear(lx, T=1, batch=one, states=None, decay=decay(abi.DECAY_STEP, x, F32, 4), out=places[over], **at) == 1

@@ -5,9 +5,10 @@
 
 namespace dro {
 
-// The cosines and sines of N angles at a position, from quarter turns a position. The product of a 31-bit and a 53-bit number is right to 2^-53 in 64 bits;
-// whole quarter turns are taken off it there, so what is left of a far position is as good as of a near one. The rest u, an
-// eighth of a turn at most, goes into Taylor's series in f32 (what they leave off is below 2^-29 and 2^-32).
+// The cosines and sines of N angles at a position, from quarter turns a position. The product of a 31-bit and a 53-bit number is right to 2^-53 in 64 bits, and so is the
+// second of them: the angle is off by 2^-52 of itself. Whole quarter turns are taken off it there, so up to 2^26 radians what is left of a far position
+// is as good as of a near one, to f32's rounding (2^-25); at 2^31 it is 2^-21 off. The rest u, an eighth of a turn at most, goes into Taylor's series in f32 (what they leave
+// off is below 2^-29 and 2^-32).
 template <int N>
 __device__ __forceinline__ void angles(const double (&quarters)[N], int position, float* c, float* s) {
 #pragma unroll

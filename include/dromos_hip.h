@@ -330,7 +330,7 @@ typedef struct {
   int count;
 } lx_states;
 /* lx_rotate: y[t, h, :rot] = amplitude * x[t, h, :rot] turned by the angles p * freq[i], i < rot / 2 (f32 on the device; formed and reduced in
- * 64 bits), pairs (i, i + rot / 2), or (2 i, 2 i + 1) where `interleaved`: (a, b) -> (a cos - b sin, b cos + a sin); the values behind them as
+ * 64 bits: 2^-52 of themselves off), pairs (i, i + rot / 2), or (2 i, 2 i + 1) where `interleaved`: (a, b) -> (a cos - b sin, b cos + a sin); the values behind them as
  * they are. rot even (0: a copy), dim up to 1024. p is positions[t] (any int32; batch may be null then and every row counts) or, where positions is
  * null, the batch's. x and y f32 or bf16, row strides in elements (heads behind one another); y may be x where type and stride agree.
  * Queries and keys that lie side by side in a row are one call. T * heads < 2^31.

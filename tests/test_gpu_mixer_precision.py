@@ -1,7 +1,8 @@
-"""What lx_causal_conv and lx_linear_attention keep of f32 where little things add up or sizes are extreme, and that a sequence's bits do not depend on how many others
-a call has."""
+"""What lx_rotate, lx_causal_conv and lx_linear_attention keep of f32 where little things add up or sizes are extreme: slow decays, updates' weights,
+gates, infinities, far positions; and that a sequence's bits do not depend on how many others a call has."""
 
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -181,3 +182,35 @@ def test_silu_of_a_convolution(hip, out):
     assert got[-1].item() == float("inf")
     share = 2.0**-21 if out == F else 2.0**-17 + 2.0**-8 * 1.01
     assert bool(((got - want).abs()[:-1] <= share * want.abs()[:-1] + 2e-36).all())
+
+
+# pi to 60 places after the point.
+PI = Fraction(3141592653589793238462643383279502884197169399375105820974944, 10**60)
+
+
+def exact_turn(position, freq):
+    """cos and sin of position * freq, the angle reduced in whole numbers."""
+    angle = position * Fraction(freq)
+    left = float(angle - round(angle / (2 * PI)) * 2 * PI)
+    t = torch.tensor(left, dtype=torch.float64)
+    return t.cos().item(), t.sin().item()
+
+
+@pytest.mark.parametrize("interleaved", [0, 1])
+def test_rotation_at_far_positions(hip, interleaved):
+    """The angle is the product in 64 bits, off by 2^-53 twice: p f 2^-52; cosine and sine beside that by 2^-23 (the reduced angle's rounding, 2^-25, and the series');
+    two products and a sum 2^-22 of |a| + |b|."""
+    freq = torch.tensor([1.0, 0.7, 1e-2, 3.3e-5], dtype=F)
+    positions = [0, 1, 131071, 1 << 20, (1 << 26) + 5, (1 << 30) - 1, (1 << 31) - 1, -(1 << 31), -77777777]
+    T, rot = len(positions), 8
+    x = torch.randn(T, rot, generator=torch.Generator().manual_seed(1))
+    y = torch.full((T, rot), UNTOUCHED, device="cuda")
+    hip("rotate", x.cuda(), F32, rot, y, F32, rot, None, torch.tensor(positions, dtype=torch.int32).cuda(), freq.cuda(), 1.0, rot, interleaved, T, 1, rot)
+    got = y.double().cpu()
+    for t, position in enumerate(positions):
+        for i in range(rot // 2):
+            c, s = exact_turn(position, freq[i].item())
+            at = (2 * i, 2 * i + 1) if interleaved else (i, i + rot // 2)
+            a, b = x[t, at[0]].item(), x[t, at[1]].item()
+            bound = (abs(a) + abs(b)) * (abs(position * freq[i].item()) * 2.0**-52 + 2.0**-23 + 2.0**-22)
+            assert abs(got[t, at[0]].item() - (a * c - b * s)) <= bound and abs(got[t, at[1]].item() - (b * c + a * s)) <= bound, (position, i)

@@ -100,7 +100,9 @@ __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 3) linear_step_kernel(co
     u32x4 ks[ROWS / 8], qs[ROWS / 8];
 #pragma unroll
     for (int r = 0; r < ROWS / 8; ++r) ks[r] = row0 + 8 * r < p.dk ? key[r] : u32x4{}, qs[r] = row0 + 8 * r < p.dk ? query[r] : u32x4{};
-    const float fade = of_token(fades, i), left = of_token(lefts, i), weight = of_token(weights, i);
+    float fade = of_token(fades, i);
+    const float left = of_token(lefts, i), weight = of_token(weights, i);
+    asm("s_nop 1" : "+s"(fade));  // a lane's value read into a scalar: two cycles before the instructions below, which the compiler does not look into
     const f32x4 raw = four_of(value), z = four_of(gate), v = raw * weight;
     if (i + 1 < rows) ask(i + 1);
     constexpr int kSums = COLS == 8 && ROWS > 8 ? 2 : 1;

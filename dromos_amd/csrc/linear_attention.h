@@ -46,7 +46,7 @@ __device__ __forceinline__ float quick_expm1(float x) {
   return d == 0.0f ? x : d * x * __builtin_amdgcn_rcpf(__builtin_amdgcn_logf(e) * 0.693147181f);
 }
 
-// e^log in two parts: rounded, near 1, it is off to the same side time after time. The first is rounded down and the second above nothing, 2^-126 at least, so that the state's
+// e^log in two parts: rounded, near 1, it is off to the same side time after time. The first is rounded down and the second above nothing, 2^-149 at least, so that the state's
 // products with both have one sign and an infinite one stays what it is.
 struct Fade {
   float high, low;
@@ -56,7 +56,7 @@ __device__ __forceinline__ Fade fade_from(float high, float low) {
     const float below = __int_as_float(__float_as_int(high) - 1);
     low += high - below, high = below;
   }
-  return {high, high > 0.0f ? fmaxf(low, 0x1p-126f) : 0.0f};
+  return {high, high > 0.0f ? fmaxf(low, 0x1p-149f) : 0.0f};
 }
 __device__ __forceinline__ Fade fade_of(float log) {
   const float less = quick_expm1(log), high = 1.0f + less;

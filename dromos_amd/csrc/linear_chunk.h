@@ -161,7 +161,7 @@ struct Tokens {
   float update[kChunk];  // e^{G_63 - G_j} b_j
   float seen[kChunk];    // scale e^{G_i}
   float fade;            // e^{G_63}, and what its rounding left of the chunks before
-  float left;            // what its own rounding leaves, for a state that no further chunk of the call follows
+  float left;            // what its own rounding leaves, of a call's last chunk: no further one follows the state; next to nothing otherwise
   float whole;           // the logarithm of e^{G_63}
   int quick;
 };
@@ -337,10 +337,10 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
     const Fade fade = fade_of(whole);
     const float more = __builtin_fmaf(fade.high, carried, fade.low), factor = fade.high + more;
     const float left = more - (factor - fade.high);
-    const Fade last = fade_from(factor, left);
+    const Fade last = fade_from(factor, (chunk + 1) * kChunk < rows ? 0.0f : left);
     carried = left * __builtin_amdgcn_rcpf(factor);
     if (!(fabsf(carried) < 1.0f)) carried = 0.0f;
-    if (lane == 0) t.whole = whole, t.fade = (chunk + 1) * kChunk < rows ? factor : last.high, t.left = last.low;
+    if (lane == 0) t.whole = whole, t.fade = last.high, t.left = last.low;
   };
   if (counts) ask_decay(0);
 
@@ -756,20 +756,26 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
         }
         split_eight<false>(x, scaled_v[k % 2]);
       };
-      // In front of the products' first operands: behind them, the branch costs registers that are not there (45 spilled, 184 us for the 4096 tokens).
-      if (OUT && !more) {
-        const float left = t.left;
-#pragma unroll
-        for (int x = 0; x < kRows / 32; ++x)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) state[x][e] = __builtin_fmaf(state[x][e], fade, state[x][e] * left);
-      } else {
-#pragma unroll
-        for (int x = 0; x < kRows / 32; ++x) state[x] *= fade;
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      const float left = t.left;
       __builtin_amdgcn_s_setprio(1);
       ready(0);
+      // A branch around the second factor, or the compiler's own sum, costs registers that are not there (45 spilled, 184 us for the 4096 tokens): always, in place.
+#pragma unroll
+      for (int x = 0; x < kRows / 32; ++x) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if constexpr (OUT) {
+            float in = state[x][e];
+            const float rest = in * left;  // and by this it is known to be there
+            asm("v_fma_f32 %0, %0, %1, %2" : "+v"(in) : "v"(fade), "v"(rest));
+            state[x][e] = in;
+          } else {
+            state[x][e] *= fade;
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (OUT) asm volatile("s_nop 1");  // products do not wait for what they are not told of
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k) {

@@ -69,6 +69,16 @@ def test_slow_decays_of_many_short_calls(hip, rows, pieces):
     assert apart.abs().max().item() <= 2.0**-22 * -whole + 2.0**-19
 
 
+@pytest.mark.parametrize("rows", [1, 6, 7, 64, 300])
+def test_strong_decays_of_a_state(hip, rows):
+    """One factor, or some, down to the smallest normal number: each right to 2^-22 (an exponential and its correction) and a rounding of the state, of a token, or of a chunk or a
+    part. A chunk's logarithm is a sum, a product and a part's sum, each of 24 bits: 3 2^-24 of itself."""
+    for log in (-0.3, -0.6, -5.0, -40.0, -80.0, -86.5):
+        f = Fading(hip, rows, log / rows, 3)
+        f.call()
+        assert f.errors(rows).abs().max().item() <= (2.0**-22 + 2.0**-24) * (rows if rows <= 6 else (rows + 63) // 64) + (3 * 2.0**-24 * -log if rows > 6 else 0)
+
+
 def relative(got, want):
     errors = got.double().cpu() / want - 1
     return errors.square().mean().sqrt().item(), errors.abs().max().item()

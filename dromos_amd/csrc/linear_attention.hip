@@ -7,9 +7,10 @@ namespace {
 
 constexpr int kMaxDk = 256, kMaxDv = 512, kMaxHeads = 4096;
 constexpr int kMaxStride = 1 << 22;  // values: rows of a chunk are told apart in 31 bits
-// Rows of a sequence that go token by token; from there on by chunks, whose products cost the same for one row and 64. 128 heads of 128 by 64, by tokens and by a chunk: 8
-// sequences of 4 rows 17.2 us and 18.8, of 8 24.5 and 19.2, of 16 37.6 and 20.7; 64 sequences of 4 105 and 132, of 8 139 and 136; one sequence of 32 heads of 128 by
-// 128, 4 rows 7.0 and 11.3, 8 rows 10.0 and 11.3, 12 rows 13.0 and 11.3.
+// Rows of a sequence that go token by token; from there on by chunks, whose products cost the same for one row and 64. The two cross at 5 rows where the states of some sequences
+// fill the device, at 9 where one does not or where many are bound by their bytes: one number between them, so that a token's roundings go by max_rows alone. By tokens and by a
+// chunk, 128 heads of 128 by 64: 8 sequences of 4 rows 17.4 us and 19.6, of 6 21.0 and 19.7, of 8 24.5 and 19.8, of 16 38.5 and 20.8; 64 sequences of 4 103 and 140, of 8 138 and
+// 145, of 12 175 and 148; one sequence of 32 heads of 128 by 128, 4 rows 7.2 and 11.6, 8 rows 10.3 and 11.6, 12 rows 13.5 and 11.6.
 constexpr int kMostSteps = 6;
 
 template <int COLS, int ROWS>
@@ -24,8 +25,8 @@ int launch_step(const LinearArgs& p, hipStream_t s) {
 
 int steps(const LinearArgs& p, hipStream_t s) {
   if (p.dk <= 64) return launch_step<8, 8>(p, s);
-  // 16 columns a wavefront where 32 leave the device short of wavefronts: one sequence of 32 heads of 128 by 128 4.4 us, 4.9 by 32; eight of 128 heads of 128 by 64,
-  // 2048 wavefronts of 32 columns, 17.6 us and 18.1 by 16.
+  // 16 columns a wavefront where 32 leave the device short of wavefronts (sums are made in the same order): one sequence of 32 heads of 128 by 128 4.0 us, 4.6 by 32; eight of 128
+  // heads of 128 by 64, 2048 wavefronts of 32 columns, 17.6 us and 18.1 by 16.
   const bool few = static_cast<int64_t>(p.b.seqs) * p.heads * ((p.dv + 31) / 32) < 4 * compute_units();
   if (p.dk <= 128) return few ? launch_step<4, 8>(p, s) : launch_step<8, 16>(p, s);
   return few ? launch_step<4, 16>(p, s) : launch_step<8, 32>(p, s);
@@ -38,22 +39,22 @@ struct Cut {
   int size, places;  // rows of a part; parts of long sequences there may be
 };
 
-constexpr int kLeastPart = 128;  // rows; five sequences of up to 611 rows of 12 heads 32.7 us, 43.2 by 256
+constexpr int kLeastPart = 128;  // rows; five sequences of up to 611 rows of 12 heads 33.8 us, 43.9 by 256
 // Of sequences of so many parts the outputs' kernel adds up what is in front of a part by itself; of more, where that would be most of what it reads, a kernel in between
-// runs through them once. 4096 tokens of 128 heads, 8 parts: 114 us and 128; eight sequences of up to 4 parts of 8 heads of 256 by 256: 123 and 150.
+// runs through them once. 4096 tokens of 128 heads, 8 parts: 128 us and 138; eight sequences of up to 4 parts of 8 heads of 256 by 256: 126 and 161.
 constexpr int kFewParts = 8;
 
 Cut cut_of(int T, int max_rows, int heads, int k_heads, int dk, int dv) {
   Cut c;
   const int group = heads / k_heads;
   // A head of 64 columns or fewer has two wavefronts, and a workgroup two such heads, if there are two that read the same keys (4096 tokens of 128 heads, 16 of
-  // them to a key head: 125 us, 167 by one head a workgroup); 256 keys' values are too many loads for two wavefronts.
+  // them to a key head: 128 us, 173 by one head a workgroup); 256 keys' values are too many loads for two wavefronts.
   c.teams = dv <= 64 && group > 1 ? 2 : 1;
   c.waves = dv <= 64 && (c.teams == 2 || dk <= 128) ? 2 : 4;
   c.across = c.teams > 1 ? (group + 1) / 2 : group * ((dv + 32 * c.waves - 1) / (32 * c.waves));
   // As many parts as two workgroups a unit of the device: a part costs a second look at its keys and values, but few of them end together. By one, two and four
-  // workgroups a unit: 4096 tokens of 128 heads 156, 131 and 169 us, 16384 of 16 heads 141, 136 and 155 us; eight prompts of up to 2048 of 8 heads of 256 by 256, of which
-  // a unit has one at a time, by one 134 us, by two 124.
+  // workgroups a unit: 4096 tokens of 128 heads 161, 128 and 173 us, 16384 of 16 heads 145, 134 and 168 us; eight prompts of up to 2048 of 8 heads of 256 by 256, of which
+  // a unit has one at a time, 135, 126 and 235 us.
   const int64_t places = 2 * static_cast<int64_t>(compute_units()), columns = static_cast<int64_t>(c.across) * k_heads;
   const int64_t even = (T * columns + places - 1) / places, size = (even + kChunk - 1) / kChunk * kChunk;
   c.size = static_cast<int>(size < kLeastPart ? kLeastPart : size);

@@ -6,7 +6,8 @@
 // Every exponent is a difference of sums at most 0, formed from sums in 64 bits (as two f32 each): nothing overflows, and near tokens lose nothing where the sums
 // are large. What is rounded to go into a product goes in as bf16 terms, a value, what its rounding left, and so on: three of the values that a state is made of
 // (24 bits; with two, states were right to 2.6e-6, with one to 2^-9, and what a state has lost goes on from chunk to chunk), and of the state and the weights where results
-// are f32; two of those where results are rounded to bf16, 2^-8 of them, in any case.
+// are f32; two of those, 2^-17 of them, where results are rounded to bf16, 2^-8 of them, in any case (one result in 400 to 2000 is another one, mostly its neighbour; three terms there
+// too: 4096 tokens 190 us in place of 135, 16384 tokens 146 and 137, the wide prompts 139 and 127).
 //
 // A wavefront owns 32 columns of a head's state in registers, all rows or (of more than 128 keys) one half of them, for the whole of a sequence's part. Its layout is what
 // makes that work: v_mfma_f32_32x32x16 leaves a lane with four neighbouring rows, and four others 8 further, of its column. Rows and columns are given to
@@ -14,7 +15,7 @@
 // so a lane's eight values are neighbours: the state is the next product's operand as it lies, an output's eight values are one
 // store. Products are transposed, out^T = S^T Q^T + V^T P^T, so that a row's factors are a lane's own.
 // Halves give each other what they have for the other's 32 tokens through LDS (a wavefront with all 256 rows leaves a SIMD to itself: eight prompts of up to 2048
-// of 8 heads of 256 by 256 168 us, 150 by halves).
+// of 8 heads of 256 by 256, with two terms throughout and a kernel between sums and outputs, 168 us, 150 by halves).
 //
 // Queries, keys and values of a chunk stand in LDS, read along rows (16 bytes a lane) and across (ds_read_tr16), units of 16 bytes swizzled so that both
 // fall on all banks. The weights P of a head are made once by its wavefronts, 32 x 32 tiles on and below the diagonal, and shared through
@@ -25,9 +26,9 @@
 // only), and this one starts from the sums in front of its part; where there are many, a kernel in between runs through them and leaves the state in front of every
 // part.
 //
-// What bounds it: a wavefront's vector arithmetic (terms, exponentials, gates: 1200 instructions a chunk) and its products (104, 3300 cycles), one after
-// another in each of the two wavefronts that a SIMD has registers for. 4096 tokens of 128 heads of 128 by 64, 16 to a key head: 124 - 132 us (devices differ; sums 38,
-// outputs 100), 16384 of 16 heads of 128 by 128 131 - 136 us (42, 15 in between, 80), eight prompts of up to 2048 of 8 heads of 256 by 256 122 us (44, 91).
+// What bounds it: a wavefront's vector arithmetic (terms, exponentials, gates: 1290 instructions a chunk) and its products (104, 3300 cycles), one after
+// another in each of the two wavefronts that a SIMD has registers for. 4096 tokens of 128 heads of 128 by 64, 16 to a key head: 127 - 135 us (devices differ; sums 37,
+// outputs 101), 16384 of 16 heads of 128 by 128 133 - 137 us (41, 16 in between, 81), eight prompts of up to 2048 of 8 heads of 256 by 256 126 us (44, 94).
 #pragma once
 
 #include <type_traits>
@@ -194,7 +195,9 @@ __device__ __forceinline__ void buffer_store(__amdgpu_buffer_rsrc_t b, unsigned 
 __device__ __forceinline__ int rows_bytes(int m, int64_t ld, int width, int size) { return m > 0 ? ((m - 1) * static_cast<int>(ld) + width) * size : 0; }
 
 // OUT: outputs and states; otherwise a part's sum of a long sequence only. PLAIN: bf16 that can be moved 16 bytes at a time, gates bf16 or
-// none (everything else in its own kernel: its loads and stores, a value at a time perhaps, would cost this one registers).
+// none (everything else in its own kernel: its loads and stores, a value at a time perhaps, would cost this one registers). Two wavefronts a SIMD, but for heads of 128 keys and up to 64
+// columns that share no keys: their workgroups of two wavefronts load twice as many keys a lane, 52 registers of which would be spilled. By one wavefront a SIMD and by two: 4096 tokens of 32
+// heads of 128 by 64 69 us and 106, 16384 of 8 heads of 128 by 48 79 and 116, four sequences of 512 of 16 heads 33 and 44, eight of up to 2048 59 and 100.
 template <int DK, int TW, int TEAMS, int HALVES, bool OUT, bool PLAIN, int TERMS>
 __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW * TEAMS * HALVES == 2 ? 1 : 2) linear_chunk_kernel(const ChunkArgs c) {
   using L = ChunkTiles<DK, TW, TEAMS, HALVES, TERMS>;
@@ -521,7 +524,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
           for (int e = 0; e < 8; ++e) v[e] = state[step / 2][step % 2 * 8 + e];
           split_eight<true>(v, held[now]);
         };
-        // A wavefront with products goes in front of one with vector arithmetic (here and below: 126.6 -> 124.3 us for the 4096 tokens).
+        // A wavefront with products goes in front of one with vector arithmetic (here and below: 126.6 us without for the 4096 tokens, 124.3 then).
         __builtin_amdgcn_s_setprio(1);
         ready(0);
         __builtin_amdgcn_sched_barrier(0);

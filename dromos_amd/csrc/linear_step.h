@@ -4,7 +4,7 @@
 // Bytes decide, so a state is read once and written once, in pieces that are whole lines, everything asked for before the first use: a
 // wavefront takes 4 COLS columns of one head's state (all its rows: no other wavefront is waited for), four columns a lane,
 // 64 / COLS parts of the rows. The columns' sums over the rows cross the lanes once a token. 64 sequences of a token, 128 heads of 128 by 64: 90.8 us, 5.0 TB/s, the
-// rate of a copy; 8 sequences of 5 drafted tokens 17.5 us, where a token's sums wait for the last one's state; one of 32 heads of 128 by 128 4.5 us, a launch and a
+// rate of a copy; 8 sequences of 5 drafted tokens 17.6 us, where a token's sums wait for the last one's state; one of 32 heads of 128 by 128 4.5 us, a launch and a
 // chain of loads.
 #pragma once
 
@@ -16,7 +16,8 @@ namespace dro {
 
 // COLS lanes side by side in a row of the state; ROWS rows of it a lane. Sums over the rows are made in the same order by four lanes of up to 16 rows and by eight of up to
 // 32, whose two halves are summed apart: which of them a call takes goes by the number of its sequences, and no sequence's bits may. PLAIN: queries, keys, values and gates bf16 that can be moved 16 bytes at
-// a time (everything else in its own kernel: the registers of its loads would be missing here).
+// a time (everything else in its own kernel: the registers of its loads would be missing here). f32 queries, keys and values are rounded to bf16 as by chunks, so that
+// a token is the same to either form, and as lx_gemm_w's BF16 math rounds its rows.
 template <int COLS, int ROWS, bool PLAIN>
 __global__ void __launch_bounds__(256, ROWS >= 32 ? 2 : 3) linear_step_kernel(const LinearArgs p) {
   static_assert(COLS == 4 || COLS == 8, "lanes of a row");

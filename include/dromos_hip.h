@@ -363,8 +363,9 @@ typedef struct {
  * q, k and v all bf16 or all f32 (rounded to bf16, as lx_gemm_w's BF16 math does), out f32 or bf16, apart from what is read (out that is q, k, v, gate or x is refused), row strides in elements, up to
  * 2^22; states f32 [count, heads, dk, dv], 16-byte aligned, or null. Calls of few rows a sequence go token by token in f32, longer ones by chunks of 64 tokens
  * on the matrix cores: f32 factors (weights of tokens, values times their decay, the state) enter products there as bf16 terms, three of them for
- * states and for f32 results (24 bits are kept), two for bf16 results (16 bits), and sums are f32. An infinity of a state stays one where keys and values are finite;
- * by chunks, results that see one, and states that an infinite value goes into, may be NaNs, in its column alone. Neither form's bits depend on the other
+ * states and for f32 results (24 bits are kept), two for bf16 results (16 bits), and sums are f32. An infinity of a state stays one where keys and values are
+ * finite, until the decays of a token, or of a chunk or part, leave nothing in f32 (below -87; 0 times it is a NaN, as of a state's NaN); by chunks, results that see one, and
+ * states that an infinite value goes into, may be NaNs, in its column alone. Neither form's bits depend on the other
  * sequences of the call; which form a call takes depends on max_rows, and where a long sequence is cut on T and the sizes. The workspace holds sums and states of
  * the parts of long sequences, 16-byte aligned, may hold garbage, and belongs to one call at a time; lx_linear_attention_workspace_bytes (0: none, may
  * be null) answers for the call of these sizes and for every one with no larger T. */

@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
     const Fade fade = fade_of(whole);
     const float more = __builtin_fmaf(fade.high, carried, fade.low), factor = fade.high + more;
     const float left = more - (factor - fade.high);
-    const Fade last = fade_from(factor, (chunk + 1) * kChunk < rows ? 0.0f : left);
+    const Fade last = fade_from(factor, OUT && (chunk + 1) * kChunk >= rows ? left : 0.0f);  // a part's sum takes the nearest factor alone
     carried = left * __builtin_amdgcn_rcpf(factor);
     if (!(fabsf(carried) < 1.0f)) carried = 0.0f;
     if (lane == 0) t.whole = whole, t.fade = last.high, t.left = last.low;

@@ -6,7 +6,7 @@
 // Every exponent is a difference of sums at most 0, formed from sums in 64 bits (as two f32 each): nothing overflows, and near tokens lose nothing where the sums
 // are large. What is rounded to go into a product goes in as bf16 terms, a value, what its rounding left, and so on: three of the values that a state is made of
 // (24 bits; with two, states were right to 2.6e-6, with one to 2^-9, and what a state has lost goes on from chunk to chunk), and of the state and the weights where results
-// are f32; two of those, 2^-17 of them, where results are rounded to bf16, 2^-8 of them, in any case (one result in 400 to 2000 is another one, mostly its neighbour; three terms there
+// are f32; two of those, 2^-17 of them, where results are rounded to bf16, 2^-8 of them, in any case (one result in 400 to 7000 is another one, mostly its neighbour; three terms there
 // too: 4096 tokens 190 us in place of 135, 16384 tokens 146 and 137, the wide prompts 139 and 127).
 //
 // A wavefront owns 32 columns of a head's state in registers, all rows or (of more than 128 keys) one half of them, for the whole of a sequence's part. Its layout is what
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
   // ---- the decays -----------------------------------------------------------------------------------------------------
   // A token a lane: asked for two chunks ahead, made ready one ahead, by the team's last wavefront.
   Tokens* const tokens = reinterpret_cast<Tokens*>(lds + L::kTokens) + 2 * team;
-  // The scale is part of the rows' factors, the skip of a row's weight of its own token.
+  // The scale is part of the rows' factors.
   const bool counts = mate == TW - 1 && half == HALVES - 1;
   const HeadDecay head_numbers = head_decay(p, head);
   uint32_t next_raw;
@@ -493,19 +493,6 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
           put_weights(block, g, v);
         }
       };
-      // The skip, added to the rows' weights of their own tokens.
-      auto add_skip = [&](int block) __attribute__((always_inline)) {
-        if (h != (n >> 2 & 1)) return;
-        asm volatile("" ::: "memory");  // written as other types
-        uint16_t* const at = reinterpret_cast<uint16_t*>(lds + block * L::kBlock + (to ^ 16 * (n >> 3)) + 8 * h + 2 * (n & 3));
-        float whole = 0.0f;
-#pragma unroll
-        for (int term = TERMS - 1; term >= 0; --term) whole += bf16_bits_to_f32(at[3 * L::kBlock / 2 * term]);
-        uint32_t parts[TERMS];
-        split_two<false>(whole + skip, 0.0f, parts);
-#pragma unroll
-        for (int term = 0; term < TERMS; ++term) at[3 * L::kBlock / 2 * term] = static_cast<uint16_t>(parts[term]);
-      };
       // What the rows see of the state, and the products of `kTiles` tiles of weights, which read the same queries; a step's operands are made ready one
       // ahead. `block`: the first tile (two: (0, 0) and (1, 0), of the same keys).
       auto see = [&](auto tiles, int block) __attribute__((always_inline)) {
@@ -580,7 +567,6 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
       } else {
         see(std::integral_constant<int, 0>(), 0);
       }
-      if (p.skip && makes && block != (kEach ? 1 : -1)) add_skip(block);
 #pragma unroll
       for (int i = 0; i < 2; ++i) out[i] *= t.seen[32 * i + n];
       if constexpr (HALVES > 1) {  // a half keeps the rows of its own number
@@ -682,6 +668,21 @@ __global__ void __launch_bounds__(kWave * TW * TEAMS * HALVES, DK == 128 && TW *
       if (some_odd) {
 #pragma unroll
         for (int k = 0; k < kChunk / 16; ++k) v[k] = values_across(k);
+      }
+      // The skip, as token by token (as part of a row's weight of its own token, it was two terms of a bf16 result: 4096 tokens 130 us in place of 131, one result in 2000 another one
+      // in place of one in 7000).
+      if (p.skip) {
+#pragma unroll
+        for (int i = 0; i < kOutTiles; ++i)
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            const u32x4 eight = __builtin_bit_cast(u32x4, eight_at(lds, L::kValues + tile_place<L::kValuePitch>(now(32 * (i + half) + n), 4 * wave + 2 * a + h)));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t pair = eight[e / 2];
+              out[i][8 * a + e] = __builtin_fmaf(skip, __uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16), out[i][8 * a + e]);
+            }
+          }
       }
       if constexpr (PLAIN) {
         const bool short_out = p.out_type == LX_BF16;

@@ -1,5 +1,5 @@
 """What lx_rotate, lx_causal_conv and lx_linear_attention keep of f32 where little things add up or sizes are extreme: slow decays, updates' weights,
-gates, infinities, far positions; and that a sequence's bits do not depend on how many others a call has."""
+gates, skips, infinities, far positions; and that a sequence's bits do not depend on how many others a call has."""
 
 import math
 from fractions import Fraction
@@ -77,6 +77,17 @@ def test_strong_decays_of_a_state(hip, rows):
         f = Fading(hip, rows, log / rows, 3)
         f.call()
         assert f.errors(rows).abs().max().item() <= (2.0**-22 + 2.0**-24) * (rows if rows <= 6 else (rows + 63) // 64) + (3 * 2.0**-24 * -log if rows > 6 else 0)
+
+
+def test_steps_of_any_width(hip):
+    """softplus(x) from 1e-7 to 20, as the first update of a state of ones: an exponential right to 2^-23 and a rounding, a logarithm to 2^-22, two more roundings."""
+    seqs, heads = 64, 64
+    m = Mixer(Rows([1] * seqs, [1] * seqs), heads, 1, 8, 8, "step", seed=1, bias=False, spare=0)
+    m.x = torch.linspace(-16, 20, seqs * heads).view(seqs, heads)
+    m.k, m.v = torch.ones(seqs, 8, dtype=BF), torch.ones(seqs, heads * 8, dtype=BF)
+    _, kept = m.run(hip)
+    want = torch.log1p(torch.exp(m.x.double()))[:, :, None, None]
+    assert ((kept.double().cpu() / want - 1).abs().max().item()) <= 2.0**-22 + 2.0**-23 + 3 * 2.0**-24
 
 
 def relative(got, want):
@@ -177,6 +188,18 @@ def test_gates_of_f32_results(hip, rows, gate):
     assert out[0, 5].item() == float("inf")
     out[0, 5] = want[0, 5] = 0.0
     assert bool(((out - want).abs() <= (2.0**-21 + 2.0**-23) * want.abs() + 2e-36).all())
+
+
+@pytest.mark.parametrize("rows", [3, 64, 300])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (256, 72)])
+def test_skips_of_bf16_results(hip, rows, dk, dv):
+    """Queries of zero: a result is the skip's product, rounded to f32 and to bf16. The first rounding, 2^-24, moves the second one where a product is as near to a border, whose
+    distances are 2^-8 or more: in 2^-15 of all. Twice that and a few."""
+    m = Mixer(Rows([rows], [rows]), 4, 2, dk, dv, "step", True, seed=rows)
+    m.q.zero_()
+    out, _ = m.run(hip)
+    want = (m.skip.double()[:, None] * m.v.double().view(rows, 4, dv)).view(rows, 4 * dv).to(BF)
+    assert (out.cpu() != want).sum().item() <= 2.0**-14 * out.numel() + 4
 
 
 @pytest.mark.parametrize("out", [F, BF])

@@ -26,9 +26,9 @@
 // only), and this one starts from the sums in front of its part; where there are many, a kernel in between runs through them and leaves the state in front of every
 // part.
 //
-// What bounds it: a wavefront's vector arithmetic (terms, exponentials, gates: 1290 instructions a chunk) and its products (104, 3300 cycles), one after
-// another in each of the two wavefronts that a SIMD has registers for. 4096 tokens of 128 heads of 128 by 64, 16 to a key head: 127 - 135 us (devices differ; sums 37,
-// outputs 101), 16384 of 16 heads of 128 by 128 133 - 137 us (41, 16 in between, 81), eight prompts of up to 2048 of 8 heads of 256 by 256 126 us (44, 94).
+// What bounds it: a wavefront's vector arithmetic (terms, exponentials, skips, gates: 1370 instructions a chunk) and its products (104, 3300 cycles), one after
+// another in each of the two wavefronts that a SIMD has registers for. 4096 tokens of 128 heads of 128 by 64, 16 to a key head: 128 - 135 us (devices differ; sums 38,
+// outputs 105), 16384 of 16 heads of 128 by 128 133 - 137 us (42, 16 in between, 82), eight prompts of up to 2048 of 8 heads of 256 by 256 126 us (43, 93).
 #pragma once
 
 #include <type_traits>
